@@ -35,6 +35,7 @@ extern "C" {
 #define B200_TYPE_Q5_0 6
 #define B200_TYPE_Q8_0 8
 #define B200_TYPE_I32  26
+#define B200_TYPE_BF16 30
 
 /* ---- block formats ---------------------------------------------------------------------------
  * ggml stores 32 weights per block: block_q5_0 = {f16 d; u8 qh[4]; u8 qs[16]} (22 B),
@@ -251,6 +252,109 @@ int b200_get_rows(int type, const void * table, int64_t nb_total_or_row_stride, 
 #define B200_TOPK_MAX 8
 typedef struct { int32_t n, k; float max, logsumexp; int32_t ids[B200_TOPK_MAX]; float vals[B200_TOPK_MAX]; } b200_topk_result;
 int b200_topk_rows(const float * const * rows, b200_topk_result * const * out, int n_rows, int64_t n, int k, void * stream);
+
+/* ---- beam search on the device, on a paged key/value cache ------------------------------------------------------
+ * whisper's beam search samples, sorts and copies caches on the host (whisper_sample_token_topk, whisper_full_with_state,
+ * src/whisper.cpp:5230-5430, 5880-6010: one decoder per beam, whisper_kv_cache_seq_cp for the caches).  The entry points
+ * below do the same work next to the logits.  They are defined by their formulas, not by a reference kernel: sums, softmax
+ * statistics and scores are held in 32 bits or more, and every result is independent of the order in which blocks run.
+ * None of them allocates, synchronises or keeps anything between calls; all may be captured into a graph.  Scratch memory
+ * comes from the caller (16-byte aligned); two calls that may overlap on the device need a scratch area each. */
+
+/* The next beams of every sequence.  Row r = sequence * n_beam + beam has n_vocab logits x (F32, F16 or BF16; nb_row bytes
+ * between rows) and an accumulated score.  Candidates are
+ *   of a live beam b   every token v that is not banned:  score[b] + x[v] - max(x) - log(sum(exp(x - max(x))))
+ *   of a done beam b   the one token eos, with score[b]
+ * and the n_beam best become the new beams, best first, ties towards the lower b * n_vocab + v.  Banned tokens (bit v of word
+ * v / 32; banned_stride words between the rows' masks, 0 = one mask for all) and NaN count as -inf logits; a candidate of
+ * score -inf or NaN is none, and a row whose score is that, or that is done, is not read.  The new beam is done when its parent
+ * was or its token is eos.  Where candidates run out: score -inf, token and parent -1, done 1.
+ * score_out / done_out may be score / done.  n_beam <= B200_BEAM_MAX, n_beam * ceil(n_vocab / 4096) <= 32768, any alignment
+ * of the rows that suits their type.  done, banned may be NULL. */
+#define B200_BEAM_MAX 32
+typedef struct {
+    const void * logits; int type; int64_t nb_row; int64_t n_vocab; int n_seq, n_beam;
+    const float * score; const uint8_t * done; int32_t eos;
+    const uint32_t * banned; int64_t banned_stride;
+    float * score_out; int32_t * token_out; int32_t * parent_out; uint8_t * done_out;    /* [n_seq * n_beam] each */
+    void * workspace; int64_t workspace_bytes;
+} b200_beam_select_args;
+int64_t b200_beam_select_workspace(int n_seq, int n_beam, int64_t n_vocab);
+int b200_beam_select(const b200_beam_select_args * a, void * stream);
+
+/* State that is kept per beam follows its parent, in place: for every outer index o of every block, the row_bytes bytes at
+ * base + o * nb_outer + (sequence * n_beam + b) * nb_row become those of row parent[sequence * n_beam + b] of the same
+ * sequence (any value outside 0..n_beam-1 leaves the row as it is).  Caches of all layers, token histories, any state with a
+ * row per beam.  Any alignment (16-byte aligned base and strides are fastest); rows must not overlap; at most 8 blocks. */
+typedef struct { void * base; int64_t n_outer, nb_outer, nb_row, row_bytes; } b200_beam_block;
+int b200_beam_reorder(const b200_beam_block * blocks, int n_blocks, const int32_t * parent, int n_seq, int n_beam, void * stream);
+
+/* A paged key/value cache.  The value of token t (0..page_size-1), head h, dimension i of page p in layer l lies at
+ * base + l * nb_layer + p * nb_page + t * nb_tok + h * nb_head + 2 * i  (bytes; F16 or BF16; all strides and both bases
+ * multiples of 16, so token-major and head-major pages are both possible).  head_dim is 64 or 128, page_size >= 1. */
+typedef struct {
+    void * k; void * v; int type, n_layer, n_pages, page_size, n_head_kv, head_dim;
+    int64_t nb_layer, nb_page, nb_tok, nb_head;
+} b200_page_pool;
+/* Who uses the pages: row i (a sequence, or a beam of one) holds lens[i] tokens in pages tables[i * table_stride + 0 ..
+ * ceil(lens[i] / page_size) - 1]; refs[p] counts the holders of page p over all rows (plus any holder of the caller's own),
+ * 0 = free.  At most 8192 rows; table_stride * page_size < 2^31. */
+typedef struct { int32_t * tables; int32_t * lens; int32_t * refs; int64_t n_rows, table_stride; } b200_page_state;
+int64_t b200_pages_workspace(int64_t n_rows, int64_t n_pages);
+
+/* Row i becomes the first keep[i] tokens of row parent[i], with room for n_new[i] more - fork (parent != i), truncate
+ * (keep < length), free (keep = n_new = 0), grow (n_new > 0), in any mix.  `from` is read, `to` (same n_rows and table_stride) is written;
+ * the two must not overlap (a program keeps two states and swaps them).  Whole pages are shared.  A partly filled last page that will be written
+ * (n_new > 0) stays where it is for one row only: if nobody else holds it, or, among several such rows and no other holder, for
+ * the first of them; the others get a new page with a copy of its keep[i] % page_size tokens, in every layer of the pool.  New
+ * pages are those free in `from`, lowest number first, row by row (within a row: first the copy, then the following pages);
+ * pages that become free here can be taken by the next call.  Table entries behind a row's last page are set to -1.
+ * parent NULL: every row is its own parent.  pool NULL: tables only; b200_pages_copy then makes the copies, for as many
+ * pools as the caller has (n_pages and page_size are needed, so they come with pool: pass k = v = NULL for tables only).
+ * status[0] (device): 0; the number of pages that are missing; or -1 (a parent, keep, n_new or table entry out of range: a
+ * row cannot keep more than its parent holds, nor grow beyond table_stride pages).  If it is not 0, `to` is a copy of `from` and
+ * nothing else happened.  status[1]: pages copied. */
+int b200_pages_update(const b200_page_pool * pool, const b200_page_state * from, const b200_page_state * to, const int32_t * parent,
+                      const int32_t * keep, const int32_t * n_new, int32_t * status, void * workspace, int64_t workspace_bytes, void * stream);
+
+/* With L pages in use, the i-th used page numbered L or more moves to the i-th free page below L.  `to` receives tables, lens
+ * and refs in the new numbers, remap[p] the new number of page p (-1: free) for holders that the tables do not show.  `from` and
+ * `to` must not overlap; the pages themselves move within the pool.  status as above ([0]: 0, or -1 for a table entry out of
+ * range or on a free page; [1]: pages moved). */
+int b200_pages_compact(const b200_page_pool * pool, const b200_page_state * from, const b200_page_state * to, int32_t * remap,
+                       int32_t * status, void * workspace, int64_t workspace_bytes, void * stream);
+
+/* Repeats the page copies of the last b200_pages_update / b200_pages_compact that used this workspace (same n_rows,
+ * n_pages and page_size) in another pool: one pool per layer, or a draft model's cache beside the main one. */
+int b200_pages_copy(const b200_page_pool * pool, int64_t n_rows, const void * workspace, int64_t workspace_bytes, void * stream);
+
+/* Attention of a chunk of new tokens over the paged cache, one token per sequence included (the single-token step).
+ * Sequence s has the query tokens q_start[s] .. q_start[s+1]-1 (n_new of them) and lens[s] tokens in its pages, the new ones
+ * last: query t stands at position p = lens[s] - n_new + t and attends to positions 0..p (causal), or to all lens[s] (causal
+ * = 0).  Query head h reads key/value head h / (n_head / n_head_kv).  q is F16 or BF16 like the pool, or F32; dst has q's type:
+ *   dst[tok][h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale * q.k_j - m),   lse[tok][h] = m + log(sum_j w_j)   (lse may be NULL)
+ * Scores and sums are 32-bit; for 16-bit q the weights w_j are rounded to the pool's type before the product with V, which
+ * adds at most half a step of that type relative to each weight, the size of the output's own rounding.  For F32 q nothing is rounded to fewer bits.  A query
+ * without a key gives zeros and lse -inf; a NaN or infinite value in a position that a query does not attend to has no effect on it.
+ * k_new / v_new (type of q, [n_tok][n_head_kv][head_dim] with strides nb_new_tok, nb_new_head) are first stored at their positions,
+ * rounded to the pool's type; NULL (both) if the pages hold them already.  nb_* in bytes, multiples of 16, and 16-byte
+ * aligned pointers.  max_new and max_len bound n_new and lens from above (device values beyond them, or beyond the tables, are cut
+ * off); n_tok = q_start[n_seq].  A table entry outside the pool reads as keys and values of zero and stores nothing. */
+typedef struct {
+    const void * q; int q_type; int64_t nb_q_tok, nb_q_head;
+    void * dst; int64_t nb_dst_tok, nb_dst_head;
+    const void * k_new; const void * v_new; int64_t nb_new_tok, nb_new_head;
+    int layer;
+    const int32_t * tables; int64_t table_stride; const int32_t * lens; const int32_t * q_start;
+    int64_t n_tok; int n_seq, n_head; int64_t max_new, max_len; int causal; float scale;
+    float * lse;
+    void * workspace; int64_t workspace_bytes;
+} b200_paged_attn_args;
+int64_t b200_paged_attn_workspace(const b200_page_pool * pool, const b200_paged_attn_args * a);
+int b200_paged_attn(const b200_page_pool * pool, const b200_paged_attn_args * a, void * stream);
+/* The store alone (prompts whose attention runs elsewhere, caches filled from another source); uses of *a: k_new .. q_start,
+ * n_tok, n_seq, max_new, max_len, and q_type as the type of k_new / v_new. */
+int b200_paged_store(const b200_page_pool * pool, const b200_paged_attn_args * a, void * stream);
 
 /* IM2COL 1-D, F16 output (ops.cpp:5784-5855): x f32 [IW, IC] (row stride bytes) ->
  * dst f16 [IC*KW, OW]. */

@@ -7,3 +7,4 @@ plus libb200_driver.so, a flat C wrapper over whisper.h used by the Python harne
 """
 from . import synth  # noqa: F401
 from .host import Whisper, kernels_lib, load_plugin, PKG_DIR, REF_DIR, HOST_DIR  # noqa: F401
+from .host import BeamSelectArgs, BeamBlock, PagePool, PageState, PagedAttnArgs  # noqa: F401

@@ -1,0 +1,421 @@
+// Beam search on the device: the next beams over (beam, vocabulary) and the reordering of per-beam state.
+// Counterpart on the host in the reference: whisper_sample_token_topk and the candidate sort of whisper_full_with_state
+// (src/whisper.cpp:5230-5430, 5880-6010), which scan and copy on the CPU.
+#include "b200_common.cuh"
+#include <cuda_bf16.h>
+
+// ---- selection -----------------------------------------------------------------------------------
+// score(b, v) = score[b] + (x - m) - log(sum exp(x - m)).  Within a row the order of the candidates is the order of the
+// logits, so a row's n_beam best logits are all it can contribute: pass 1 cuts every row into slices and leaves, per slice,
+// its maximum, its sum of exponentials and its n_beam best logits; pass 2 joins the slices of a sequence's rows and picks
+// the n_beam best of their sorted lists.  The logits are read once; what bounds pass 1 is that read, and at few rows the
+// latency of load -> maximum -> sum -> list.
+#define SEL_THREADS 256
+#define SEL_EPT     16                              // logits per thread, all in registers
+#define SEL_SLICE   (SEL_THREADS * SEL_EPT)
+#define SEL_LISTS   32768                           // slices of a sequence's rows that pass 2 can join (a byte of shared memory each)
+
+// order-preserving map of a float to an unsigned integer (larger float -> larger integer); 0 is left for "nothing"
+__device__ __forceinline__ uint32_t sel_key(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float sel_val(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+__device__ __forceinline__ unsigned long long sel_key(double x) {
+    const unsigned long long u = (unsigned long long) __double_as_longlong(x);
+    return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double sel_val(unsigned long long k) {
+    return __longlong_as_double((long long) ((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));
+}
+
+// The VEC consecutive logits of one thread, with the widest loads that the row's alignment allows.  Which thread sums which
+// logits does not depend on the alignment, so equal rows give equal bits wherever they lie.
+template <typename T, int VEC>
+__device__ __forceinline__ void sel_load(const T * p, int align, float (&x)[VEC]) {
+    static_assert(VEC * sizeof(T) == 16, "one 16-byte vector");
+    union { uint4 q; uint2 h[2]; uint32_t w[4]; T t[VEC]; } u;
+    if (align >= 16)      u.q = *(const uint4 *) p;
+    else if (align == 8)  { u.h[0] = ((const uint2 *) p)[0]; u.h[1] = ((const uint2 *) p)[1]; }
+    else if (align == 4)  { for (int i = 0; i < 4; ++i) u.w[i] = ((const uint32_t *) p)[i]; }
+    else                  { for (int i = 0; i < VEC; ++i) u.t[i] = p[i]; }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = (float) u.t[i];
+}
+
+struct SelSlices {            // workspace of a call: [rows][n_slice] maxima and sums, [rows][n_slice][n_beam] best logits
+    float * m; double * s; float * x; int32_t * v;
+};
+
+static __host__ __device__ inline int64_t sel_slices(int64_t n_vocab) { return (n_vocab + SEL_SLICE - 1) / SEL_SLICE; }
+
+static inline SelSlices sel_layout(void * ws, int64_t rows, int64_t n_slice, int n_beam, int64_t * bytes) {
+    const int64_t n = rows * n_slice;
+    SelSlices p;
+    char * b = (char *) ws;
+    p.s = (double *) b;            b += 8 * n;
+    p.m = (float *) b;             b += 4 * n;
+    p.x = (float *) b;             b += 4 * n * n_beam;
+    p.v = (int32_t *) b;           b += 4 * n * n_beam;
+    *bytes = b - (char *) ws;
+    return p;
+}
+
+__device__ __forceinline__ bool sel_row_live(const float * score, const uint8_t * done, int64_t row) {
+    return score[row] > -INFINITY && !(done && done[row]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SEL_THREADS)
+k_beam_scan(const char * logits, int64_t nb_row, int n_vocab, const float * score, const uint8_t * done,
+            const uint32_t * banned, int64_t banned_stride, int n_beam, SelSlices out) {
+    constexpr int VEC = 16 / sizeof(T), NV = SEL_EPT / VEC, NW = SEL_THREADS / 32;
+    chain_release();
+    chain_wait();
+    const int64_t row = blockIdx.x;
+    const int slice = blockIdx.y, n_slice = gridDim.y;
+    if (!sel_row_live(score, done, row)) return;
+    __shared__ float  s_m[NW];
+    __shared__ double s_s[NW];
+    __shared__ unsigned long long s_top[NW * B200_BEAM_MAX];
+    __shared__ unsigned long long s_cand[B200_BEAM_MAX * SEL_EPT];
+    __shared__ int s_n;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const T * x_row = (const T *) (logits + row * nb_row);
+    const int align = (uintptr_t) x_row & 15 ? (int) ((uintptr_t) x_row & (~(uintptr_t) x_row + 1)) : 16;   // 2, 4, 8 or 16
+    const int base = slice * SEL_SLICE;
+    if (tid == 0) s_n = 0;
+
+    float x[NV][VEC];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int e = base + (j * SEL_THREADS + tid) * VEC;
+        if (e + VEC <= n_vocab) sel_load<T, VEC>(x_row + e, align, x[j]);
+        else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[j][i] = e + i < n_vocab ? (float) x_row[e + i] : -INFINITY;
+        }
+    }
+    if (banned) {
+        const uint32_t * mask = banned + row * banned_stride;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = base + (j * SEL_THREADS + tid) * VEC;
+            if (e < n_vocab) {              // VEC divides 32 and e is a multiple of it: one word covers the vector
+                const uint32_t w = mask[e >> 5] >> (e & 31);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) if (w >> i & 1) x[j][i] = -INFINITY;
+            }
+        }
+    }
+    float m = -INFINITY;
+    int   mi = 0;                           // this thread's best logit: the lowest index among equals (indices ascend)
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            x[j][i] = x[j][i] >= -INFINITY ? x[j][i] + 0.0f : -INFINITY;      // no NaN, one zero
+            if (x[j][i] > m) { m = x[j][i]; mi = base + (j * SEL_THREADS + tid) * VEC + i; }
+        }
+    // the warp's n_beam best thread maxima, best first; their first one is the warp's maximum
+    uint32_t hi = m > -INFINITY ? sel_key(m) : 0, lo = hi ? ~(uint32_t) mi : 0;
+    for (int r = 0; r < n_beam; ++r) {
+        const uint32_t bh = __reduce_max_sync(0xffffffffu, hi);
+        const uint32_t bl = __reduce_max_sync(0xffffffffu, hi == bh ? lo : 0u);
+        if (lane == 0) {
+            s_top[r * NW + warp] = (unsigned long long) bh << 32 | bl;
+            if (r == 0) s_m[warp] = bh ? sel_val(bh) : -INFINITY;
+        }
+        if (hi == bh && lo == bl) hi = lo = 0;
+    }
+    __syncthreads();
+    float mx = s_m[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, s_m[w]);
+    const int64_t at = row * n_slice + slice;
+    if (mx == -INFINITY) {
+        if (tid == 0) { out.m[at] = -INFINITY; out.s[at] = 0.0; }
+        if (tid < n_beam) out.v[at * n_beam + tid] = -1;
+        return;
+    }
+    // sum of exp(x - mx): 16 terms per thread in f32, joined in f64
+    float se = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) se += x[j][i] == mx ? 1.0f : __expf(x[j][i] - mx);
+    double sd = se;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sd += __shfl_xor_sync(0xffffffffu, sd, o);
+    if (lane == 0) s_s[warp] = sd;
+    // the n_beam-th best of the thread maxima bounds the slice's n_beam best from below, and the threads that reach it
+    // (n_beam of them) hold all of those: at most n_beam * SEL_EPT logits are left to be sorted
+    unsigned long long bound = 0;
+    {
+        unsigned long long k0[NW];          // lane r holds the r-th best of every warp
+#pragma unroll
+        for (int w = 0; w < NW; ++w) k0[w] = lane < n_beam ? s_top[lane * NW + w] : 0;
+        for (int r = 0; r < n_beam; ++r) {
+            unsigned long long b = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) b = k0[w] > b ? k0[w] : b;
+            const uint32_t h = (uint32_t) (b >> 32), l = (uint32_t) b;
+            const uint32_t bh = __reduce_max_sync(0xffffffffu, h);
+            const uint32_t bl = __reduce_max_sync(0xffffffffu, h == bh ? l : 0u);
+            bound = (unsigned long long) bh << 32 | bl;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) if (k0[w] == bound) k0[w] = 0;
+        }
+    }
+    if (bound == 0) bound = 1;              // fewer candidates than beams: all that there are
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            if (x[j][i] > -INFINITY) {
+                const unsigned long long k = (unsigned long long) sel_key(x[j][i]) << 32 | ~(uint32_t) (base + (j * SEL_THREADS + tid) * VEC + i);
+                if (k >= bound) {
+                    const int p = atomicAdd(&s_n, 1);
+                    s_cand[p] = k;          // the order of arrival does not matter: they are ranked below
+                }
+            }
+        }
+    __syncthreads();
+    const int n = s_n;
+    for (int c = tid; c < n; c += SEL_THREADS) {
+        const unsigned long long k = s_cand[c];
+        int rank = 0;
+        for (int o = 0; o < n; ++o) rank += s_cand[o] > k;
+        if (rank < n_beam) {
+            out.x[at * n_beam + rank] = sel_val((uint32_t) (k >> 32));
+            out.v[at * n_beam + rank] = (int32_t) ~(uint32_t) k;
+        }
+    }
+    if (tid >= n && tid < n_beam) out.v[at * n_beam + tid] = -1;
+    if (tid == 0) {
+        double s = s_s[0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) s += s_s[w];
+        out.m[at] = mx; out.s[at] = s;
+    }
+}
+
+// One CTA per sequence.  The slices' sorted lists are the threads' (list l = beam * n_slice + slice belongs to thread l mod
+// blockDim): n_beam rounds of an arg-max over the lists' heads, each round one barrier.  Keys are (score as ordered 64-bit
+// integer, lowest beam * n_vocab + token).
+__global__ void __launch_bounds__(1024)
+k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam, int n_slice, int n_vocab, int eos,
+            float * score_out, int32_t * token_out, int32_t * parent_out, uint8_t * done_out) {
+    chain_release();
+    chain_wait();
+    extern __shared__ unsigned char s_head[];              // next entry of every list
+    __shared__ double s_score[B200_BEAM_MAX], s_m[B200_BEAM_MAX], s_log[B200_BEAM_MAX];
+    __shared__ uint8_t s_done[B200_BEAM_MAX], s_live[B200_BEAM_MAX];
+    __shared__ uint32_t s_hi[2][32], s_lo[2][32], s_ix[2][32];
+    const int64_t row0 = (int64_t) blockIdx.x * n_beam;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warp = blockDim.x >> 5, n_list = n_beam * n_slice;
+    for (int b = warp; b < n_beam; b += n_warp) {
+        const float sc = score[row0 + b];
+        const bool d = done && done[row0 + b], ok = sc > -INFINITY, live = ok && !d;
+        float m = -INFINITY;
+        double s = 0.0;
+        if (live) {
+            for (int j = lane; j < n_slice; j += 32) m = fmaxf(m, in.m[(row0 + b) * n_slice + j]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (m > -INFINITY)
+                for (int j = lane; j < n_slice; j += 32) {
+                    const float mj = in.m[(row0 + b) * n_slice + j];
+                    if (mj == m) s += in.s[(row0 + b) * n_slice + j];
+                    else if (mj > -INFINITY) s += in.s[(row0 + b) * n_slice + j] * exp((double) mj - (double) m);
+                }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        }
+        if (lane == 0) {
+            s_score[b] = sc; s_m[b] = m; s_log[b] = s > 0.0 ? log(s) : 0.0;
+            s_done[b] = d; s_live[b] = live && m > -INFINITY ? 1 : ok && d ? 2 : 0;
+        }
+    }
+    for (int l = tid; l < n_list; l += blockDim.x) s_head[l] = 0;
+    __syncthreads();
+
+    unsigned long long mine = 0;
+    uint32_t mine_ix = 0;                    // ~(b * n_vocab + v) of this thread's best head, 0: none
+    int mine_l = -1;
+    auto look = [&]() {                      // best head among this thread's lists
+        mine = 0; mine_ix = 0; mine_l = -1;
+        for (int l = tid; l < n_list; l += blockDim.x) {
+            const int b = l / n_slice, sl = l - b * n_slice, h = s_head[l];
+            double v; int tok;
+            if (s_live[b] == 1) {
+                if (h >= n_beam) continue;
+                const int64_t at = ((row0 + b) * n_slice + sl) * n_beam + h;
+                tok = in.v[at];
+                if (tok < 0) continue;
+                const double x = in.x[at];
+                v = s_score[b] + ((x == s_m[b] ? 0.0 : x - s_m[b]) - s_log[b]);
+                if (!(v > -INFINITY)) continue;
+            } else if (s_live[b] == 2 && sl == 0 && h == 0) {
+                tok = eos >= 0 && eos < n_vocab ? eos : 0;         // its place among equals; the token itself may be any number
+                v = s_score[b];
+            } else continue;
+            const unsigned long long k = sel_key(v + 0.0);         // one zero
+            const uint32_t ix = ~(uint32_t) (b * n_vocab + tok);
+            if (mine_l < 0 || k > mine || (k == mine && ix > mine_ix)) { mine = k; mine_ix = ix; mine_l = l; }
+        }
+    };
+    look();
+    for (int r = 0; r < n_beam; ++r) {
+        const uint32_t h = (uint32_t) (mine >> 32), l = (uint32_t) mine;
+        uint32_t bh = __reduce_max_sync(0xffffffffu, h);
+        uint32_t bl = __reduce_max_sync(0xffffffffu, h == bh ? l : 0u);
+        uint32_t bi = __reduce_max_sync(0xffffffffu, h == bh && l == bl ? mine_ix : 0u);
+        if (n_warp > 1) {
+            if (lane == 0) { s_hi[r & 1][warp] = bh; s_lo[r & 1][warp] = bl; s_ix[r & 1][warp] = bi; }
+            __syncthreads();
+            const uint32_t wh = lane < n_warp ? s_hi[r & 1][lane] : 0, wl = lane < n_warp ? s_lo[r & 1][lane] : 0, wi = lane < n_warp ? s_ix[r & 1][lane] : 0;
+            bh = __reduce_max_sync(0xffffffffu, wh);
+            bl = __reduce_max_sync(0xffffffffu, wh == bh ? wl : 0u);
+            bi = __reduce_max_sync(0xffffffffu, wh == bh && wl == bl ? wi : 0u);
+        }
+        const bool none = bh == 0 && bl == 0;
+        if (!none && mine_l >= 0 && mine == ((unsigned long long) bh << 32 | bl) && mine_ix == bi) {
+            const uint32_t flat = ~bi;
+            const int b = mine_l / n_slice;
+            const int tok = s_live[b] == 2 ? eos : (int) (flat - (uint32_t) b * (uint32_t) n_vocab);
+            score_out[row0 + r] = (float) sel_val(mine);
+            token_out[row0 + r] = tok;
+            parent_out[row0 + r] = b;
+            done_out[row0 + r] = s_done[b] || tok == eos;
+            ++s_head[mine_l];
+            look();
+        }
+        if (none && tid == 0) { score_out[row0 + r] = -INFINITY; token_out[row0 + r] = -1; parent_out[row0 + r] = -1; done_out[row0 + r] = 1; }
+    }
+}
+
+extern "C" int64_t b200_beam_select_workspace(int n_seq, int n_beam, int64_t n_vocab) {
+    if (n_seq < 0 || n_beam < 1 || n_beam > B200_BEAM_MAX || n_vocab < 1 || n_vocab >= (1ll << 31) || sel_slices(n_vocab) * n_beam > SEL_LISTS) return 0;
+    int64_t bytes;
+    sel_layout(nullptr, (int64_t) n_seq * n_beam, sel_slices(n_vocab), n_beam, &bytes);
+    return bytes;
+}
+
+extern "C" int b200_beam_select(const b200_beam_select_args * a, void * stream) {
+    if (!a || a->n_seq < 0 || a->n_beam < 1 || a->n_beam > B200_BEAM_MAX || a->n_vocab < 1 || a->n_vocab >= (1ll << 31)) return B200_ERR_ARG;
+    const int64_t rows = (int64_t) a->n_seq * a->n_beam, n_slice = sel_slices(a->n_vocab);
+    if (n_slice * a->n_beam > SEL_LISTS) return B200_ERR_ARG;
+    const int size = a->type == B200_TYPE_F32 ? 4 : a->type == B200_TYPE_F16 || a->type == B200_TYPE_BF16 ? 2 : 0;
+    if (!size || a->nb_row % size || a->nb_row < a->n_vocab * size || a->banned_stride < 0 || rows > 0x7fffffff) return B200_ERR_ARG;
+    if (a->n_seq == 0) return 0;
+    if (!a->logits || !a->score || !a->score_out || !a->token_out || !a->parent_out || !a->done_out || (uintptr_t) a->logits % size) return B200_ERR_ARG;
+    if (!a->workspace || (uintptr_t) a->workspace % 16 || a->workspace_bytes < b200_beam_select_workspace(a->n_seq, a->n_beam, a->n_vocab)) return B200_ERR_ARG;
+    int64_t bytes;
+    const SelSlices ws = sel_layout(a->workspace, rows, n_slice, a->n_beam, &bytes);
+    const cudaStream_t st = as_stream(stream);
+    const dim3 grid((unsigned) rows, (unsigned) n_slice);
+    auto scan = a->type == B200_TYPE_F32 ? k_beam_scan<float> : a->type == B200_TYPE_F16 ? k_beam_scan<__half> : k_beam_scan<__nv_bfloat16>;
+    cudaError_t e = launch_chained(scan, grid, dim3(SEL_THREADS), 0, st, (const char *) a->logits, a->nb_row, (int) a->n_vocab, a->score, a->done,
+                                   a->banned, a->banned_stride, a->n_beam, ws);
+    if (e != cudaSuccess) return (int) e;
+    B200_LAUNCHED();
+    const int64_t n_list = n_slice * a->n_beam;
+    const unsigned threads = (unsigned) (n_list >= 1024 ? 1024 : (n_list + 31) / 32 * 32);
+    e = launch_chained(k_beam_pick, dim3((unsigned) a->n_seq), dim3(threads), (size_t) n_list, st, ws, a->score, a->done, a->n_beam, (int) n_slice,
+                       (int) a->n_vocab, (int) a->eos, a->score_out, a->token_out, a->parent_out, a->done_out);
+    if (e != cudaSuccess) return (int) e;
+    B200_RETURN_LAST();
+}
+
+// ---- reordering ----------------------------------------------------------------------------------
+// A thread owns one column (up to 16 bytes at the same offset of every row of a sequence): it loads the columns of all
+// parents and only then stores, so the move is in place without a second buffer, and a beam that follows itself costs
+// nothing.  Bound by memory: rows that change are written once, their parents read once (a parent of several beams comes
+// from L1 the second time).
+#define REORDER_THREADS 256
+#define REORDER_BLOCKS  8
+struct ReorderBlock { char * base; int64_t nb_outer, nb_row, row_bytes, first; unsigned tiles, n_outer; int vec; };
+struct ReorderArgs { ReorderBlock b[REORDER_BLOCKS]; int n; };
+
+template <typename V, int NB>
+__device__ __forceinline__ void reorder_column(char * col, int64_t nb_row, int64_t left, const int (&p)[NB], int n_beam) {
+    V v[NB];
+    if (left >= (int64_t) sizeof(V)) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) if (b < n_beam && p[b] != b) v[b] = *(const V *) (col + p[b] * nb_row);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) if (b < n_beam && p[b] != b) *(V *) (col + b * nb_row) = v[b];
+    } else {                                   // the end of a row that is no multiple of the vector
+        for (int64_t i = 0; i < left; ++i) {
+            unsigned char c[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) if (b < n_beam && p[b] != b) c[b] = ((const unsigned char *) col)[p[b] * nb_row + i];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) if (b < n_beam && p[b] != b) ((unsigned char *) col)[b * nb_row + i] = c[b];
+        }
+    }
+}
+
+template <int NB>
+__global__ void __launch_bounds__(REORDER_THREADS)
+k_beam_reorder(const __grid_constant__ ReorderArgs a, const int32_t * parent, int n_seq, int n_beam) {
+    chain_release();
+    chain_wait();
+    int k = 0;
+    while (k + 1 < a.n && (int64_t) blockIdx.x >= a.b[k + 1].first) ++k;
+    const ReorderBlock & blk = a.b[k];
+    int64_t r = (int64_t) blockIdx.x - blk.first;
+    const unsigned tile = (unsigned) (r % blk.tiles); r /= blk.tiles;
+    const int seq = (int) (r % n_seq);
+    const int64_t outer = r / n_seq;
+    int p[NB];
+    bool any = false;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        p[b] = b;
+        if (b < n_beam) {
+            const int q = parent[(int64_t) seq * n_beam + b];
+            if (q >= 0 && q < n_beam) p[b] = q;
+            any |= p[b] != b;
+        }
+    }
+    if (!any) return;
+    const int64_t off = ((int64_t) tile * REORDER_THREADS + threadIdx.x) * blk.vec, left = blk.row_bytes - off;
+    if (left <= 0) return;
+    char * col = blk.base + outer * blk.nb_outer + (int64_t) seq * n_beam * blk.nb_row + off;
+    if (blk.vec == 16)     reorder_column<uint4, NB>(col, blk.nb_row, left, p, n_beam);
+    else if (blk.vec == 4) reorder_column<uint32_t, NB>(col, blk.nb_row, left, p, n_beam);
+    else                   reorder_column<unsigned char, NB>(col, blk.nb_row, left, p, n_beam);
+}
+
+extern "C" int b200_beam_reorder(const b200_beam_block * blocks, int n_blocks, const int32_t * parent, int n_seq, int n_beam, void * stream) {
+    if (n_blocks < 0 || n_blocks > REORDER_BLOCKS || n_seq < 0 || n_beam < 1 || n_beam > B200_BEAM_MAX || (n_blocks && !blocks)) return B200_ERR_ARG;
+    ReorderArgs a = {};
+    int64_t ctas = 0;
+    for (int i = 0; i < n_blocks; ++i) {
+        const b200_beam_block & s = blocks[i];
+        if (s.n_outer < 0 || s.row_bytes < 0 || s.n_outer > 0x7fffffff || s.row_bytes > (1ll << 40)) return B200_ERR_ARG;
+        if (s.n_outer == 0 || s.row_bytes == 0 || n_seq == 0 || n_beam == 1) continue;
+        const int64_t rows = (int64_t) n_seq * n_beam;
+        if (!s.base || s.nb_row < s.row_bytes || s.nb_row > (1ll << 40) / rows || s.nb_outer < 0 || s.nb_outer > (1ll << 50) / s.n_outer) return B200_ERR_ARG;
+        if (s.n_outer > 1 && s.nb_outer < (rows - 1) * s.nb_row + s.row_bytes &&          // rows inside an outer step, or outer steps inside a row
+            (s.nb_outer < s.row_bytes || s.nb_row < (s.n_outer - 1) * s.nb_outer + s.row_bytes)) return B200_ERR_ARG;
+        const uintptr_t bits = (uintptr_t) s.base | (uintptr_t) s.nb_row | (s.n_outer > 1 ? (uintptr_t) s.nb_outer : 0);
+        ReorderBlock & d = a.b[a.n++];
+        d.base = (char *) s.base; d.nb_outer = s.nb_outer; d.nb_row = s.nb_row; d.row_bytes = s.row_bytes; d.first = ctas;
+        d.vec = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+        d.n_outer = (unsigned) s.n_outer;
+        const int64_t tiles = (s.row_bytes + (int64_t) d.vec * REORDER_THREADS - 1) / ((int64_t) d.vec * REORDER_THREADS);
+        if (tiles > 0x7fffffff) return B200_ERR_ARG;
+        d.tiles = (unsigned) tiles;
+        if (tiles * s.n_outer > 0x7fffffff || tiles * s.n_outer * n_seq > 0x7fffffff - ctas) return B200_ERR_ARG;
+        ctas += tiles * s.n_outer * n_seq;
+    }
+    if (ctas == 0) return 0;
+    if (!parent) return B200_ERR_ARG;
+    auto k = n_beam <= 4 ? k_beam_reorder<4> : n_beam <= 8 ? k_beam_reorder<8> : n_beam <= 16 ? k_beam_reorder<16> : k_beam_reorder<32>;
+    const cudaError_t e = launch_chained(k, dim3((unsigned) ctas), dim3(REORDER_THREADS), 0, as_stream(stream), a, parent, n_seq, n_beam);
+    if (e != cudaSuccess) return (int) e;
+    B200_RETURN_LAST();
+}

@@ -26,6 +26,40 @@ _kernels = None
 _drivers = {}
 
 
+class BeamSelectArgs(C.Structure):
+    """b200_beam_select_args of include/b200_whisper.h"""
+    _fields_ = [("logits", C.c_void_p), ("type", C.c_int), ("nb_row", C.c_int64), ("n_vocab", C.c_int64), ("n_seq", C.c_int), ("n_beam", C.c_int),
+                ("score", C.c_void_p), ("done", C.c_void_p), ("eos", C.c_int32), ("banned", C.c_void_p), ("banned_stride", C.c_int64),
+                ("score_out", C.c_void_p), ("token_out", C.c_void_p), ("parent_out", C.c_void_p), ("done_out", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class BeamBlock(C.Structure):
+    """b200_beam_block of include/b200_whisper.h"""
+    _fields_ = [("base", C.c_void_p), ("n_outer", C.c_int64), ("nb_outer", C.c_int64), ("nb_row", C.c_int64), ("row_bytes", C.c_int64)]
+
+
+class PagePool(C.Structure):
+    """b200_page_pool of include/b200_whisper.h"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("n_layer", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("n_head_kv", C.c_int), ("head_dim", C.c_int), ("nb_layer", C.c_int64), ("nb_page", C.c_int64), ("nb_tok", C.c_int64), ("nb_head", C.c_int64)]
+
+
+class PageState(C.Structure):
+    """b200_page_state of include/b200_whisper.h"""
+    _fields_ = [("tables", C.c_void_p), ("lens", C.c_void_p), ("refs", C.c_void_p), ("n_rows", C.c_int64), ("table_stride", C.c_int64)]
+
+
+class PagedAttnArgs(C.Structure):
+    """b200_paged_attn_args of include/b200_whisper.h"""
+    _fields_ = [("q", C.c_void_p), ("q_type", C.c_int), ("nb_q_tok", C.c_int64), ("nb_q_head", C.c_int64),
+                ("dst", C.c_void_p), ("nb_dst_tok", C.c_int64), ("nb_dst_head", C.c_int64),
+                ("k_new", C.c_void_p), ("v_new", C.c_void_p), ("nb_new_tok", C.c_int64), ("nb_new_head", C.c_int64), ("layer", C.c_int),
+                ("tables", C.c_void_p), ("table_stride", C.c_int64), ("lens", C.c_void_p), ("q_start", C.c_void_p),
+                ("n_tok", C.c_int64), ("n_seq", C.c_int), ("n_head", C.c_int), ("max_new", C.c_int64), ("max_len", C.c_int64),
+                ("causal", C.c_int), ("scale", C.c_float), ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 def kernels_lib() -> C.CDLL:
     """libb200_kernels.so with argument types set for the entry points used from Python."""
     global _kernels
@@ -36,6 +70,20 @@ def kernels_lib() -> C.CDLL:
         lib = C.CDLL(path)
         lib.b200_launch_count.restype = C.c_int64
         lib.b200_version.restype = C.c_char_p
+        vp, ci, i64 = C.c_void_p, C.c_int, C.c_int64
+        pool, state, attn = C.POINTER(PagePool), C.POINTER(PageState), C.POINTER(PagedAttnArgs)
+        lib.b200_beam_select_workspace.argtypes = [ci, ci, i64]
+        lib.b200_beam_select.argtypes = [C.POINTER(BeamSelectArgs), vp]
+        lib.b200_beam_reorder.argtypes = [C.POINTER(BeamBlock), ci, vp, ci, ci, vp]
+        lib.b200_pages_workspace.argtypes = [i64, i64]
+        lib.b200_pages_update.argtypes = [pool, state, state, vp, vp, vp, vp, vp, i64, vp]
+        lib.b200_pages_compact.argtypes = [pool, state, state, vp, vp, vp, i64, vp]
+        lib.b200_pages_copy.argtypes = [pool, i64, vp, i64, vp]
+        lib.b200_paged_attn_workspace.argtypes = [pool, attn]
+        lib.b200_paged_attn.argtypes = [pool, attn, vp]
+        lib.b200_paged_store.argtypes = [pool, attn, vp]
+        for f in ("b200_beam_select_workspace", "b200_pages_workspace", "b200_paged_attn_workspace"):
+            getattr(lib, f).restype = i64
         _kernels = lib
     return _kernels
 

@@ -13,7 +13,7 @@ struct PaArgs {
     const char * k; const char * v; int64_t nb_page, nb_tok, nb_head;
     const int32_t * tables; int64_t table_stride; const int32_t * lens; const int32_t * q_start;
     float * lse;
-    float * part;                   // [split][n_tok * n_head] x (head_dim + 2): sums, maximum, sum of weights
+    float * part;                   // [split][n_tok * n_head] x (head_dim + 4): sums, maximum, sum of weights, pad
     int64_t n_tok, max_len;
     int n_pages, page_size, n_head, n_head_kv, group, max_new, causal, n_split, chunk;
     float scale_log2;               // scale * log2(e): weights are powers of two
@@ -89,119 +89,336 @@ k_paged_store(PaArgs a, PaNew x, int vec_head) {
     }
 }
 
-// ---- attention, one key per lane -----------------------------------------------------------------
-// A CTA takes 8 rows (a row = one query token of one query head; rows of a key/value head are numbered token * group + head in
-// group) of one sequence and key/value head, over one split of the keys; its four warps take every fourth block of 32 keys.
-// Scores: a lane owns a key, the queries come from shared memory.  Products with V: a lane owns head_dim / 32 dimensions.
-// Running maximum and sum per row; the warps, then the splits, are joined at the end.
-#define PA_ROWS 8
+// ---- attention of few rows, and of f32 queries ---------------------------------------------------
+// A row is one query token of one query head; the rows of a key/value head are numbered token * group + head in group.  A CTA
+// takes 16 rows of one sequence and key/value head over one split of the keys - the 16 rows of an mma.sync m16n8k16 - and each of
+// its four warps streams every fourth block of 32 keys through its own shared-memory ring (two blocks deep, K and V separate
+// cp.async groups), so nothing in the loop waits for another warp.  Running maximum and sum per row; the warps are joined through
+// shared memory at the end, the splits by k_paged_join.  Bound by the stream of K and V: a block of 32 keys is 16 KB (head_dim
+// 128) for 64 MMAs.
+//
+// F32 queries: q and the weights are written as sums of two f16 (the second scaled by 2^11, q scaled by a power of two per row
+// so that no part underflows) or three bf16 values, which hold 22 or 24 bits of them, and each part is multiplied on the tensor
+// pipe; products of a block are added to the f32 accumulator by FADD, because the tensor pipe's own accumulation truncates.
+#define PA_ROWS  16
+#define PA_KEYS  32
+#define PA_WARPS 4
+#define PA_MIN_CHUNK 256
+
+template <typename T> struct PaPack;
+template <> struct PaPack<__half> {
+    static __device__ __forceinline__ uint32_t two(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *(const uint32_t *) &h; }
+    static __device__ __forceinline__ float2 back(uint32_t w) { return __half22float2(*(const __half2 *) &w); }
+    static __device__ __forceinline__ uint32_t odd(uint32_t w) { return ((w & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u); }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t * a, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <> struct PaPack<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t two(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *(const uint32_t *) &h; }
+    static __device__ __forceinline__ float2 back(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    static __device__ __forceinline__ uint32_t odd(uint32_t w) { return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u); }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t * a, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+// parts of an f32 operand; `lift` is the factor between one part and the next (1: none)
+template <typename Q, typename KV> struct PaParts { static constexpr int n = 1; static constexpr float lift = 1.0f; };
+template <> struct PaParts<float, __half>        { static constexpr int n = 2; static constexpr float lift = 2048.0f; };
+template <> struct PaParts<float, __nv_bfloat16> { static constexpr int n = 3; static constexpr float lift = 1.0f; };
+
+template <typename Q, typename KV>
+__device__ __forceinline__ void pa_parts(float a, float b, uint32_t (&out)[PaParts<Q, KV>::n]) {
+    using P = PaParts<Q, KV>;
+#pragma unroll
+    for (int i = 0; i < P::n; ++i) {
+        out[i] = PaPack<KV>::two(a, b);
+        const float2 f = PaPack<KV>::back(out[i]);
+        a = (a - f.x) * P::lift; b = (b - f.y) * P::lift;
+    }
+}
+
+__device__ __forceinline__ uint32_t pa_smem(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
+__device__ __forceinline__ void pa_cp16(uint32_t dst, const void * src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void pa_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void pa_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+__device__ __forceinline__ void pa_ldm(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3},[%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void pa_ldm_t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3},[%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+
+// keys that any of the 16 rows from row0 on sees, from the first key
+__device__ __forceinline__ int pa_reach(const PaArgs & a, const PaSeq & s, int row0) {
+    const int last_t = (min(row0 + PA_ROWS, s.n_new * a.group) - 1) / a.group;
+    return a.causal ? min(s.len, max(s.len - s.n_new + last_t + 1, 0)) : s.len;
+}
+
 template <typename Q, typename KV, int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(32 * PA_WARPS)
 k_paged_attn(PaArgs a) {
+    using P = PaPack<KV>;
+    constexpr int NP = PaParts<Q, KV>::n, NC = D / 8, KS = D / 16;      // parts, 16-byte chunks and MMA steps of a head
+    constexpr float LIFT = PaParts<Q, KV>::lift;
+    constexpr int BLOCK = PA_KEYS * D * 2;                              // bytes of a block of K or V
+    extern __shared__ __align__(16) char smem[];
     chain_release();
     chain_wait();
-    constexpr int DL = D / 32;
-    __shared__ float s_q[PA_ROWS][D];
-    __shared__ float s_p[4][PA_ROWS][32];
-    __shared__ float s_m[4][PA_ROWS], s_l[4][PA_ROWS];
-    __shared__ float s_o[4][PA_ROWS][D];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int seq = blockIdx.z / a.n_split, split = blockIdx.z % a.n_split, kvh = blockIdx.y, row0 = blockIdx.x * PA_ROWS;
     const PaSeq s = pa_seq(a, seq);
     const int n_rows = s.n_new * a.group;
     if (row0 >= n_rows) return;
-    const int last_t = (min(row0 + PA_ROWS, n_rows) - 1) / a.group;
-    const int reach = a.causal ? min(s.len, max(s.len - s.n_new + last_t + 1, 0)) : s.len;      // keys that any row of the tile sees
-    const int k0 = split * a.chunk, k1 = min(reach, k0 + a.chunk);
-    if (k0 >= k1 && !(split == 0)) return;               // an empty split: the join does not read it
-    for (int i = tid; i < PA_ROWS * D; i += 128) {
-        const int r = row0 + i / D, t = r / a.group, h = kvh * a.group + r % a.group;
-        s_q[i / D][i % D] = r < n_rows ? (float) ((const Q *) (a.q + (s.tok0 + t) * a.nb_q_tok + h * a.nb_q_head))[i % D] * a.scale_log2 : 0.0f;
-    }
-    int last[PA_ROWS];                                   // last key of every row
-#pragma unroll
-    for (int r = 0; r < PA_ROWS; ++r) last[r] = row0 + r >= n_rows ? -1 : a.causal ? s.len - s.n_new + (row0 + r) / a.group : s.len - 1;
-    __syncthreads();
-    float m[PA_ROWS], l[PA_ROWS], o[PA_ROWS][DL];
-#pragma unroll
-    for (int r = 0; r < PA_ROWS; ++r) { m[r] = -INFINITY; l[r] = 0.0f; for (int i = 0; i < DL; ++i) o[r][i] = 0.0f; }
+    const int k0 = split * a.chunk, k1 = min(pa_reach(a, s, row0), k0 + a.chunk);
+    if (k0 >= k1 && split != 0) return;                  // an empty split: the join does not read it
+
+    const char * kp = a.k + kvh * a.nb_head, * vp = a.v + kvh * a.nb_head;
     const int32_t * table = a.tables + seq * a.table_stride;
-    for (int kb = k0 + warp * 32; kb < k1; kb += 128) {
-        const int key = kb + lane;
-        int64_t at = -1;
-        if (key < k1) {
-            const int page = table[key / a.page_size];
-            if (page >= 0 && page < a.n_pages) at = page * a.nb_page + (key % a.page_size) * a.nb_tok + kvh * a.nb_head;
-        }
-        float sc[PA_ROWS] = {};
-        if (at >= 0) {
+    const uint32_t ring = pa_smem(smem) + warp * 4 * BLOCK;             // K0 K1 V0 V1
+    const int n_block = k1 > k0 ? (k1 - k0 + PA_KEYS - 1) / PA_KEYS : 0, n_mine = (n_block - warp + PA_WARPS - 1) / PA_WARPS;
+    auto key_of = [&](int i) { return k0 + (i * PA_WARPS + warp) * PA_KEYS + lane; };
+    auto page_of = [&](int i) { const int key = key_of(i); return i < n_mine && key < k1 ? table[key / a.page_size] : -1; };
+    auto at_of = [&](int i, int page) -> int64_t {       // this lane's key's place in the pool, -1: none
+        return page >= 0 && page < a.n_pages ? page * a.nb_page + (key_of(i) % a.page_size) * a.nb_tok : -1;
+    };
+    auto load = [&](int i, int64_t at, const char * base, uint32_t dst) {
+        if (i < n_mine) {
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-                float kx[8];
-                pa_unpack8<KV>(*(const uint4 *) (a.k + at + c * 16), kx);
-#pragma unroll
-                for (int r = 0; r < PA_ROWS; ++r)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sc[r] = fmaf(s_q[r][c * 8 + i], kx[i], sc[r]);
+            for (int c = 0; c < NC; ++c) {
+                const int x = c * 32 + lane, r = x / NC, ch = x % NC;
+                const int64_t off = __shfl_sync(0xffffffffu, at, r);
+                pa_cp16(dst + r * D * 2 + ((ch ^ (r & 7)) << 4), base + (off < 0 ? 0 : off + ch * 16), off >= 0);
             }
         }
-#pragma unroll
-        for (int r = 0; r < PA_ROWS; ++r) {
-            const float x = key < k1 && key <= last[r] ? sc[r] : -INFINITY;
-            float mx = x;
-#pragma unroll
-            for (int of = 16; of > 0; of >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, of));
-            const float m1 = fmaxf(m[r], mx), base = m1 == -INFINITY ? 0.0f : m1;
-            const float f = exp2f(m[r] - base), p = exp2f(x - base);
-            l[r] = l[r] * f + p;
-            m[r] = m1;
-#pragma unroll
-            for (int i = 0; i < DL; ++i) o[r][i] *= f;
-            s_p[warp][r][lane] = p;
-        }
-        __syncwarp();
-        const int n = min(32, k1 - kb);
-        for (int j = 0; j < n; ++j) {
-            const int64_t vat = __shfl_sync(0xffffffffu, at, j);
-            if (vat < 0) continue;
-            float vx[DL];
-#pragma unroll
-            for (int i = 0; i < DL; ++i) vx[i] = (float) ((const KV *) (a.v + vat))[lane * DL + i];
-#pragma unroll
-            for (int r = 0; r < PA_ROWS; ++r) {
-                if (kb + j > last[r]) continue;            // not 0 * v: v may be infinite or NaN where the row does not look
-                const float p = s_p[warp][r][j];
-#pragma unroll
-                for (int i = 0; i < DL; ++i) o[r][i] = fmaf(p, vx[i], o[r][i]);
-            }
-        }
-        __syncwarp();
+        pa_commit();
+    };
+    int64_t at_next;
+    {
+        const int p0 = page_of(0), p1 = page_of(1);
+        const int64_t at0 = at_of(0, p0), at1 = at_of(1, p1);
+        load(0, at0, kp, ring); load(0, at0, vp, ring + 2 * BLOCK);
+        load(1, at1, kp, ring + BLOCK); load(1, at1, vp, ring + 3 * BLOCK);
     }
+    int page_next = page_of(2);
+
+    // this lane's two rows: lane / 4 and lane / 4 + 8 of the tile
+    const int ra = row0 + (lane >> 2), rb = ra + 8;
+    const int last_a = ra >= n_rows ? -1 : a.causal ? s.len - s.n_new + ra / a.group : s.len - 1;
+    const int last_b = rb >= n_rows ? -1 : a.causal ? s.len - s.n_new + rb / a.group : s.len - 1;
+    const int first_last = a.causal ? s.len - s.n_new + row0 / a.group : s.len - 1;     // keys up to here: seen by every row
+    uint32_t qf[NP][KS][4];
+    float fa = a.scale_log2, fb = a.scale_log2;
+    {
+        const int ia = min(ra, n_rows - 1), ib = min(rb, n_rows - 1);
+        const Q * qa = (const Q *) (a.q + (s.tok0 + ia / a.group) * a.nb_q_tok + (kvh * a.group + ia % a.group) * a.nb_q_head) + (lane & 3) * 2;
+        const Q * qb = (const Q *) (a.q + (s.tok0 + ib / a.group) * a.nb_q_tok + (kvh * a.group + ib % a.group) * a.nb_q_head) + (lane & 3) * 2;
+        if constexpr (NP == 1) {
 #pragma unroll
-    for (int r = 0; r < PA_ROWS; ++r) {
+            for (int i = 0; i < KS; ++i) {
+                qf[0][i][0] = *(const uint32_t *) (qa + 16 * i);     qf[0][i][1] = *(const uint32_t *) (qb + 16 * i);
+                qf[0][i][2] = *(const uint32_t *) (qa + 16 * i + 8); qf[0][i][3] = *(const uint32_t *) (qb + 16 * i + 8);
+            }
+        } else {
+            float2 x[KS][4];
+            float ma = 0.0f, mb = 0.0f;
 #pragma unroll
-        for (int of = 16; of > 0; of >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], of);
-        if (lane == 0) { s_m[warp][r] = m[r]; s_l[warp][r] = l[r]; }
+            for (int i = 0; i < KS; ++i) {
+                x[i][0] = *(const float2 *) (qa + 16 * i);     x[i][1] = *(const float2 *) (qb + 16 * i);
+                x[i][2] = *(const float2 *) (qa + 16 * i + 8); x[i][3] = *(const float2 *) (qb + 16 * i + 8);
+                ma = fmaxf(fmaxf(ma, fmaxf(fabsf(x[i][0].x), fabsf(x[i][0].y))), fmaxf(fabsf(x[i][2].x), fabsf(x[i][2].y)));
+                mb = fmaxf(fmaxf(mb, fmaxf(fabsf(x[i][1].x), fabsf(x[i][1].y))), fmaxf(fabsf(x[i][3].x), fabsf(x[i][3].y)));
+            }
+            float sa = 1.0f, sb = 1.0f;
+            if constexpr (LIFT != 1.0f) {                // powers of two that bring the row's largest value to [1, 2)
 #pragma unroll
-        for (int i = 0; i < DL; ++i) s_o[warp][r][lane * DL + i] = o[r][i];
+                for (int o = 1; o < 4; o <<= 1) { ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, o)); mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o)); }
+                auto inverse = [](float m) { const int e = (int) (__float_as_uint(m) >> 23); return e == 0 || e == 255 ? 1.0f : __uint_as_float((uint32_t) max(1, 254 - e) << 23); };
+                sa = inverse(ma); sb = inverse(mb);
+                fa = a.scale_log2 / sa; fb = a.scale_log2 / sb;
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float f = j & 1 ? sb : sa;
+                    uint32_t w[NP];
+                    pa_parts<Q, KV>(x[i][j].x * f, x[i][j].y * f, w);
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) qf[n][i][j] = w[n];
+                }
+        }
+    }
+
+    float o[NC][4] = {}, ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
+    for (int i = 0; i < n_mine; ++i) {
+        const uint32_t kb = ring + (i & 1) * BLOCK, vb = kb + 2 * BLOCK;
+        const int key0 = k0 + (i * PA_WARPS + warp) * PA_KEYS;
+        at_next = at_of(i + 2, page_next);
+        page_next = page_of(i + 3);
+        pa_wait<3>();
+        __syncwarp();
+        // scores of 16 rows and 32 keys
+        float sc[4][4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float part[NP][4] = {};
+#pragma unroll
+            for (int h = 0; h < KS / 2; ++h) {
+                uint32_t b[4];
+                pa_ldm(b, kb + (8 * j + (lane & 7)) * D * 2 + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NP; ++n) { P::mma(part[n], qf[n][2 * h], b[0], b[1]); P::mma(part[n], qf[n][2 * h + 1], b[2], b[3]); }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float v = part[NP - 1][e];
+#pragma unroll
+                for (int n = NP - 2; n >= 0; --n) v = part[n][e] + v * (1.0f / LIFT);
+                sc[j][e] = v;
+            }
+        }
+        __syncwarp();
+        load(i + 2, at_next, kp, kb);
+        const bool edge = key0 + PA_KEYS - 1 > first_last || key0 + PA_KEYS > k1;
+        float xa = -INFINITY, xb = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                sc[j][e] *= fa; sc[j][e + 2] *= fb;
+                if (edge) {
+                    const int key = key0 + 8 * j + (lane & 3) * 2 + e;
+                    if (key >= k1 || key > last_a) sc[j][e] = -INFINITY;
+                    if (key >= k1 || key > last_b) sc[j][e + 2] = -INFINITY;
+                }
+                xa = fmaxf(xa, sc[j][e]); xb = fmaxf(xb, sc[j][e + 2]);
+            }
+#pragma unroll
+        for (int of = 1; of < 4; of <<= 1) { xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, of)); xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, of)); }
+        xa = fmaxf(xa, ma); xb = fmaxf(xb, mb);
+        const float ba = xa == -INFINITY ? 0.0f : xa, bb = xb == -INFINITY ? 0.0f : xb;
+        const float ca = exp2f(ma - ba), cb = exp2f(mb - bb);
+        ma = xa; mb = xb;
+        la *= ca; lb *= cb;
+        uint32_t pf[NP][2][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                sc[j][e] = exp2f(sc[j][e] - ba); sc[j][e + 2] = exp2f(sc[j][e + 2] - bb);
+                la += sc[j][e]; lb += sc[j][e + 2];
+            }
+            uint32_t w[NP];
+            pa_parts<Q, KV>(sc[j][0], sc[j][1], w);
+#pragma unroll
+            for (int n = 0; n < NP; ++n) pf[n][j >> 1][(j & 1) * 2] = w[n];
+            pa_parts<Q, KV>(sc[j][2], sc[j][3], w);
+#pragma unroll
+            for (int n = 0; n < NP; ++n) pf[n][j >> 1][(j & 1) * 2 + 1] = w[n];
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) { o[c][0] *= ca; o[c][1] *= ca; o[c][2] *= cb; o[c][3] *= cb; }
+        pa_wait<3>();
+        __syncwarp();
+        uint32_t odd = 0;
+#pragma unroll
+        for (int c = 0; c < NC / 2; ++c) {
+            float part[NP][2][4] = {};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t b[4];
+                pa_ldm_t(b, vb + (16 * h + (lane & 15)) * D * 2 + (((2 * c + (lane >> 4)) ^ (lane & 7)) << 4));
+                if (edge) {                               // 0 * v is not 0 where v is infinite or NaN: such values are taken out here
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) { const uint32_t x = P::odd(b[w]); odd |= x; b[w] &= ~x; }
+                }
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    if constexpr (NP == 1) { P::mma(o[2 * c], pf[0][h], b[0], b[1]); P::mma(o[2 * c + 1], pf[0][h], b[2], b[3]); }
+                    else { P::mma(part[n][0], pf[n][h], b[0], b[1]); P::mma(part[n][1], pf[n][h], b[2], b[3]); }
+                }
+            }
+            if constexpr (NP > 1) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float v = part[NP - 1][u][e];
+#pragma unroll
+                        for (int n = NP - 2; n >= 0; --n) v = part[n][u][e] + v * (1.0f / LIFT);
+                        o[2 * c + u][e] += v;
+                    }
+            }
+        }
+        if (edge && __any_sync(0xffffffffu, odd)) {       // ... and given back to the rows that see them
+            for (int j = 0; j < min(PA_KEYS, k1 - key0); ++j)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const KV * v = (const KV *) (smem + (vb - pa_smem(smem)) + j * D * 2 + ((c ^ (j & 7)) << 4)) + (lane & 3) * 2;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float x = (float) v[e];
+                        if (!(fabsf(x) < INFINITY)) {
+                            if (key0 + j <= last_a) o[c][e] += x;
+                            if (key0 + j <= last_b) o[c][e + 2] += x;
+                        }
+                    }
+                }
+        }
+        __syncwarp();
+        load(i + 2, at_next, vp, vb);
+    }
+    pa_wait<0>();
+#pragma unroll
+    for (int of = 1; of < 4; of <<= 1) { la += __shfl_xor_sync(0xffffffffu, la, of); lb += __shfl_xor_sync(0xffffffffu, lb, of); }
+    __syncthreads();
+    // join of the four warps: [warp][row] maxima and sums, [warp][row][D + 4] accumulators over the rings
+    float * sm = (float *) smem, * sl = sm + PA_WARPS * PA_ROWS, * so = sl + PA_WARPS * PA_ROWS;
+    constexpr int LD = D + 4;
+    {
+        const int wa = warp * PA_ROWS + (lane >> 2), wb = wa + 8;
+        if ((lane & 3) == 0) { sm[wa] = ma; sm[wb] = mb; sl[wa] = la; sl[wb] = lb; }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            *(float2 *) (so + wa * LD + c * 8 + (lane & 3) * 2) = make_float2(o[c][0], o[c][1]);
+            *(float2 *) (so + wb * LD + c * 8 + (lane & 3) * 2) = make_float2(o[c][2], o[c][3]);
+        }
     }
     __syncthreads();
-    for (int i = tid; i < PA_ROWS * D; i += 128) {
-        const int r = i / D, d = i % D, row = row0 + r;
-        if (row >= n_rows) break;
-        float mx = s_m[0][r];
-        for (int w = 1; w < 4; ++w) mx = fmaxf(mx, s_m[w][r]);
+    const int rows = min(PA_ROWS, n_rows - row0);
+    for (int i = tid; i < rows * (D / 4); i += 32 * PA_WARPS) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4, row = row0 + r;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) mx = fmaxf(mx, sm[w * PA_ROWS + r]);
         const float base = mx == -INFINITY ? 0.0f : mx;
-        float sum = 0.0f, acc = 0.0f;
-        for (int w = 0; w < 4; ++w) { const float f = exp2f(s_m[w][r] - base); sum += f * s_l[w][r]; if (f != 0.0f) acc += f * s_o[w][r][d]; }
+        float sum = 0.0f, x[4] = {};
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) {
+            const float f = exp2f(sm[w * PA_ROWS + r] - base);
+            sum += f * sl[w * PA_ROWS + r];              // NaN of a warp without a finite maximum stays NaN
+            if (f != 0.0f) {
+                const float4 v = *(const float4 *) (so + (w * PA_ROWS + r) * LD + d);
+                x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w;
+            }
+        }
         const int t = row / a.group, h = kvh * a.group + row % a.group;
         const int64_t out = (s.tok0 + t) * a.n_head + h;
         if (a.n_split == 1) {
-            ((Q *) (a.dst + (s.tok0 + t) * a.nb_dst_tok + h * a.nb_dst_head))[d] = (Q) (sum == 0.0f ? 0.0f : acc / sum);
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            char * dst = a.dst + (s.tok0 + t) * a.nb_dst_tok + h * a.nb_dst_head + d * sizeof(Q);
+            if constexpr (NP == 1) *(uint2 *) dst = make_uint2(P::two(x[0] * inv, x[1] * inv), P::two(x[2] * inv, x[3] * inv));
+            else *(float4 *) dst = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
             if (a.lse && d == 0) a.lse[out] = sum == 0.0f ? -INFINITY : mx * 0.69314718f + logf(sum);
         } else {
-            float * p = a.part + (split * a.n_tok * a.n_head + out) * (D + 2);
-            p[d] = acc;
+            float * p = a.part + (split * a.n_tok * a.n_head + out) * (D + 4);
+            *(float4 *) (p + d) = make_float4(x[0], x[1], x[2], x[3]);
             if (d == 0) { p[D] = mx; p[D + 1] = sum; }
         }
     }
@@ -221,11 +438,9 @@ k_paged_join(PaArgs a) {
         const int t = (int) (w / a.n_head), h = (int) (w - (int64_t) t * a.n_head);
         const int64_t out = (s.tok0 + t) * a.n_head + h;
         const int row = t * a.group + h % a.group, row0 = row / PA_ROWS * PA_ROWS;
-        const int last_t = (min(row0 + PA_ROWS, s.n_new * a.group) - 1) / a.group;
-        const int reach = a.causal ? min(s.len, max(s.len - s.n_new + last_t + 1, 0)) : s.len;
-        const int n = max(1, (reach + a.chunk - 1) / a.chunk);
-        const float * p = a.part + out * (D + 2);
-        const int64_t step = a.n_tok * a.n_head * (D + 2);
+        const int n = max(1, (pa_reach(a, s, row0) + a.chunk - 1) / a.chunk);
+        const float * p = a.part + out * (D + 4);
+        const int64_t step = a.n_tok * a.n_head * (D + 4);
         float mx = -INFINITY;
         for (int i = lane; i < n; i += 32) mx = fmaxf(mx, p[i * step + D]);
 #pragma unroll
@@ -269,12 +484,14 @@ static void pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a, in
     const int64_t group = a->n_head / p->n_head_kv;
     const int64_t new_max = a->max_new < a->n_tok ? a->max_new : a->n_tok;
     const int64_t ctas = (new_max * group + PA_ROWS - 1) / PA_ROWS * p->n_head_kv * a->n_seq;
-    int64_t want = (148 * 8 + ctas - 1) / ctas, most = (a->max_len + 127) / 128;
+    const int64_t resident = 148 * (p->head_dim == 64 ? 3 : 1);
+    int64_t want = (3 * resident + ctas - 1) / ctas, most = (a->max_len + PA_MIN_CHUNK - 1) / PA_MIN_CHUNK;
     if (want > most) want = most;
     if (want > 64) want = 64;
     if (want < 1) want = 1;
-    int64_t c = ((a->max_len + want - 1) / want + 31) / 32 * 32;
-    if (c < 32) c = 32;
+    const int64_t step = PA_KEYS * PA_WARPS;
+    int64_t c = ((a->max_len + want - 1) / want + step - 1) / step * step;
+    if (c < step) c = step;
     *chunk = (int) c;
     *n_split = (int) ((a->max_len + c - 1) / c);
     if (*n_split < 1) *n_split = 1;
@@ -285,7 +502,7 @@ extern "C" int64_t b200_paged_attn_workspace(const b200_page_pool * pool, const 
         a->n_head < 1 || a->n_head % pool->n_head_kv) return 0;
     int n_split, chunk;
     pa_plan(pool, a, &n_split, &chunk);
-    return n_split == 1 ? 0 : (int64_t) n_split * a->n_tok * a->n_head * (pool->head_dim + 2) * 4;
+    return n_split == 1 ? 0 : (int64_t) n_split * a->n_tok * a->n_head * (pool->head_dim + 4) * 4;
 }
 
 static PaArgs pa_pack(const b200_page_pool * p, const b200_paged_attn_args * a) {
@@ -324,7 +541,10 @@ extern "C" int b200_paged_store(const b200_page_pool * pool, const b200_paged_at
 template <typename Q, typename KV, int D>
 static cudaError_t pa_launch(PaArgs & k, int n_seq, cudaStream_t st) {
     const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
-    cudaError_t e = launch_chained(k_paged_attn<Q, KV, D>, dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) (n_seq * k.n_split)), dim3(128), 0, st, k);
+    constexpr int smem = 4 * PA_WARPS * PA_KEYS * D * 2;
+    cudaError_t e = cudaFuncSetAttribute(k_paged_attn<Q, KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    e = launch_chained(k_paged_attn<Q, KV, D>, dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) (n_seq * k.n_split)), dim3(32 * PA_WARPS), smem, st, k);
     if (e != cudaSuccess) return e;
     B200_LAUNCHED();
     if (k.n_split == 1) return cudaGetLastError();

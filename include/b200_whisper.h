@@ -352,6 +352,8 @@ typedef struct {
 } b200_paged_attn_args;
 int64_t b200_paged_attn_workspace(const b200_page_pool * pool, const b200_paged_attn_args * a);
 int b200_paged_attn(const b200_page_pool * pool, const b200_paged_attn_args * a, void * stream);
+/* 0, or the code of a device-side wait that ran out in an earlier launch (which then left its rows unfinished); synchronises. */
+int b200_paged_attn_status(void);
 /* The store alone (prompts whose attention runs elsewhere, caches filled from another source); uses of *a: k_new .. q_start,
  * n_tok, n_seq, max_new, max_len, and q_type as the type of k_new / v_new. */
 int b200_paged_store(const b200_page_pool * pool, const b200_paged_attn_args * a, void * stream);

@@ -2,37 +2,9 @@
 // The reference has one dense cache per state (whisper_kv_cache, src/whisper.cpp:1000-1200) and decodes through
 // ggml_compute_forward_flash_attn_ext_f16 (ggml/src/ggml-cpu/ops.cpp:6638-6851); this operator is defined by its formula
 // (include/b200_whisper.h), with 32-bit scores, weights' sums and accumulators.
-#include "b200_common.cuh"
-#include <cuda_bf16.h>
+#include "paged_attn.cuh"
 
 bool b200_pool_ok(const b200_page_pool * p, bool data);    // k_pages.cu
-
-struct PaArgs {
-    const char * q; int64_t nb_q_tok, nb_q_head;
-    char * dst; int64_t nb_dst_tok, nb_dst_head;
-    const char * k; const char * v; int64_t nb_page, nb_tok, nb_head;
-    const int32_t * tables; int64_t table_stride; const int32_t * lens; const int32_t * q_start;
-    float * lse;
-    float * part;                   // [split][n_tok * n_head] x (head_dim + 4): sums, maximum, sum of weights, pad
-    int64_t n_tok, max_len;
-    int n_pages, page_size, n_head, n_head_kv, group, max_new, causal, n_split, chunk;
-    float scale_log2;               // scale * log2(e): weights are powers of two
-};
-
-// the sequence's tokens: first query token, number of queries, keys in the pages (all cut to what the host was told)
-struct PaSeq { int64_t tok0; int n_new, len; };
-__device__ __forceinline__ PaSeq pa_seq(const PaArgs & a, int s) {
-    PaSeq r;
-    const int64_t b = a.q_start[s], e = a.q_start[s + 1];
-    r.tok0 = b;
-    const int64_t n = (b < 0 || e > a.n_tok || e < b) ? 0 : e - b;
-    r.n_new = (int) (n < a.max_new ? n : a.max_new);
-    int64_t len = a.lens[s];
-    len = len < 0 ? 0 : len < a.max_len ? len : a.max_len;
-    const int64_t room = a.table_stride * a.page_size;
-    r.len = (int) (len < room ? len : room);
-    return r;
-}
 
 // ---- store ---------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ uint4 pa_pack8(const float * x);
@@ -104,6 +76,7 @@ k_paged_store(PaArgs a, PaNew x, int vec_head) {
 #define PA_KEYS  32
 #define PA_WARPS 4
 #define PA_MIN_CHUNK 256
+#define PA_TC_MIN_ROWS 64
 
 template <typename T> struct PaPack;
 template <> struct PaPack<__half> {
@@ -154,12 +127,6 @@ __device__ __forceinline__ void pa_ldm_t(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3},[%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 
-// keys that any of the 16 rows from row0 on sees, from the first key
-__device__ __forceinline__ int pa_reach(const PaArgs & a, const PaSeq & s, int row0) {
-    const int last_t = (min(row0 + PA_ROWS, s.n_new * a.group) - 1) / a.group;
-    return a.causal ? min(s.len, max(s.len - s.n_new + last_t + 1, 0)) : s.len;
-}
-
 template <typename Q, typename KV, int D>
 __global__ void __launch_bounds__(32 * PA_WARPS)
 k_paged_attn(PaArgs a) {
@@ -185,7 +152,9 @@ k_paged_attn(PaArgs a) {
     auto key_of = [&](int i) { return k0 + (i * PA_WARPS + warp) * PA_KEYS + lane; };
     auto page_of = [&](int i) { const int key = key_of(i); return i < n_mine && key < k1 ? table[key / a.page_size] : -1; };
     auto at_of = [&](int i, int page) -> int64_t {       // this lane's key's place in the pool, -1: none
-        return page >= 0 && page < a.n_pages ? page * a.nb_page + (key_of(i) % a.page_size) * a.nb_tok : -1;
+        int64_t at = page >= 0 && page < a.n_pages ? page * a.nb_page + (key_of(i) % a.page_size) * a.nb_tok : -1;
+        asm volatile("" : "+l"(at));                     // kept: the compiler computes it again for every chunk otherwise, division included
+        return at;
     };
     auto load = [&](int i, int64_t at, const char * base, uint32_t dst) {
         if (i < n_mine) {
@@ -437,7 +406,7 @@ k_paged_join(PaArgs a) {
     for (int64_t w = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 5); w < (int64_t) s.n_new * a.n_head; w += (int64_t) gridDim.x * 4) {
         const int t = (int) (w / a.n_head), h = (int) (w - (int64_t) t * a.n_head);
         const int64_t out = (s.tok0 + t) * a.n_head + h;
-        const int row = t * a.group + h % a.group, row0 = row / PA_ROWS * PA_ROWS;
+        const int row = t * a.group + h % a.group, row0 = row / a.tile_rows * a.tile_rows;
         const int n = max(1, (pa_reach(a, s, row0) + a.chunk - 1) / a.chunk);
         const float * p = a.part + out * (D + 4);
         const int64_t step = a.n_tok * a.n_head * (D + 4);
@@ -479,30 +448,36 @@ static bool pa_args_ok(const b200_page_pool * p, const b200_paged_attn_args * a,
     return a->scale == a->scale && a->scale - a->scale == 0.0f;        // finite
 }
 
-// keys per split and number of splits: enough CTAs to fill the device, no split shorter than a few blocks of keys
-static void pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a, int * n_split, int * chunk) {
+// which kernel, keys per split and number of splits
+struct PaPlan { bool tc; int n_split, chunk; };
+static PaPlan pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a) {
+    PaPlan r;
     const int64_t group = a->n_head / p->n_head_kv;
-    const int64_t new_max = a->max_new < a->n_tok ? a->max_new : a->n_tok;
-    const int64_t ctas = (new_max * group + PA_ROWS - 1) / PA_ROWS * p->n_head_kv * a->n_seq;
-    const int64_t resident = 148 * (p->head_dim == 64 ? 3 : 1);
-    int64_t want = (3 * resident + ctas - 1) / ctas, most = (a->max_len + PA_MIN_CHUNK - 1) / PA_MIN_CHUNK;
+    const int64_t rows = (a->max_new < a->n_tok ? a->max_new : a->n_tok) * group;
+    r.tc = a->q_type != B200_TYPE_F32 && rows > PA_TC_MIN_ROWS;
+    const int64_t tile = r.tc ? PA_TC_ROWS : PA_ROWS;
+    const int64_t ctas = (rows + tile - 1) / tile * p->n_head_kv * a->n_seq;
+    const int64_t resident = 148 * (r.tc ? (p->head_dim == 64 ? 2 : 1) : (p->head_dim == 64 ? 3 : 1));
+    const int64_t least = r.tc ? 512 : PA_MIN_CHUNK;
+    int64_t want = ((r.tc ? 1 : 3) * resident + ctas - 1) / ctas, most = (a->max_len + least - 1) / least;
+    if (r.tc && ctas * 2 > resident) want = 1;
     if (want > most) want = most;
     if (want > 64) want = 64;
     if (want < 1) want = 1;
-    const int64_t step = PA_KEYS * PA_WARPS;
+    const int64_t step = 128;
     int64_t c = ((a->max_len + want - 1) / want + step - 1) / step * step;
     if (c < step) c = step;
-    *chunk = (int) c;
-    *n_split = (int) ((a->max_len + c - 1) / c);
-    if (*n_split < 1) *n_split = 1;
+    r.chunk = (int) c;
+    r.n_split = (int) ((a->max_len + c - 1) / c);
+    if (r.n_split < 1) r.n_split = 1;
+    return r;
 }
 
 extern "C" int64_t b200_paged_attn_workspace(const b200_page_pool * pool, const b200_paged_attn_args * a) {
     if (!a || !b200_pool_ok(pool, true) || a->n_tok < 1 || a->n_seq < 1 || a->max_new < 1 || a->max_len < 0 || a->max_len >= (1ll << 30) ||
         a->n_head < 1 || a->n_head % pool->n_head_kv) return 0;
-    int n_split, chunk;
-    pa_plan(pool, a, &n_split, &chunk);
-    return n_split == 1 ? 0 : (int64_t) n_split * a->n_tok * a->n_head * (pool->head_dim + 4) * 4;
+    const PaPlan r = pa_plan(pool, a);
+    return r.n_split == 1 ? 0 : (int64_t) r.n_split * a->n_tok * a->n_head * (pool->head_dim + 4) * 4;
 }
 
 static PaArgs pa_pack(const b200_page_pool * p, const b200_paged_attn_args * a) {
@@ -540,13 +515,19 @@ extern "C" int b200_paged_store(const b200_page_pool * pool, const b200_paged_at
 
 template <typename Q, typename KV, int D>
 static cudaError_t pa_launch(PaArgs & k, int n_seq, cudaStream_t st) {
+    cudaError_t e;
+    if (k.tile_rows == PA_TC_ROWS) {
+        e = pa_tc_launch(k, D, std::is_same<KV, __half>::value ? B200_TYPE_F16 : B200_TYPE_BF16, n_seq, st);
+        if (e != cudaSuccess) return e;
+    } else {
     const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
     constexpr int smem = 4 * PA_WARPS * PA_KEYS * D * 2;
-    cudaError_t e = cudaFuncSetAttribute(k_paged_attn<Q, KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(k_paged_attn<Q, KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     e = launch_chained(k_paged_attn<Q, KV, D>, dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) (n_seq * k.n_split)), dim3(32 * PA_WARPS), smem, st, k);
     if (e != cudaSuccess) return e;
     B200_LAUNCHED();
+    }
     if (k.n_split == 1) return cudaGetLastError();
     int64_t n = ((int64_t) k.max_new * k.n_head + 3) / 4;
     if (n > 4096) n = 4096;
@@ -559,7 +540,8 @@ extern "C" int b200_paged_attn(const b200_page_pool * pool, const b200_paged_att
     if (!pa_args_ok(pool, a, true)) return B200_ERR_ARG;
     if (a->n_seq == 0 || a->n_tok == 0 || a->max_new == 0) return 0;
     PaArgs k = pa_pack(pool, a);
-    pa_plan(pool, a, &k.n_split, &k.chunk);
+    const PaPlan r = pa_plan(pool, a);
+    k.n_split = r.n_split; k.chunk = r.chunk; k.tile_rows = r.tc ? PA_TC_ROWS : PA_ROWS;
     const int64_t need = b200_paged_attn_workspace(pool, a);
     if (need && (!a->workspace || (uintptr_t) a->workspace % 16 || a->workspace_bytes < need)) return B200_ERR_ARG;
     if ((int64_t) a->n_seq * k.n_split > 65535) return B200_ERR_ARG;

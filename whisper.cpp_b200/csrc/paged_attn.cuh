@@ -1,0 +1,41 @@
+// What the kernels of attention over a paged cache share (k_paged_attn.cu, k_paged_attn_tc.cu).
+#pragma once
+#include "b200_common.cuh"
+#include <cuda_bf16.h>
+
+struct PaArgs {
+    const char * q; int64_t nb_q_tok, nb_q_head;
+    char * dst; int64_t nb_dst_tok, nb_dst_head;
+    const char * k; const char * v; int64_t nb_page, nb_tok, nb_head;
+    const int32_t * tables; int64_t table_stride; const int32_t * lens; const int32_t * q_start;
+    float * lse;
+    float * part;                   // [split][n_tok * n_head] x (head_dim + 4): sums, maximum, sum of weights, pad
+    int64_t n_tok, max_len;
+    int n_pages, page_size, n_head, n_head_kv, group, max_new, causal, n_split, chunk, tile_rows;
+    float scale_log2;               // scale * log2(e): weights are powers of two
+};
+
+// the sequence's tokens: first query token, number of queries, keys in the pages (all cut to what the host was told)
+struct PaSeq { int64_t tok0; int n_new, len; };
+__device__ __forceinline__ PaSeq pa_seq(const PaArgs & a, int s) {
+    PaSeq r;
+    const int64_t b = a.q_start[s], e = a.q_start[s + 1];
+    r.tok0 = b;
+    const int64_t n = (b < 0 || e > a.n_tok || e < b) ? 0 : e - b;
+    r.n_new = (int) (n < a.max_new ? n : a.max_new);
+    int64_t len = a.lens[s];
+    len = len < 0 ? 0 : len < a.max_len ? len : a.max_len;
+    const int64_t room = a.table_stride * a.page_size;
+    r.len = (int) (len < room ? len : room);
+    return r;
+}
+
+// keys that any row of the tile (tile_rows rows, row0 the first) sees, from the first key
+__device__ __forceinline__ int pa_reach(const PaArgs & a, const PaSeq & s, int row0) {
+    const int last_t = (min(row0 + a.tile_rows, s.n_new * a.group) - 1) / a.group;
+    return a.causal ? min(s.len, max(s.len - s.n_new + last_t + 1, 0)) : s.len;
+}
+
+// the tcgen05 form (k_paged_attn_tc.cu); rows of a tile, and its launch: a.n_split, a.chunk (a multiple of 128) and a.tile_rows are set
+#define PA_TC_ROWS 256
+cudaError_t pa_tc_launch(const PaArgs & a, int head_dim, int type, int n_seq, cudaStream_t st);

@@ -12,13 +12,16 @@
 //                    sums are exact in the same sense, and the rescaling of O (a read and a write of tensor memory) is rare.
 //   warp 8           one thread issues all MMAs.  S_t(j+1) follows P_t V(j) in issue order, so the commit behind S_t(j+1) also says that
 //                    O_t is at rest and that P_t may be overwritten; no further barrier is needed for either.
-//   warps 9, 10      bring K and V: per key one page lookup, 16-byte cp.async into the swizzled tile, zeros for keys out of reach and
-//                    pages out of the pool, then a proxy fence and the barrier that the MMA thread waits for.
+//   warps 9, 10      bring K and V by TMA, page by page into the swizzled tile, where pages fit into blocks or blocks into pages (page
+//                    sizes 8, 16, 32, .. and multiples of BN); otherwise per key one page lookup and 16-byte cp.async.  Zeros for keys
+//                    out of reach and pages out of the pool.
 // 0 * v is not 0 where v is infinite or NaN: in blocks that are not wholly seen the V warp takes such values out of its tile and raises
 // a flag; the rows that do see them add them at the end, from the pages.
 // All waits are bounded (about a second), record a code (b200_paged_attn_status) and make every role leave through the exit that frees
 // tensor memory.
 #include "paged_attn.cuh"
+#include <cuda.h>
+#include <string.h>
 
 __device__ int g_pa_status;
 
@@ -29,11 +32,14 @@ extern "C" int b200_paged_attn_status(void) {
 }
 
 #define PT_THREADS 352
+#ifndef PT_FMA_EXP
+#define PT_FMA_EXP 3           // pairs of eight whose exponential goes to the FMA pipe
+#endif
 
 template <int D, int BN, int NS> struct PtSmem {
     static constexpr int TILE = BN * D * 2, QT = 128 * D * 2;
     static constexpr int Q = 0, K = 2 * QT, V = K + NS * TILE, BAR = V + NS * TILE;
-    static constexpr int N_BAR = 4 * NS + 7;             // k_full, k_empty, v_full, v_empty [NS]; q_full; s_full, p_full, o_full [2]
+    static constexpr int N_BAR = 5 * NS + 7;             // k_full, k_empty, v_full, v_empty, v_here [NS]; q_full; s_full, p_full, o_full [2]
     static constexpr int MISC = BAR + N_BAR * 8;         // tensor-memory address, abort flag, odd-value flag
     static constexpr int BYTES = MISC + 16 + 1024;       // the dynamic array starts on 16 bytes: tiles are moved to 1024
 };
@@ -133,6 +139,43 @@ template <typename T> __device__ __forceinline__ uint32_t pt_odd(uint32_t w) {
     return ((w & e) == e ? 0xffffu : 0u) | ((w >> 16 & e) == e ? 0xffff0000u : 0u);
 }
 
+// K and V as (dimension, head, token of the page, page) for TMA: boxes of 64 dimensions, one head, `box` tokens.  box = 0: pages that
+// a block of BN keys is no multiple or part of (or that no map could be made for): cp.async instead.
+struct PtMaps { CUtensorMap k, v; int box; };
+__device__ __forceinline__ void pt_tma(uint32_t dst, const CUtensorMap * map, int x, int head, int tok, int page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(head), "r"(tok), "r"(page) : "memory");
+}
+__device__ __forceinline__ void pt_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+
+typedef unsigned long long pt_f2;                         // two floats for the packed instructions
+__device__ __forceinline__ pt_f2 pt_pair(float a, float b) { pt_f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void pt_split(pt_f2 v, float & a, float & b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ pt_f2 pt_fma2(pt_f2 a, pt_f2 b, pt_f2 c) { pt_f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ pt_f2 pt_add2(pt_f2 a, pt_f2 b) { pt_f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ pt_f2 pt_mul2(pt_f2 a, pt_f2 b) { pt_f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+// 2^y of a pair on the FMA pipe, for y <= 127: y = n + f with |f| <= 1/2, a polynomial in f (Chebyshev interpolation of degree 5, computed
+// for this file: off by less than 2^-22) times 2^n.  Below 2^-126 it stays there.  The exponential unit does one value where the FMA
+// pipe does about one too: sharing the work shortens the softmax, which the tensor core waits for.
+__device__ __forceinline__ void pt_exp2_fma(float & y0, float & y1) {
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(y0));       // at least -126; NaN stays NaN
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(y1));
+    const pt_f2 y = pt_pair(y0, y1);
+    const pt_f2 r = pt_add2(y, pt_pair(12582912.0f, 12582912.0f));                       // 1.5 * 2^23: the integer part lands in the low bits
+    const pt_f2 f = pt_add2(y, pt_fma2(r, pt_pair(-1.0f, -1.0f), pt_pair(12582912.0f, 12582912.0f)));
+    pt_f2 p = pt_fma2(pt_pair(0.0013390863314270973f, 0.0013390863314270973f), f, pt_pair(0.009676031768321991f, 0.009676031768321991f));
+    p = pt_fma2(p, f, pt_pair(0.055503569543361664f, 0.055503569543361664f));
+    p = pt_fma2(p, f, pt_pair(0.2402210682630539f, 0.2402210682630539f));
+    p = pt_fma2(p, f, pt_pair(0.6931471824645996f, 0.6931471824645996f));
+    p = pt_fma2(p, f, pt_pair(1.0000001192092896f, 1.0000001192092896f));
+    float r0, r1;
+    pt_split(r, r0, r1);
+    p = pt_mul2(p, pt_pair(__uint_as_float((__float_as_uint(r0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(r1) << 23) + 0x3f800000u)));
+    pt_split(p, y0, y1);
+}
+
 // any + 0 * every value of x
 template <typename T> __device__ __forceinline__ float pt_zero_times(uint4 x, float any) {
     const uint32_t w[4] = { x.x, x.y, x.z, x.w };
@@ -147,7 +190,7 @@ template <typename T> __device__ __forceinline__ float pt_zero_times(uint4 x, fl
 
 template <typename T, int D, int BN, int NS, int MIN_CTAS>
 __global__ void __launch_bounds__(PT_THREADS, MIN_CTAS)
-k_paged_attn_tc(const __grid_constant__ PaArgs a) {
+k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps maps) {
     using L = PtSmem<D, BN, NS>;
     constexpr int COLS = 2 * BN + 2 * D <= 256 ? 256 : 512, NC = D / 8;
     extern __shared__ __align__(16) char smem_raw[];
@@ -173,14 +216,14 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a) {
     const int n = max(n_blk[0], n_blk[1]);
     char * smem = smem_raw + ((1024 - ((uint32_t) __cvta_generic_to_shared(smem_raw) & 1023)) & 1023);
     const uint32_t sb = (uint32_t) __cvta_generic_to_shared(smem);
-    const uint32_t k_full = sb + L::BAR, k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS, q_full = v_empty + 8 * NS,
-                   s_full = q_full + 8, p_full = s_full + 16, o_full = p_full + 16;
+    const uint32_t k_full = sb + L::BAR, k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS, v_here = v_empty + 8 * NS,
+                   q_full = v_here + 8 * NS, s_full = q_full + 8, p_full = s_full + 16, o_full = p_full + 16;
     uint32_t * tmem_slot = (uint32_t *) (smem + L::MISC);
     volatile int * abort_flag = (volatile int *) (smem + L::MISC + 4);
     volatile int * odd_flag = (volatile int *) (smem + L::MISC + 8);
     if (tid == 0) {
         auto init = [](uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count)); };
-        for (int i = 0; i < 4 * NS; ++i) init(k_full + 8 * i, 1);
+        for (int i = 0; i < 5 * NS; ++i) init(k_full + 8 * i, 1);
         init(q_full, 8);
         for (int t = 0; t < 2; ++t) { init(s_full + 8 * t, 1); init(p_full + 8 * t, 4); init(o_full + 8 * t, 1); }
         *abort_flag = 0;
@@ -228,7 +271,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a) {
             uint32_t x[BN];
 #pragma unroll
             for (int c = 0; c < BN; c += 32) pt_ld32(x + c, ts + c);
-            float mx = -INFINITY;
+            float m4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
                 pt_wait32(x + c);
@@ -237,8 +280,11 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a) {
                     for (int i = c; i < c + 32; ++i) if (i >= seen) x[i] = 0xff800000u;
                 }
 #pragma unroll
-                for (int i = c; i < c + 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
+                for (int i = c; i < c + 32; i += 8)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], fmaxf(__uint_as_float(x[i + u]), __uint_as_float(x[i + 4 + u])));
             }
+            float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
             mx = mx == -INFINITY ? mx : mx * scale;
             const bool grow = mx > m + 8.0f;                              // also when there was no key so far
             if (__any_sync(0xffffffffu, grow)) {
@@ -258,20 +304,25 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a) {
                 }
             }
             const float base = m == -INFINITY ? 0.0f : -m;
-            float l0 = 0.0f, l1 = 0.0f;
+            pt_f2 l2[2] = { 0ull, 0ull };
+            const pt_f2 scale2 = pt_pair(scale, scale), base2 = pt_pair(base, base);
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float y0 = fmaf(__uint_as_float(x[c + 2 * i]), scale, base), y1 = fmaf(__uint_as_float(x[c + 2 * i + 1]), scale, base);
+                    float y0, y1;
+                    pt_split(pt_fma2(pt_pair(__uint_as_float(x[c + 2 * i]), __uint_as_float(x[c + 2 * i + 1])), scale2, base2), y0, y1);
                     if (edge) { if (c + 2 * i >= seen) y0 = -INFINITY; if (c + 2 * i + 1 >= seen) y1 = -INFINITY; }       // -inf * 0 is not -inf
-                    y0 = pt_exp2(y0); y1 = pt_exp2(y1);
-                    l0 += y0; l1 += y1;
+                    if (i % 8 < PT_FMA_EXP && !edge) pt_exp2_fma(y0, y1);
+                    else { y0 = pt_exp2(y0); y1 = pt_exp2(y1); }
+                    l2[i & 1] = pt_add2(l2[i & 1], pt_pair(y0, y1));
                     w[i] = pt_two<T>(y0, y1);
                 }
                 pt_st16(ts + c / 2, w);
             }
+            float l0, l1;
+            pt_split(pt_add2(l2[0], l2[1]), l0, l1);
             l += l0 + l1;
             pt_wait_st();
             pt_before();
@@ -359,6 +410,77 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a) {
         const uint32_t ring = sb + (is_v ? L::V : L::K), full = is_v ? v_full : k_full, empty = is_v ? v_empty : k_empty;
         const int32_t * table = a.tables + seq * a.table_stride;
         constexpr int G = BN / 32, LAG = NS - 2;
+        const int box = maps.box;
+        // V's non-finite values, in blocks that are not wholly seen, are taken out; a lane looks at the same 16-byte chunks that it copies
+        auto clean = [&](int jj) {
+            auto place = [&](int g, int c) {
+                const int i = c * 32 + lane, r = i / NC, ch = i % NC;
+                return (uint4 *) (smem + L::V + (jj % NS) * L::TILE + (ch >> 3) * BN * 128 + (g * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4));
+            };
+            float any = 0.0f;                                             // NaN as soon as a value is infinite or NaN: x * 0
+            const int rows = k1 - (k0 + jj * BN);                         // behind them nobody looks: zeros, whatever the page holds
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    if (g * 32 + (c * 32 + lane) / NC < rows) any = pt_zero_times<T>(*place(g, c), any);
+                    else *place(g, c) = make_uint4(0, 0, 0, 0);
+                }
+            if (any != any) {
+#pragma unroll 1
+                for (int g = 0; g < G; ++g)
+#pragma unroll 1
+                    for (int c = 0; c < NC; ++c) {
+                        uint4 * p = place(g, c);
+                        uint4 x = *p;
+                        x.x &= ~pt_odd<T>(x.x); x.y &= ~pt_odd<T>(x.y); x.z &= ~pt_odd<T>(x.z); x.w &= ~pt_odd<T>(x.w);
+                        *p = x;
+                    }
+                *odd_flag = 1;
+            }
+            pt_proxy_fence();
+        };
+        if (box) {
+            // TMA: lane i brings the block's i-th page (or its part of one); pages out of reach or out of the pool are named n_pages, which
+            // reads as zeros.  A page's tokens behind the sequence's end come along: K's are masked, V's cleaned.
+            const int per = BN / box;
+            auto page_of = [&](int j) {
+                const int key = k0 + j * BN + lane * box;
+                if (j >= n || lane >= per || key >= k1) return a.n_pages;
+                const int p = table[key / a.page_size];
+                return p < 0 || p > a.n_pages ? a.n_pages : p;
+            };
+            int page = page_of(0);
+            for (int j = 0; j < n + LAG; ++j) {
+                if (j < n) {
+                    const int now = page;
+                    page = page_of(j + 1);
+                    if (!pt_wait_warp(empty + 8 * (j % NS), (j / NS & 1) ^ 1, abort_flag, 8)) {
+                        for (int i = max(0, j - NS); i < j; ++i) pt_poll((is_v ? v_here : k_full) + 8 * (i % NS), i / NS & 1);       // copies under way
+                        goto done;
+                    }
+                    const uint32_t bar = (is_v ? v_here : k_full) + 8 * (j % NS), dst = ring + (j % NS) * L::TILE + lane * box * 128;
+                    if (lane == 0) pt_expect(bar, L::TILE);
+                    __syncwarp();
+                    if (lane < per) {
+                        const int tok = (k0 + j * BN + lane * box) % a.page_size;
+#pragma unroll
+                        for (int h = 0; h < D / 64; ++h) pt_tma(dst + h * BN * 128, is_v ? &maps.v : &maps.k, h * 64, kvh, tok, now, bar);
+                    }
+                    __syncwarp();
+                }
+                if (is_v && j >= LAG) {
+                    const int jj = j - LAG;
+                    if (!pt_wait_warp(v_here + 8 * (jj % NS), jj / NS & 1, abort_flag, 9)) goto done;
+                    if (k0 + (jj + 1) * BN > sure[0]) clean(jj);
+                    __syncwarp();
+                    if (lane == 0) pt_arrive(v_full + 8 * (jj % NS));
+                }
+            }
+            if (!is_v)                                                    // nothing may be under way when the CTA ends
+                for (int j = max(0, n - NS); j < n; ++j) if (!pt_wait_warp(k_full + 8 * (j % NS), j / NS & 1, abort_flag, 10)) break;
+            goto done;
+        }
         int page[G];
         auto look = [&](int j) {
 #pragma unroll
@@ -391,29 +513,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a) {
             if (j >= LAG) {
                 const int jj = j - LAG;
                 asm volatile("cp.async.wait_group %0;" :: "n"(LAG) : "memory");
-                if (is_v && k0 + (jj + 1) * BN > sure[0]) {               // a thread looks at what it has copied itself
-                    auto place = [&](int g, int c) {
-                        const int i = c * 32 + lane, r = i / NC, ch = i % NC;
-                        return (uint4 *) (smem + L::V + (jj % NS) * L::TILE + (ch >> 3) * BN * 128 + (g * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4));
-                    };
-                    float any = 0.0f;                                     // NaN as soon as a value is infinite or NaN: x * 0
-#pragma unroll
-                    for (int g = 0; g < G; ++g)
-#pragma unroll
-                        for (int c = 0; c < NC; ++c) { const uint4 x = *place(g, c); any = pt_zero_times<T>(x, any); }
-                    if (any != any) {
-#pragma unroll 1
-                        for (int g = 0; g < G; ++g)
-#pragma unroll 1
-                            for (int c = 0; c < NC; ++c) {
-                                uint4 * p = place(g, c);
-                                uint4 x = *p;
-                                x.x &= ~pt_odd<T>(x.x); x.y &= ~pt_odd<T>(x.y); x.z &= ~pt_odd<T>(x.z); x.w &= ~pt_odd<T>(x.w);
-                                *p = x;
-                            }
-                        *odd_flag = 1;
-                    }
-                }
+                if (is_v && k0 + (jj + 1) * BN > sure[0]) clean(jj);
                 pt_proxy_fence();
                 __syncwarp();
                 if (lane == 0) pt_arrive(full + 8 * (jj % NS));
@@ -431,6 +531,33 @@ done:
     }
 }
 
+typedef CUresult (*pt_encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static pt_encode_fn pt_encode() {
+    static const pt_encode_fn f = [] {
+        void * p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess) { cudaGetLastError(); p = nullptr; }
+        return (pt_encode_fn) p;
+    }();
+    return f;
+}
+
+// maps.box = 0 where the page size does not fit TMA boxes of whole 8-row groups, or the driver makes no map
+static void pt_make_maps(PtMaps & m, const PaArgs & a, int D, int BN, bool f16) {
+    memset(&m, 0, sizeof(m));
+    const int ps = a.page_size, box = ps < BN ? ps : BN;
+    if (ps % 8 || (ps < BN ? BN % ps : ps % BN) || !pt_encode()) return;
+    const cuuint64_t dims[4] = { (cuuint64_t) D, (cuuint64_t) a.n_head_kv, (cuuint64_t) ps, (cuuint64_t) a.n_pages };
+    const cuuint64_t row = (cuuint64_t) D * 2;
+    const cuuint64_t strides[3] = { a.n_head_kv > 1 ? (cuuint64_t) a.nb_head : row, (cuuint64_t) a.nb_tok, (cuuint64_t) a.nb_page };
+    const cuuint32_t size[4] = { 64, 1, (cuuint32_t) box, 1 }, one[4] = { 1, 1, 1, 1 };
+    for (int i = 0; i < 2; ++i)
+        if (pt_encode()(i ? &m.v : &m.k, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void *) (i ? a.v : a.k), dims, strides, size, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return;
+    m.box = box;
+}
+
 template <typename T, int D, int BN, int NS, int MIN_CTAS>
 static cudaError_t pt_go(const PaArgs & a, int n_seq, cudaStream_t st) {
     const int smem = PtSmem<D, BN, NS>::BYTES;
@@ -438,7 +565,9 @@ static cudaError_t pt_go(const PaArgs & a, int n_seq, cudaStream_t st) {
     auto k = k_paged_attn_tc<T, D, BN, NS, MIN_CTAS>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    e = launch_chained(k, dim3((unsigned) tiles, (unsigned) a.n_head_kv, (unsigned) (n_seq * a.n_split)), dim3(PT_THREADS), smem, st, a);
+    PtMaps maps;
+    pt_make_maps(maps, a, D, BN, std::is_same<T, __half>::value);
+    e = launch_chained(k, dim3((unsigned) tiles, (unsigned) a.n_head_kv, (unsigned) (n_seq * a.n_split)), dim3(PT_THREADS), smem, st, a, maps);
     if (e == cudaSuccess) B200_LAUNCHED();
     return e;
 }

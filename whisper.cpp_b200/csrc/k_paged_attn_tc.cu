@@ -9,7 +9,9 @@
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread owns a row.  It reads its scores (tcgen05.ld), masks only blocks that some row
 //                    does not see wholly, and writes the weights back as P.  The reference point of the exponentials is the running
 //                    maximum, but it follows it only when the maximum has grown by more than 2^8: the weights stay below 256, the
-//                    sums are exact in the same sense, and the rescaling of O (a read and a write of tensor memory) is rare.
+//                    sums are exact in the same sense, and the rescaling of O (a read and a write of tensor memory) is rare.  All
+//                    exponentials go to the exponential unit: two to five of eight pairs as a polynomial on the FMA pipe made a chunk of
+//                    2048 over 16k keys slower (1.11 -> 1.41 .. 1.83 ms).
 //   warp 8           one thread issues all MMAs.  S_t(j+1) follows P_t V(j) in issue order, so the commit behind S_t(j+1) also says that
 //                    O_t is at rest and that P_t may be overwritten; no further barrier is needed for either.
 //   warps 9, 10      bring K and V by TMA, page by page into the swizzled tile, where pages fit into blocks or blocks into pages (page
@@ -32,9 +34,6 @@ extern "C" int b200_paged_attn_status(void) {
 }
 
 #define PT_THREADS 352
-#ifndef PT_FMA_EXP
-#define PT_FMA_EXP 3           // pairs of eight whose exponential goes to the FMA pipe
-#endif
 
 template <int D, int BN, int NS> struct PtSmem {
     static constexpr int TILE = BN * D * 2, QT = 128 * D * 2;
@@ -155,27 +154,6 @@ __device__ __forceinline__ pt_f2 pt_pair(float a, float b) { pt_f2 r; asm("mov.b
 __device__ __forceinline__ void pt_split(pt_f2 v, float & a, float & b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 __device__ __forceinline__ pt_f2 pt_fma2(pt_f2 a, pt_f2 b, pt_f2 c) { pt_f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 __device__ __forceinline__ pt_f2 pt_add2(pt_f2 a, pt_f2 b) { pt_f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ pt_f2 pt_mul2(pt_f2 a, pt_f2 b) { pt_f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-// 2^y of a pair on the FMA pipe, for y <= 127: y = n + f with |f| <= 1/2, a polynomial in f (Chebyshev interpolation of degree 5, computed
-// for this file: off by less than 2^-22) times 2^n.  Below 2^-126 it stays there.  The exponential unit does one value where the FMA
-// pipe does about one too: sharing the work shortens the softmax, which the tensor core waits for.
-__device__ __forceinline__ void pt_exp2_fma(float & y0, float & y1) {
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(y0));       // at least -126; NaN stays NaN
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(y1));
-    const pt_f2 y = pt_pair(y0, y1);
-    const pt_f2 r = pt_add2(y, pt_pair(12582912.0f, 12582912.0f));                       // 1.5 * 2^23: the integer part lands in the low bits
-    const pt_f2 f = pt_add2(y, pt_fma2(r, pt_pair(-1.0f, -1.0f), pt_pair(12582912.0f, 12582912.0f)));
-    pt_f2 p = pt_fma2(pt_pair(0.0013390863314270973f, 0.0013390863314270973f), f, pt_pair(0.009676031768321991f, 0.009676031768321991f));
-    p = pt_fma2(p, f, pt_pair(0.055503569543361664f, 0.055503569543361664f));
-    p = pt_fma2(p, f, pt_pair(0.2402210682630539f, 0.2402210682630539f));
-    p = pt_fma2(p, f, pt_pair(0.6931471824645996f, 0.6931471824645996f));
-    p = pt_fma2(p, f, pt_pair(1.0000001192092896f, 1.0000001192092896f));
-    float r0, r1;
-    pt_split(r, r0, r1);
-    p = pt_mul2(p, pt_pair(__uint_as_float((__float_as_uint(r0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(r1) << 23) + 0x3f800000u)));
-    pt_split(p, y0, y1);
-}
-
 // any + 0 * every value of x
 template <typename T> __device__ __forceinline__ float pt_zero_times(uint4 x, float any) {
     const uint32_t w[4] = { x.x, x.y, x.z, x.w };
@@ -314,8 +292,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                     float y0, y1;
                     pt_split(pt_fma2(pt_pair(__uint_as_float(x[c + 2 * i]), __uint_as_float(x[c + 2 * i + 1])), scale2, base2), y0, y1);
                     if (edge) { if (c + 2 * i >= seen) y0 = -INFINITY; if (c + 2 * i + 1 >= seen) y1 = -INFINITY; }       // -inf * 0 is not -inf
-                    if (i % 8 < PT_FMA_EXP && !edge) pt_exp2_fma(y0, y1);
-                    else { y0 = pt_exp2(y0); y1 = pt_exp2(y1); }
+                    y0 = pt_exp2(y0); y1 = pt_exp2(y1);
                     l2[i & 1] = pt_add2(l2[i & 1], pt_pair(y0, y1));
                     w[i] = pt_two<T>(y0, y1);
                 }

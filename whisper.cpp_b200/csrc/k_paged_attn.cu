@@ -64,16 +64,16 @@ k_paged_store(PaArgs a, PaNew x, int vec_head) {
 // ---- attention of few rows, and of f32 queries ---------------------------------------------------
 // A row is one query token of one query head; the rows of a key/value head are numbered token * group + head in group.  A CTA
 // takes 16 rows of one sequence and key/value head over one split of the keys - the 16 rows of an mma.sync m16n8k16 - and each of
-// its four warps streams every fourth block of 32 keys through its own shared-memory ring (two blocks deep, K and V separate
-// cp.async groups), so nothing in the loop waits for another warp.  Running maximum and sum per row; the warps are joined through
-// shared memory at the end, the splits by k_paged_join.  Bound by the stream of K and V: a block of 32 keys is 16 KB (head_dim
-// 128) for 64 MMAs.
+// its four warps streams every fourth block of keys (4 KB of K, 4 KB of V) through its own shared-memory ring (two blocks deep, K and
+// V separate cp.async groups), so nothing in the loop waits for another warp.  Running maximum and sum per row; the warps are joined through
+// shared memory at the end, the splits by k_paged_join.  Bound by the stream of K and V.  Rings of 16 KB
+// put three CTAs on an SM; with twice the block, and one CTA, 64 sequences of up to 8192 keys (head_dim 128) took 292 us instead of 189.
 //
 // F32 queries: q and the weights are written as sums of two f16 (the second scaled by 2^11, q scaled by a power of two per row
 // so that no part underflows) or three bf16 values, which hold 22 or 24 bits of them, and each part is multiplied on the tensor
 // pipe; products of a block are added to the f32 accumulator by FADD, because the tensor pipe's own accumulation truncates.
 #define PA_ROWS  16
-#define PA_KEYS  32
+#define PA_BLOCK 4096                            // bytes of a block of K or V: 32 keys of 64 or 16 of 128 dimensions
 #define PA_WARPS 4
 #define PA_MIN_CHUNK 256
 #define PA_TC_MIN_ROWS 64
@@ -84,7 +84,7 @@ template <> struct PaPack<__half> {
     static __device__ __forceinline__ float2 back(uint32_t w) { return __half22float2(*(const __half2 *) &w); }
     static __device__ __forceinline__ uint32_t odd(uint32_t w) { return ((w & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u); }
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t * a, uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 };
@@ -93,7 +93,7 @@ template <> struct PaPack<__nv_bfloat16> {
     static __device__ __forceinline__ float2 back(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
     static __device__ __forceinline__ uint32_t odd(uint32_t w) { return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u); }
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t * a, uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 };
@@ -133,7 +133,7 @@ k_paged_attn(PaArgs a) {
     using P = PaPack<KV>;
     constexpr int NP = PaParts<Q, KV>::n, NC = D / 8, KS = D / 16;      // parts, 16-byte chunks and MMA steps of a head
     constexpr float LIFT = PaParts<Q, KV>::lift;
-    constexpr int BLOCK = PA_KEYS * D * 2;                              // bytes of a block of K or V
+    constexpr int BLOCK = PA_BLOCK, KEYS = BLOCK / (2 * D), NK = KEYS / 8;       // keys of a block, MMA columns of its scores
     extern __shared__ __align__(16) char smem[];
     chain_release();
     chain_wait();
@@ -148,9 +148,9 @@ k_paged_attn(PaArgs a) {
     const char * kp = a.k + kvh * a.nb_head, * vp = a.v + kvh * a.nb_head;
     const int32_t * table = a.tables + seq * a.table_stride;
     const uint32_t ring = pa_smem(smem) + warp * 4 * BLOCK;             // K0 K1 V0 V1
-    const int n_block = k1 > k0 ? (k1 - k0 + PA_KEYS - 1) / PA_KEYS : 0, n_mine = (n_block - warp + PA_WARPS - 1) / PA_WARPS;
-    auto key_of = [&](int i) { return k0 + (i * PA_WARPS + warp) * PA_KEYS + lane; };
-    auto page_of = [&](int i) { const int key = key_of(i); return i < n_mine && key < k1 ? table[key / a.page_size] : -1; };
+    const int n_block = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0, n_mine = (n_block - warp + PA_WARPS - 1) / PA_WARPS;
+    auto key_of = [&](int i) { return k0 + (i * PA_WARPS + warp) * KEYS + lane; };
+    auto page_of = [&](int i) { const int key = key_of(i); return i < n_mine && lane < KEYS && key < k1 ? table[key / a.page_size] : -1; };
     auto at_of = [&](int i, int page) -> int64_t {       // this lane's key's place in the pool, -1: none
         int64_t at = page >= 0 && page < a.n_pages ? page * a.nb_page + (key_of(i) % a.page_size) * a.nb_tok : -1;
         asm volatile("" : "+l"(at));                     // kept: the compiler computes it again for every chunk otherwise, division included
@@ -159,7 +159,7 @@ k_paged_attn(PaArgs a) {
     auto load = [&](int i, int64_t at, const char * base, uint32_t dst) {
         if (i < n_mine) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
+            for (int c = 0; c < NC * KEYS / 32; ++c) {
                 const int x = c * 32 + lane, r = x / NC, ch = x % NC;
                 const int64_t off = __shfl_sync(0xffffffffu, at, r);
                 pa_cp16(dst + r * D * 2 + ((ch ^ (r & 7)) << 4), base + (off < 0 ? 0 : off + ch * 16), off >= 0);
@@ -227,37 +227,43 @@ k_paged_attn(PaArgs a) {
     float o[NC][4] = {}, ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
     for (int i = 0; i < n_mine; ++i) {
         const uint32_t kb = ring + (i & 1) * BLOCK, vb = kb + 2 * BLOCK;
-        const int key0 = k0 + (i * PA_WARPS + warp) * PA_KEYS;
+        const int key0 = k0 + (i * PA_WARPS + warp) * KEYS;
         at_next = at_of(i + 2, page_next);
         page_next = page_of(i + 3);
         pa_wait<3>();
         __syncwarp();
-        // scores of 16 rows and 32 keys
-        float sc[4][4] = {};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float part[NP][4] = {};
+        // scores of 16 rows and the block's keys
+        float sc[NK][4];
+        {
+            float part[NP][NK][4] = {};
 #pragma unroll
             for (int h = 0; h < KS / 2; ++h) {
-                uint32_t b[4];
-                pa_ldm(b, kb + (8 * j + (lane & 7)) * D * 2 + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4));
+                uint32_t b[NK][4];
 #pragma unroll
-                for (int n = 0; n < NP; ++n) { P::mma(part[n], qf[n][2 * h], b[0], b[1]); P::mma(part[n], qf[n][2 * h + 1], b[2], b[3]); }
+                for (int j = 0; j < NK; ++j) pa_ldm(b[j], kb + (8 * j + (lane & 7)) * D * 2 + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NP; ++n)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int j = 0; j < NK; ++j) P::mma(part[n][j], qf[n][2 * h + u], b[j][2 * u], b[j][2 * u + 1]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float v = part[NP - 1][e];
+            for (int j = 0; j < NK; ++j)
 #pragma unroll
-                for (int n = NP - 2; n >= 0; --n) v = part[n][e] + v * (1.0f / LIFT);
-                sc[j][e] = v;
-            }
+                for (int e = 0; e < 4; ++e) {
+                    float v = part[NP - 1][j][e];
+#pragma unroll
+                    for (int n = NP - 2; n >= 0; --n) v = part[n][j][e] + v * (1.0f / LIFT);
+                    sc[j][e] = v;
+                }
         }
         __syncwarp();
         load(i + 2, at_next, kp, kb);
-        const bool edge = key0 + PA_KEYS - 1 > first_last || key0 + PA_KEYS > k1;
+        const bool edge = key0 + KEYS - 1 > first_last || key0 + KEYS > k1;
         float xa = -INFINITY, xb = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NK; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 sc[j][e] *= fa; sc[j][e + 2] *= fb;
@@ -275,9 +281,9 @@ k_paged_attn(PaArgs a) {
         const float ca = exp2f(ma - ba), cb = exp2f(mb - bb);
         ma = xa; mb = xb;
         la *= ca; lb *= cb;
-        uint32_t pf[NP][2][4];
+        uint32_t pf[NP][NK / 2][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < NK; ++j) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 sc[j][e] = exp2f(sc[j][e] - ba); sc[j][e + 2] = exp2f(sc[j][e + 2] - bb);
@@ -300,7 +306,7 @@ k_paged_attn(PaArgs a) {
         for (int c = 0; c < NC / 2; ++c) {
             float part[NP][2][4] = {};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < NK / 2; ++h) {
                 uint32_t b[4];
                 pa_ldm_t(b, vb + (16 * h + (lane & 15)) * D * 2 + (((2 * c + (lane >> 4)) ^ (lane & 7)) << 4));
                 if (edge) {                               // 0 * v is not 0 where v is infinite or NaN: such values are taken out here
@@ -326,7 +332,7 @@ k_paged_attn(PaArgs a) {
             }
         }
         if (edge && __any_sync(0xffffffffu, odd)) {       // ... and given back to the rows that see them
-            for (int j = 0; j < min(PA_KEYS, k1 - key0); ++j)
+            for (int j = 0; j < min(KEYS, k1 - key0); ++j)
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const KV * v = (const KV *) (smem + (vb - pa_smem(smem)) + j * D * 2 + ((c ^ (j & 7)) << 4)) + (lane & 3) * 2;
@@ -457,14 +463,14 @@ static PaPlan pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a) 
     r.tc = a->q_type != B200_TYPE_F32 && rows > PA_TC_MIN_ROWS;
     const int64_t tile = r.tc ? PA_TC_ROWS : PA_ROWS;
     const int64_t ctas = (rows + tile - 1) / tile * p->n_head_kv * a->n_seq;
-    const int64_t resident = 148 * (r.tc ? (p->head_dim == 64 ? 2 : 1) : (p->head_dim == 64 ? 3 : 1));
+    const int64_t resident = 148 * (r.tc ? (p->head_dim == 64 ? 2 : 1) : 3);
     const int64_t least = r.tc ? 512 : PA_MIN_CHUNK;
     int64_t want = ((r.tc ? 1 : 3) * resident + ctas - 1) / ctas, most = (a->max_len + least - 1) / least;
     if (r.tc && ctas * 2 > resident) want = 1;
     if (want > most) want = most;
     if (want > 64) want = 64;
     if (want < 1) want = 1;
-    const int64_t step = 128;
+    const int64_t step = 128;          // a multiple of the blocks of both kernels
     int64_t c = ((a->max_len + want - 1) / want + step - 1) / step * step;
     if (c < step) c = step;
     r.chunk = (int) c;
@@ -521,7 +527,7 @@ static cudaError_t pa_launch(PaArgs & k, int n_seq, cudaStream_t st) {
         if (e != cudaSuccess) return e;
     } else {
     const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
-    constexpr int smem = 4 * PA_WARPS * PA_KEYS * D * 2;
+    constexpr int smem = 4 * PA_WARPS * PA_BLOCK;
     e = cudaFuncSetAttribute(k_paged_attn<Q, KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     e = launch_chained(k_paged_attn<Q, KV, D>, dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) (n_seq * k.n_split)), dim3(32 * PA_WARPS), smem, st, k);

@@ -443,6 +443,9 @@ SHAPES = [
     ([(1, 3000), (2, 1999)], 1, 8, 128, 100),
     ([(64, 1025)], 1, 16, 128, 1),
     ([(260, 515), (0, 40), (33, 33)], 1, 2, 128, 128),
+    ([(16, 100), (9, 9), (2, 300), (0, 7), (16, 17)], 2, 4, 64, 16),
+    ([(1, 5000), (1, 1), (0, 0), (1, 777), (1, 4096), (1, 64)], 3, 2, 128, 16),
+    ([(4, 3001), (1, 3), (3, 2500)], 2, 7, 64, 24),
 ]
 
 

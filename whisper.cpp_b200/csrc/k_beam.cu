@@ -8,11 +8,16 @@
 // score(b, v) = score[b] + (x - m) - log(sum exp(x - m)).  Within a row the order of the candidates is the order of the
 // logits, so a row's n_beam best logits are all it can contribute: pass 1 cuts every row into slices and leaves, per slice,
 // its maximum, its sum of exponentials and its n_beam best logits; pass 2 joins the slices of a sequence's rows and picks
-// the n_beam best of their sorted lists.  The logits are read once; what bounds pass 1 is that read, and at few rows the
-// latency of load -> maximum -> sum -> list.
+// the n_beam best of their sorted lists.  The logits are read once and stay in registers.  The n_beam-th best of the threads' maxima
+// bounds the slice's n_beam best from below, so that only logits that reach it are looked at one by one: about n_beam of them.  Where
+// equal logits make them many (more than SEL_CAP), the bound is taken once more with the index as the second part of the key; then the
+// n_beam threads that reach it hold all that do.  (A sorted list per warp, filled tile by tile, cost more in insertions: 65 us for 320
+// rows of 51866.)
 #define SEL_THREADS 256
-#define SEL_EPT     16                              // logits per thread, all in registers
-#define SEL_SLICE   (SEL_THREADS * SEL_EPT)
+#define SEL_EPT     16                              // logits per thread and tile
+#define SEL_TILE    (SEL_THREADS * SEL_EPT)
+#define SEL_MANY    4                               // tiles of a slice where rows are many (64 logits per thread); one tile otherwise
+#define SEL_CAP     (B200_BEAM_MAX * SEL_EPT * SEL_MANY)
 #define SEL_LISTS   32768                           // slices of a sequence's rows that pass 2 can join (a byte of shared memory each)
 
 // order-preserving map of a float to an unsigned integer (larger float -> larger integer); 0 is left for "nothing"
@@ -28,26 +33,37 @@ __device__ __forceinline__ unsigned long long sel_key(double x) {
 __device__ __forceinline__ double sel_val(unsigned long long k) {
     return __longlong_as_double((long long) ((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));
 }
+__device__ __forceinline__ unsigned long long sel_max(uint32_t hi, uint32_t lo) {        // over the warp
+    const uint32_t h = __reduce_max_sync(0xffffffffu, hi);
+    return (unsigned long long) h << 32 | __reduce_max_sync(0xffffffffu, hi == h ? lo : 0u);
+}
 
-// The VEC consecutive logits of one thread, with the widest loads that the row's alignment allows.  Which thread sums which
-// logits does not depend on the alignment, so equal rows give equal bits wherever they lie.
-template <typename T, int VEC>
-__device__ __forceinline__ void sel_load(const T * p, int align, float (&x)[VEC]) {
-    static_assert(VEC * sizeof(T) == 16, "one 16-byte vector");
-    union { uint4 q; uint2 h[2]; uint32_t w[4]; T t[VEC]; } u;
+// 16 consecutive bytes of logits with the widest loads that the row's alignment allows.  Which lane sums which logits does not depend
+// on the alignment, so equal rows give equal bits wherever they lie.
+template <typename T>
+__device__ __forceinline__ uint4 sel_load(const T * p, int align) {
+    union { uint4 q; uint2 h[2]; uint32_t w[4]; T t[16 / sizeof(T)]; } u;
     if (align >= 16)      u.q = *(const uint4 *) p;
     else if (align == 8)  { u.h[0] = ((const uint2 *) p)[0]; u.h[1] = ((const uint2 *) p)[1]; }
     else if (align == 4)  { for (int i = 0; i < 4; ++i) u.w[i] = ((const uint32_t *) p)[i]; }
-    else                  { for (int i = 0; i < VEC; ++i) u.t[i] = p[i]; }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = (float) u.t[i];
+    else                  { for (int i = 0; i < 16 / (int) sizeof(T); ++i) u.t[i] = p[i]; }
+    return u.q;
 }
+template <typename T> __device__ __forceinline__ float sel_get(uint4 q, int i) { union { uint4 q; T t[16 / sizeof(T)]; } u; u.q = q; return (float) u.t[i]; }
 
 struct SelSlices {            // workspace of a call: [rows][n_slice] maxima and sums, [rows][n_slice][n_beam] best logits
     float * m; double * s; float * x; int32_t * v;
 };
 
-static __host__ __device__ inline int64_t sel_slices(int64_t n_vocab) { return (n_vocab + SEL_SLICE - 1) / SEL_SLICE; }
+// tiles of a slice: single tiles as long as larger slices would not fill the device (5 rows of 51866: 65 CTAs)
+static inline int sel_tiles(int64_t rows, int n_beam, int64_t n_vocab) {
+    const int64_t slices = (n_vocab + SEL_TILE * SEL_MANY - 1) / (SEL_TILE * SEL_MANY);
+    return rows * slices >= 148 * 2 || n_beam * ((n_vocab + SEL_TILE - 1) / SEL_TILE) > 4096 ? SEL_MANY : 1;
+}
+static inline int64_t sel_slices(int64_t rows, int n_beam, int64_t n_vocab) {
+    const int64_t size = SEL_TILE * sel_tiles(rows, n_beam, n_vocab);
+    return (n_vocab + size - 1) / size;
+}
 
 static inline SelSlices sel_layout(void * ws, int64_t rows, int64_t n_slice, int n_beam, int64_t * bytes) {
     const int64_t n = rows * n_slice;
@@ -61,126 +77,156 @@ static inline SelSlices sel_layout(void * ws, int64_t rows, int64_t n_slice, int
     return p;
 }
 
-__device__ __forceinline__ bool sel_row_live(const float * score, const uint8_t * done, int64_t row) {
-    return score[row] > -INFINITY && !(done && done[row]);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(SEL_THREADS)
+template <typename T, int NT>
+__global__ void __launch_bounds__(SEL_THREADS, NT == 1 ? 4 : 2)
 k_beam_scan(const char * logits, int64_t nb_row, int n_vocab, const float * score, const uint8_t * done,
             const uint32_t * banned, int64_t banned_stride, int n_beam, SelSlices out) {
-    constexpr int VEC = 16 / sizeof(T), NV = SEL_EPT / VEC, NW = SEL_THREADS / 32;
+    constexpr int VEC = 16 / sizeof(T), NV = NT * SEL_EPT / VEC, NW = SEL_THREADS / 32;
+    __shared__ double s_s[NW];
+    __shared__ unsigned long long s_top[NW * B200_BEAM_MAX], s_bound;
+    __shared__ unsigned long long s_cand[SEL_CAP];
+    __shared__ int s_n;
     chain_release();
     chain_wait();
     const int64_t row = blockIdx.x;
-    const int slice = blockIdx.y, n_slice = gridDim.y;
-    if (!sel_row_live(score, done, row)) return;
-    __shared__ float  s_m[NW];
-    __shared__ double s_s[NW];
-    __shared__ unsigned long long s_top[NW * B200_BEAM_MAX];
-    __shared__ unsigned long long s_cand[B200_BEAM_MAX * SEL_EPT];
-    __shared__ int s_n;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int slice = blockIdx.y, n_slice = gridDim.y, base = slice * SEL_TILE * NT;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const T * x_row = (const T *) (logits + row * nb_row);
-    const int align = (uintptr_t) x_row & 15 ? (int) ((uintptr_t) x_row & (~(uintptr_t) x_row + 1)) : 16;   // 2, 4, 8 or 16
-    const int base = slice * SEL_SLICE;
-    if (tid == 0) s_n = 0;
-
+    const int align = (uintptr_t) x_row & 15 ? (int) ((uintptr_t) x_row & (~(uintptr_t) x_row + 1)) : 16;      // 2, 4, 8 or 16
+    const float sc = score[row];
+    const uint8_t dn = done ? done[row] : 0;
+    auto first = [&](int j) { return base + (j * SEL_THREADS + tid) * VEC; };
     float x[NV][VEC];
+    if (n_vocab - base >= SEL_TILE * NT) {
+        uint4 raw[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int e = base + (j * SEL_THREADS + tid) * VEC;
-        if (e + VEC <= n_vocab) sel_load<T, VEC>(x_row + e, align, x[j]);
-        else {
+        for (int j = 0; j < NV; ++j) raw[j] = sel_load<T>(x_row + first(j), align);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) x[j][i] = e + i < n_vocab ? (float) x_row[e + i] : -INFINITY;
-        }
-    }
-    if (banned) {
-        const uint32_t * mask = banned + row * banned_stride;
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[j][i] = fmaxf(sel_get<T>(raw[j], i), -INFINITY);      // no NaN
+    } else {                                    // the row ends in this slice
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int e = base + (j * SEL_THREADS + tid) * VEC;
-            if (e < n_vocab) {              // VEC divides 32 and e is a multiple of it: one word covers the vector
-                const uint32_t w = mask[e >> 5] >> (e & 31);
+            const int e = first(j);
+            uint4 raw;
+            if (e + VEC <= n_vocab) raw = sel_load<T>(x_row + e, align);
+            else {
+                union { uint4 q; T t[VEC]; } u;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) if (w >> i & 1) x[j][i] = -INFINITY;
+                for (int i = 0; i < VEC; ++i) u.t[i] = (T) (e + i < n_vocab ? (float) x_row[e + i] : -INFINITY);
+                raw = u.q;
             }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[j][i] = fmaxf(sel_get<T>(raw, i), -INFINITY);
         }
     }
+    if (!(sc > -INFINITY) || dn) return;
+    if (banned) {
+        const uint32_t * mask = banned + row * banned_stride;
+        uint32_t w[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) w[j] = first(j) < n_vocab ? mask[first(j) >> 5] >> (first(j) & 31) : 0;      // VEC divides 32 and first(j) is a multiple of it
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) if (w[j] & (1u << i)) x[j][i] = -INFINITY;
+    }
     float m = -INFINITY;
-    int   mi = 0;                           // this thread's best logit: the lowest index among equals (indices ascend)
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            x[j][i] = x[j][i] >= -INFINITY ? x[j][i] + 0.0f : -INFINITY;      // no NaN, one zero
-            if (x[j][i] > m) { m = x[j][i]; mi = base + (j * SEL_THREADS + tid) * VEC + i; }
+        for (int i = 0; i < VEC; ++i) m = fmaxf(m, x[j][i]);
+    // the n_beam best thread maxima of each warp, best first, and from them the slice's maximum and its bound
+    auto tops = [&](uint32_t hi, uint32_t lo) {
+        for (int r = 0; r < n_beam; ++r) {
+            const unsigned long long top = sel_max(hi, lo);
+            if (lane == 0) s_top[warp * n_beam + r] = top;
+            if (hi == (uint32_t) (top >> 32) && lo == (uint32_t) top) hi = lo = 0;
         }
-    // the warp's n_beam best thread maxima, best first; their first one is the warp's maximum
-    uint32_t hi = m > -INFINITY ? sel_key(m) : 0, lo = hi ? ~(uint32_t) mi : 0;
-    for (int r = 0; r < n_beam; ++r) {
-        const uint32_t bh = __reduce_max_sync(0xffffffffu, hi);
-        const uint32_t bl = __reduce_max_sync(0xffffffffu, hi == bh ? lo : 0u);
-        if (lane == 0) {
-            s_top[r * NW + warp] = (unsigned long long) bh << 32 | bl;
-            if (r == 0) s_m[warp] = bh ? sel_val(bh) : -INFINITY;
+    };
+    const int n_top = NW * n_beam;
+    auto bound_of = [&]() {                     // the n_beam-th best of all; unique keys
+        if (tid < n_top) {
+            const unsigned long long k = s_top[tid];
+            int rank = 0;
+            for (int o = 0; o < n_top; ++o) rank += s_top[o] > k;
+            if (k && rank == n_beam - 1) s_bound = k;
         }
-        if (hi == bh && lo == bl) hi = lo = 0;
-    }
+    };
+    // first with the thread as the second part of the key
+    tops(m > -INFINITY ? sel_key(m + 0.0f) : 0, m > -INFINITY ? ~(uint32_t) tid : 0);
+    if (tid == 0) { s_n = 0; s_bound = 0; }     // fewer candidates than beams: all that there are
     __syncthreads();
-    float mx = s_m[0];
+    unsigned long long best = s_top[0];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, s_m[w]);
+    for (int w = 1; w < NW; ++w) best = s_top[w * n_beam] > best ? s_top[w * n_beam] : best;
     const int64_t at = row * n_slice + slice;
-    if (mx == -INFINITY) {
+    if (best == 0) {
         if (tid == 0) { out.m[at] = -INFINITY; out.s[at] = 0.0; }
         if (tid < n_beam) out.v[at * n_beam + tid] = -1;
         return;
     }
-    // sum of exp(x - mx): 16 terms per thread in f32, joined in f64
+    const float mx = sel_val((uint32_t) (best >> 32));
+    bound_of();
+    // sum of exp(x - mx): f32 within a thread, joined in f64
     float se = 0.0f;
+    if (mx < INFINITY) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) se += x[j][i] == mx ? 1.0f : __expf(x[j][i] - mx);
+            for (int i = 0; i < VEC; ++i) se += __expf(x[j][i] - mx);
+    } else {                                     // infinite logits share the row
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) se += x[j][i] == INFINITY ? 1.0f : 0.0f;
+    }
     double sd = se;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sd += __shfl_xor_sync(0xffffffffu, sd, o);
     if (lane == 0) s_s[warp] = sd;
-    // the n_beam-th best of the thread maxima bounds the slice's n_beam best from below, and the threads that reach it
-    // (n_beam of them) hold all of those: at most n_beam * SEL_EPT logits are left to be sorted
-    unsigned long long bound = 0;
-    {
-        unsigned long long k0[NW];          // lane r holds the r-th best of every warp
+    __syncthreads();
+    auto key = [&](int j, int i) { return (unsigned long long) sel_key(x[j][i] + 0.0f) << 32 | ~(uint32_t) (first(j) + i); };      // one zero
+    const float bar = s_bound ? sel_val((uint32_t) (s_bound >> 32)) : -INFINITY;
+    if (m >= bar && m > -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < NW; ++w) k0[w] = lane < n_beam ? s_top[lane * NW + w] : 0;
-        for (int r = 0; r < n_beam; ++r) {
-            unsigned long long b = 0;
+        for (int j = 0; j < NV; ++j) {
+            float v = x[j][0];
 #pragma unroll
-            for (int w = 0; w < NW; ++w) b = k0[w] > b ? k0[w] : b;
-            const uint32_t h = (uint32_t) (b >> 32), l = (uint32_t) b;
-            const uint32_t bh = __reduce_max_sync(0xffffffffu, h);
-            const uint32_t bl = __reduce_max_sync(0xffffffffu, h == bh ? l : 0u);
-            bound = (unsigned long long) bh << 32 | bl;
+            for (int i = 1; i < VEC; ++i) v = fmaxf(v, x[j][i]);
+            if (v >= bar && v > -INFINITY) {
 #pragma unroll
-            for (int w = 0; w < NW; ++w) if (k0[w] == bound) k0[w] = 0;
-        }
-    }
-    if (bound == 0) bound = 1;              // fewer candidates than beams: all that there are
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            if (x[j][i] > -INFINITY) {
-                const unsigned long long k = (unsigned long long) sel_key(x[j][i]) << 32 | ~(uint32_t) (base + (j * SEL_THREADS + tid) * VEC + i);
-                if (k >= bound) {
-                    const int p = atomicAdd(&s_n, 1);
-                    s_cand[p] = k;          // the order of arrival does not matter: they are ranked below
-                }
+                for (int i = 0; i < VEC; ++i)
+                    if (x[j][i] >= bar && x[j][i] > -INFINITY) {
+                        const int c = atomicAdd(&s_n, 1);
+                        if (c < SEL_CAP) s_cand[c] = key(j, i);      // the order of arrival does not matter: they are ranked
+                    }
             }
         }
+    }
     __syncthreads();
+    if (s_n > SEL_CAP) {                         // equal logits: the same once more with unique keys
+        unsigned long long mine = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) if (mine == 0 && x[j][i] == m && m > -INFINITY) mine = key(j, i);      // the lowest index: indices ascend
+        __syncthreads();
+        tops((uint32_t) (mine >> 32), (uint32_t) mine);
+        if (tid == 0) { s_n = 0; s_bound = 1; }
+        __syncthreads();
+        bound_of();
+        __syncthreads();
+        const unsigned long long bound = s_bound;
+        if (mine >= bound) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) if (x[j][i] > -INFINITY && key(j, i) >= bound) s_cand[atomicAdd(&s_n, 1)] = key(j, i);
+        }
+        __syncthreads();
+    }
     const int n = s_n;
     for (int c = tid; c < n; c += SEL_THREADS) {
         const unsigned long long k = s_cand[c];
@@ -192,17 +238,17 @@ k_beam_scan(const char * logits, int64_t nb_row, int n_vocab, const float * scor
         }
     }
     if (tid >= n && tid < n_beam) out.v[at * n_beam + tid] = -1;
-    if (tid == 0) {
-        double s = s_s[0];
+    if (tid == SEL_THREADS - 1) {
+        double sum = s_s[0];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) s += s_s[w];
-        out.m[at] = mx; out.s[at] = s;
+        for (int w = 1; w < NW; ++w) sum += s_s[w];
+        out.m[at] = mx; out.s[at] = sum;
     }
 }
 
 // One CTA per sequence.  The slices' sorted lists are the threads' (list l = beam * n_slice + slice belongs to thread l mod
 // blockDim): n_beam rounds of an arg-max over the lists' heads, each round one barrier.  Keys are (score as ordered 64-bit
-// integer, lowest beam * n_vocab + token).
+// integer, lowest beam * n_vocab + token).  Bound by latency; a warp per beam forms the logarithm of its sum.
 __global__ void __launch_bounds__(1024)
 k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam, int n_slice, int n_vocab, int eos,
             float * score_out, int32_t * token_out, int32_t * parent_out, uint8_t * done_out) {
@@ -214,26 +260,30 @@ k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam,
     __shared__ uint32_t s_hi[2][32], s_lo[2][32], s_ix[2][32];
     const int64_t row0 = (int64_t) blockIdx.x * n_beam;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warp = blockDim.x >> 5, n_list = n_beam * n_slice;
+    // heads of this thread's first list, under way while the sums are formed
+    float head_x = 0.0f;
+    int   head_v = -1;
+    if (tid < n_list) { const int64_t at = (row0 * n_slice + tid) * n_beam; head_x = in.x[at]; head_v = in.v[at]; }
     for (int b = warp; b < n_beam; b += n_warp) {
         const float sc = score[row0 + b];
         const bool d = done && done[row0 + b], ok = sc > -INFINITY, live = ok && !d;
-        float m = -INFINITY;
-        double s = 0.0;
-        if (live) {
-            for (int j = lane; j < n_slice; j += 32) m = fmaxf(m, in.m[(row0 + b) * n_slice + j]);
+        const float * bm = in.m + (row0 + b) * n_slice;
+        const double * bs = in.s + (row0 + b) * n_slice;
+        const float m0 = lane < n_slice ? bm[lane] : -INFINITY;             // (a row that is not live left nothing here: not used)
+        const double s0 = lane < n_slice ? bs[lane] : 0.0;
+        float m = m0;
+        for (int j = lane + 32; j < n_slice; j += 32) m = fmaxf(m, bm[j]);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (m > -INFINITY)
-                for (int j = lane; j < n_slice; j += 32) {
-                    const float mj = in.m[(row0 + b) * n_slice + j];
-                    if (mj == m) s += in.s[(row0 + b) * n_slice + j];
-                    else if (mj > -INFINITY) s += in.s[(row0 + b) * n_slice + j] * exp((double) mj - (double) m);
-                }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        double s = m0 == m ? s0 : m0 > -INFINITY ? s0 * (double) __expf(m0 - m) : 0.0;
+        for (int j = lane + 32; j < n_slice; j += 32) {
+            const float mj = bm[j];
+            s += mj == m ? bs[j] : mj > -INFINITY ? bs[j] * (double) __expf(mj - m) : 0.0;
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0) {
-            s_score[b] = sc; s_m[b] = m; s_log[b] = s > 0.0 ? log(s) : 0.0;
+            s_score[b] = sc; s_m[b] = m; s_log[b] = live && m > -INFINITY ? log(s) : 0.0;
             s_done[b] = d; s_live[b] = live && m > -INFINITY ? 1 : ok && d ? 2 : 0;
         }
     }
@@ -243,7 +293,7 @@ k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam,
     unsigned long long mine = 0;
     uint32_t mine_ix = 0;                    // ~(b * n_vocab + v) of this thread's best head, 0: none
     int mine_l = -1;
-    auto look = [&]() {                      // best head among this thread's lists
+    auto look = [&](bool start) {            // best head among this thread's lists
         mine = 0; mine_ix = 0; mine_l = -1;
         for (int l = tid; l < n_list; l += blockDim.x) {
             const int b = l / n_slice, sl = l - b * n_slice, h = s_head[l];
@@ -251,9 +301,9 @@ k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam,
             if (s_live[b] == 1) {
                 if (h >= n_beam) continue;
                 const int64_t at = ((row0 + b) * n_slice + sl) * n_beam + h;
-                tok = in.v[at];
+                tok = start && l == tid ? head_v : in.v[at];
                 if (tok < 0) continue;
-                const double x = in.x[at];
+                const double x = start && l == tid ? head_x : in.x[at];
                 v = s_score[b] + ((x == s_m[b] ? 0.0 : x - s_m[b]) - s_log[b]);
                 if (!(v > -INFINITY)) continue;
             } else if (s_live[b] == 2 && sl == 0 && h == 0) {
@@ -265,7 +315,7 @@ k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam,
             if (mine_l < 0 || k > mine || (k == mine && ix > mine_ix)) { mine = k; mine_ix = ix; mine_l = l; }
         }
     };
-    look();
+    look(true);
     for (int r = 0; r < n_beam; ++r) {
         const uint32_t h = (uint32_t) (mine >> 32), l = (uint32_t) mine;
         uint32_t bh = __reduce_max_sync(0xffffffffu, h);
@@ -289,25 +339,30 @@ k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam,
             parent_out[row0 + r] = b;
             done_out[row0 + r] = s_done[b] || tok == eos;
             ++s_head[mine_l];
-            look();
+            look(false);
         }
         if (none && tid == 0) { score_out[row0 + r] = -INFINITY; token_out[row0 + r] = -1; parent_out[row0 + r] = -1; done_out[row0 + r] = 1; }
     }
 }
 
+static bool sel_sizes_ok(int n_seq, int n_beam, int64_t n_vocab) {
+    return n_seq >= 0 && n_beam >= 1 && n_beam <= B200_BEAM_MAX && n_vocab >= 1 && n_vocab <= (1ll << 30) && n_vocab * n_beam < (1ll << 31) &&
+           n_beam * ((n_vocab + SEL_TILE * SEL_MANY - 1) / (SEL_TILE * SEL_MANY)) <= SEL_LISTS && (int64_t) n_seq * n_beam <= 0x7fffffff;
+}
+
 extern "C" int64_t b200_beam_select_workspace(int n_seq, int n_beam, int64_t n_vocab) {
-    if (n_seq < 0 || n_beam < 1 || n_beam > B200_BEAM_MAX || n_vocab < 1 || n_vocab >= (1ll << 31) || sel_slices(n_vocab) * n_beam > SEL_LISTS) return 0;
+    if (!sel_sizes_ok(n_seq, n_beam, n_vocab)) return 0;
     int64_t bytes;
-    sel_layout(nullptr, (int64_t) n_seq * n_beam, sel_slices(n_vocab), n_beam, &bytes);
+    const int64_t rows = (int64_t) n_seq * n_beam;
+    sel_layout(nullptr, rows, sel_slices(rows, n_beam, n_vocab), n_beam, &bytes);
     return bytes;
 }
 
 extern "C" int b200_beam_select(const b200_beam_select_args * a, void * stream) {
-    if (!a || a->n_seq < 0 || a->n_beam < 1 || a->n_beam > B200_BEAM_MAX || a->n_vocab < 1 || a->n_vocab >= (1ll << 31)) return B200_ERR_ARG;
-    const int64_t rows = (int64_t) a->n_seq * a->n_beam, n_slice = sel_slices(a->n_vocab);
-    if (n_slice * a->n_beam > SEL_LISTS) return B200_ERR_ARG;
+    if (!a || !sel_sizes_ok(a->n_seq, a->n_beam, a->n_vocab)) return B200_ERR_ARG;
+    const int64_t rows = (int64_t) a->n_seq * a->n_beam, n_slice = sel_slices(rows, a->n_beam, a->n_vocab);
     const int size = a->type == B200_TYPE_F32 ? 4 : a->type == B200_TYPE_F16 || a->type == B200_TYPE_BF16 ? 2 : 0;
-    if (!size || a->nb_row % size || a->nb_row < a->n_vocab * size || a->banned_stride < 0 || rows > 0x7fffffff) return B200_ERR_ARG;
+    if (!size || a->nb_row % size || a->nb_row < a->n_vocab * size || a->banned_stride < 0) return B200_ERR_ARG;
     if (a->n_seq == 0) return 0;
     if (!a->logits || !a->score || !a->score_out || !a->token_out || !a->parent_out || !a->done_out || (uintptr_t) a->logits % size) return B200_ERR_ARG;
     if (!a->workspace || (uintptr_t) a->workspace % 16 || a->workspace_bytes < b200_beam_select_workspace(a->n_seq, a->n_beam, a->n_vocab)) return B200_ERR_ARG;
@@ -315,13 +370,16 @@ extern "C" int b200_beam_select(const b200_beam_select_args * a, void * stream) 
     const SelSlices ws = sel_layout(a->workspace, rows, n_slice, a->n_beam, &bytes);
     const cudaStream_t st = as_stream(stream);
     const dim3 grid((unsigned) rows, (unsigned) n_slice);
-    auto scan = a->type == B200_TYPE_F32 ? k_beam_scan<float> : a->type == B200_TYPE_F16 ? k_beam_scan<__half> : k_beam_scan<__nv_bfloat16>;
+    const bool many = sel_tiles(rows, a->n_beam, a->n_vocab) > 1;
+    auto scan = a->type == B200_TYPE_F32 ? (many ? k_beam_scan<float, SEL_MANY> : k_beam_scan<float, 1>)
+              : a->type == B200_TYPE_F16 ? (many ? k_beam_scan<__half, SEL_MANY> : k_beam_scan<__half, 1>)
+                                         : (many ? k_beam_scan<__nv_bfloat16, SEL_MANY> : k_beam_scan<__nv_bfloat16, 1>);
     cudaError_t e = launch_chained(scan, grid, dim3(SEL_THREADS), 0, st, (const char *) a->logits, a->nb_row, (int) a->n_vocab, a->score, a->done,
                                    a->banned, a->banned_stride, a->n_beam, ws);
     if (e != cudaSuccess) return (int) e;
     B200_LAUNCHED();
-    const int64_t n_list = n_slice * a->n_beam;
-    const unsigned threads = (unsigned) (n_list >= 1024 ? 1024 : (n_list + 31) / 32 * 32);
+    const int64_t n_list = n_slice * a->n_beam, lanes = n_list > 32 * a->n_beam ? n_list : 32 * a->n_beam;
+    const unsigned threads = (unsigned) (lanes >= 1024 ? 1024 : (lanes + 31) / 32 * 32);
     e = launch_chained(k_beam_pick, dim3((unsigned) a->n_seq), dim3(threads), (size_t) n_list, st, ws, a->score, a->done, a->n_beam, (int) n_slice,
                        (int) a->n_vocab, (int) a->eos, a->score_out, a->token_out, a->parent_out, a->done_out);
     if (e != cudaSuccess) return (int) e;

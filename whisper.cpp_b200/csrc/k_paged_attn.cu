@@ -6,6 +6,8 @@
 
 bool b200_pool_ok(const b200_page_pool * p, bool data);    // k_pages.cu
 
+struct PaNew { const char * k; const char * v; int64_t nb_tok, nb_head; };      // new rows to be stored (type of q)
+
 // ---- store ---------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ uint4 pa_pack8(const float * x);
 template <> __device__ __forceinline__ uint4 pa_pack8<__half>(const float * x) {
@@ -32,7 +34,6 @@ template <> __device__ __forceinline__ void pa_unpack8<__nv_bfloat16>(uint4 q, f
     for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
 }
 
-struct PaNew { const char * k; const char * v; int64_t nb_tok, nb_head; };
 
 // one thread per 8 values; f32 is rounded to the pool's type (to nearest even: the cache's precision), 16-bit values are copied
 template <typename KV, bool F32>
@@ -75,7 +76,7 @@ k_paged_store(PaArgs a, PaNew x, int vec_head) {
 #define PA_ROWS  16
 #define PA_BLOCK 4096                            // bytes of a block of K or V: 32 keys of 64 or 16 of 128 dimensions
 #define PA_WARPS 4
-#define PA_MIN_CHUNK 256
+#define PA_MIN_ROUNDS 8
 #define PA_TC_MIN_ROWS 64
 
 template <typename T> struct PaPack;
@@ -127,23 +128,83 @@ __device__ __forceinline__ void pa_ldm_t(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3},[%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 
+// How the work is dealt out.  Items are (sequence, key/value head, tile of 16 rows), numbered in that order; an item of a sequence of n keys
+// is ceil(n / round) rounds of PA_WARPS blocks, at least one.  Either a CTA takes one item (a.stream = 0), or the rounds of all items are one
+// line that is cut into a.stream equal parts, one per CTA: whatever the lengths, all CTAs end together.  On the line an item begins with
+// PA_START rounds of nothing, the time that it takes to get its first keys.  A CTA then has up to two partial items, at the ends of its
+// part; it leaves them in slots 0 (an item begun by another CTA) and 1, and k_paged_join puts them together.
+// (64 sequences of 1 to 8192 keys: 224 us without it, 183 with 2, 181 with 4 or 8.)
+#define PA_START 3
+struct PaLine { int64_t total, before; };                 // rounds of all sequences, and of those before a given one
+__device__ __forceinline__ int64_t pa_rounds(const PaArgs & a, const PaSeq & s, int round) {
+    return (int64_t) ((s.n_new * a.group + PA_ROWS - 1) / PA_ROWS) * a.n_head_kv * (max(1, (s.len + round - 1) / round) + PA_START);
+}
+// this warp's lanes go over the sequences, a run of them each
+__device__ __forceinline__ PaLine pa_line(const PaArgs & a, int round, int64_t target, int upto, int * seq_at, int64_t * rest) {
+    const int lane = threadIdx.x & 31, per = (a.n_seq + 31) / 32, s0 = min(a.n_seq, lane * per), s1 = min(a.n_seq, s0 + per);
+    int64_t mine = 0;
+    for (int s = s0; s < s1; ++s) mine += pa_rounds(a, pa_seq(a, s), round);
+    int64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int64_t u = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += u; }
+    PaLine l;
+    l.total = __shfl_sync(0xffffffffu, inc, 31);
+    l.before = 0;
+    if (upto >= 0) {                                       // rounds before sequence `upto`
+        int64_t b = inc - mine;
+        if (upto >= s0 && upto < s1) for (int s = s0; s < upto; ++s) b += pa_rounds(a, pa_seq(a, s), round);
+        l.before = __shfl_sync(0xffffffffu, b, upto / per);
+    }
+    if (seq_at) {                                          // the sequence that holds round target * total / a.stream
+        const int64_t w = target * l.total / a.stream;
+        const bool here = w >= inc - mine && w < inc;
+        int s = s0;
+        int64_t left = w - (inc - mine);
+        if (here) for (; s < s1; ++s) { const int64_t r = pa_rounds(a, pa_seq(a, s), round); if (left < r) break; left -= r; }
+        const unsigned who = __ballot_sync(0xffffffffu, here);
+        const int src = who ? __ffs(who) - 1 : 0;
+        *seq_at = who ? __shfl_sync(0xffffffffu, s, src) : a.n_seq;
+        *rest = __shfl_sync(0xffffffffu, left, src);
+    }
+    return l;
+}
+
+
 template <typename Q, typename KV, int D>
-__global__ void __launch_bounds__(32 * PA_WARPS)
-k_paged_attn(PaArgs a) {
+__global__ void __launch_bounds__(32 * PA_WARPS, PaParts<Q, KV>::n == 1 ? 3 : 2)
+k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw) {
     using P = PaPack<KV>;
     constexpr int NP = PaParts<Q, KV>::n, NC = D / 8, KS = D / 16;      // parts, 16-byte chunks and MMA steps of a head
     constexpr float LIFT = PaParts<Q, KV>::lift;
-    constexpr int BLOCK = PA_BLOCK, KEYS = BLOCK / (2 * D), NK = KEYS / 8;       // keys of a block, MMA columns of its scores
+    constexpr int BLOCK = PA_BLOCK, KEYS = BLOCK / (2 * D), NK = KEYS / 8, ROUND = KEYS * PA_WARPS;      // keys of a block, MMA columns of its scores
     extern __shared__ __align__(16) char smem[];
-    chain_release();
+    // The successor is let in only when CTAs end: brought in early, the CTAs of the join and of the next call took the places of this kernel's
+    // own (111 sequences of 4096 keys: 121 us a call, 85 without).
     chain_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int seq = blockIdx.z / a.n_split, split = blockIdx.z % a.n_split, kvh = blockIdx.y, row0 = blockIdx.x * PA_ROWS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // the shuffle tells the compiler that the warp agrees
+    int seq, kvh, tile, at = 0;                           // the item, and where in it (on the line) this CTA begins
+    int64_t todo = 1ll << 60;                             // what is left of this CTA's part
+    if (a.stream) {
+        int64_t rest;
+        const PaLine l = pa_line(a, ROUND, blockIdx.x, -1, &seq, &rest);
+        todo = ((int64_t) blockIdx.x + 1) * l.total / a.stream - (int64_t) blockIdx.x * l.total / a.stream;
+        if (seq >= a.n_seq || todo == 0) return;
+        const PaSeq s = pa_seq(a, seq);
+        const int rounds = max(1, (s.len + ROUND - 1) / ROUND), tiles = (s.n_new * a.group + PA_ROWS - 1) / PA_ROWS;
+        const int64_t item = rest / (rounds + PA_START);
+        at = (int) (rest - item * (rounds + PA_START));
+        kvh = (int) (item / tiles);
+        tile = (int) (item - (int64_t) kvh * tiles);
+    } else { seq = blockIdx.z; kvh = blockIdx.y; tile = gridDim.x - 1 - blockIdx.x; }      // the longest tiles first
+    for (;;) {
     const PaSeq s = pa_seq(a, seq);
-    const int n_rows = s.n_new * a.group;
-    if (row0 >= n_rows) return;
-    const int k0 = split * a.chunk, k1 = min(pa_reach(a, s, row0), k0 + a.chunk);
-    if (k0 >= k1 && split != 0) return;                  // an empty split: the join does not read it
+    const int n_rows = s.n_new * a.group, row0 = tile * PA_ROWS;
+    if (!a.stream && row0 >= n_rows) return;
+    const int rounds = max(1, (s.len + ROUND - 1) / ROUND), steps = (int) min((int64_t) (rounds + PA_START - at), todo);
+    const int first_round = max(0, at - PA_START), n_round = max(0, at + steps - PA_START) - first_round;
+    const int k0 = first_round * ROUND, k1 = min(pa_reach(a, s, row0), k0 + n_round * ROUND);
+    const bool whole = n_round == rounds;
+    if (n_round > 0) {
 
     const char * kp = a.k + kvh * a.nb_head, * vp = a.v + kvh * a.nb_head;
     const int32_t * table = a.tables + seq * a.table_stride;
@@ -151,18 +212,43 @@ k_paged_attn(PaArgs a) {
     const int n_block = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0, n_mine = (n_block - warp + PA_WARPS - 1) / PA_WARPS;
     auto key_of = [&](int i) { return k0 + (i * PA_WARPS + warp) * KEYS + lane; };
     auto page_of = [&](int i) { const int key = key_of(i); return i < n_mine && lane < KEYS && key < k1 ? table[key / a.page_size] : -1; };
+    const int new0 = nw.k ? s.len - s.n_new : 1 << 30;    // from here on K and V come from the new rows
     auto at_of = [&](int i, int page) -> int64_t {       // this lane's key's place in the pool, -1: none
         int64_t at = page >= 0 && page < a.n_pages ? page * a.nb_page + (key_of(i) % a.page_size) * a.nb_tok : -1;
         asm volatile("" : "+l"(at));                     // kept: the compiler computes it again for every chunk otherwise, division included
         return at;
     };
-    auto load = [&](int i, int64_t at, const char * base, uint32_t dst) {
+    // a block of K or V into its stage.  New rows are read where the caller has them; the last tile, which
+    // sees them all, also writes them to their pages
+    auto load = [&](int i, int64_t at, bool is_v, uint32_t dst) {
         if (i < n_mine) {
+            const char * base = is_v ? vp : kp;
+            const int key0 = k0 + (i * PA_WARPS + warp) * KEYS;
+            if (key0 + KEYS <= new0) {
 #pragma unroll
-            for (int c = 0; c < NC * KEYS / 32; ++c) {
-                const int x = c * 32 + lane, r = x / NC, ch = x % NC;
-                const int64_t off = __shfl_sync(0xffffffffu, at, r);
-                pa_cp16(dst + r * D * 2 + ((ch ^ (r & 7)) << 4), base + (off < 0 ? 0 : off + ch * 16), off >= 0);
+                for (int c = 0; c < NC * KEYS / 32; ++c) {
+                    const int x = c * 32 + lane, r = x / NC, ch = x % NC;
+                    const int64_t off = __shfl_sync(0xffffffffu, at, r);
+                    pa_cp16(dst + r * D * 2 + ((ch ^ (r & 7)) << 4), base + (off < 0 ? 0 : off + ch * 16), off >= 0);
+                }
+            } else {
+#pragma unroll 2
+                for (int c = 0; c < NC * KEYS / 32; ++c) {
+                    const int x = c * 32 + lane, r = x / NC, ch = x % NC;
+                    const int64_t off = __shfl_sync(0xffffffffu, at, r);
+                    const uint32_t d = dst + r * D * 2 + ((ch ^ (r & 7)) << 4);
+                    if (key0 + r < new0 || off < 0) { pa_cp16(d, base + (off < 0 ? 0 : off + ch * 16), off >= 0); continue; }
+                    const char * src = (is_v ? nw.v : nw.k) + (s.tok0 + key0 + r - new0) * nw.nb_tok + kvh * nw.nb_head;
+                    uint4 q;
+                    if constexpr (NP > 1) {
+                        float f[8];
+                        *(float4 *) f = ((const float4 *) src)[2 * ch];
+                        *(float4 *) (f + 4) = ((const float4 *) src)[2 * ch + 1];
+                        q = pa_pack8<KV>(f);
+                    } else q = ((const uint4 *) src)[ch];
+                    *(uint4 *) (smem + (d - pa_smem(smem))) = q;
+                    if ((tile + 1) * PA_ROWS >= n_rows) *(uint4 *) (const_cast<char *>(base) + off + ch * 16) = q;
+                }
             }
         }
         pa_commit();
@@ -171,8 +257,8 @@ k_paged_attn(PaArgs a) {
     {
         const int p0 = page_of(0), p1 = page_of(1);
         const int64_t at0 = at_of(0, p0), at1 = at_of(1, p1);
-        load(0, at0, kp, ring); load(0, at0, vp, ring + 2 * BLOCK);
-        load(1, at1, kp, ring + BLOCK); load(1, at1, vp, ring + 3 * BLOCK);
+        load(0, at0, false, ring); load(0, at0, true, ring + 2 * BLOCK);
+        load(1, at1, false, ring + BLOCK); load(1, at1, true, ring + 3 * BLOCK);
     }
     int page_next = page_of(2);
 
@@ -259,7 +345,7 @@ k_paged_attn(PaArgs a) {
                 }
         }
         __syncwarp();
-        load(i + 2, at_next, kp, kb);
+        load(i + 2, at_next, false, kb);
         const bool edge = key0 + KEYS - 1 > first_last || key0 + KEYS > k1;
         float xa = -INFINITY, xb = -INFINITY;
 #pragma unroll
@@ -347,7 +433,7 @@ k_paged_attn(PaArgs a) {
                 }
         }
         __syncwarp();
-        load(i + 2, at_next, vp, vb);
+        load(i + 2, at_next, true, vb);
     }
     pa_wait<0>();
 #pragma unroll
@@ -385,24 +471,82 @@ k_paged_attn(PaArgs a) {
         }
         const int t = row / a.group, h = kvh * a.group + row % a.group;
         const int64_t out = (s.tok0 + t) * a.n_head + h;
-        if (a.n_split == 1) {
+        if (whole) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             char * dst = a.dst + (s.tok0 + t) * a.nb_dst_tok + h * a.nb_dst_head + d * sizeof(Q);
             if constexpr (NP == 1) *(uint2 *) dst = make_uint2(P::two(x[0] * inv, x[1] * inv), P::two(x[2] * inv, x[3] * inv));
             else *(float4 *) dst = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
             if (a.lse && d == 0) a.lse[out] = sum == 0.0f ? -INFINITY : mx * 0.69314718f + logf(sum);
         } else {
-            float * p = a.part + (split * a.n_tok * a.n_head + out) * (D + 4);
+            float * p = a.part + (((int64_t) blockIdx.x * 2 + (first_round == 0)) * PA_ROWS + r) * (D + 4);
             *(float4 *) (p + d) = make_float4(x[0], x[1], x[2], x[3]);
             if (d == 0) { p[D] = mx; p[D + 1] = sum; }
         }
     }
+    }
+    // the next item of this CTA's part
+    todo -= steps;
+    if (!a.stream || todo == 0) return;
+    at = 0;
+    if (++tile * PA_ROWS >= n_rows) {
+        tile = 0;
+        if (++kvh == a.n_head_kv) {
+            kvh = 0;
+            do { if (++seq >= a.n_seq) return; } while (pa_seq(a, seq).n_new == 0);
+        }
+    }
+    __syncthreads();                                      // the accumulators are read before the ring is filled again
+    }
 }
 
-// joins the splits of a row: one warp per row
+// Joins the partial items: one warp per row of a sequence.  An item's rounds lie in CTAs c0 .. c1 of the line; the first left its part in
+// slot 1, the others in slot 0.
 template <typename Q, int D>
 __global__ void __launch_bounds__(128)
-k_paged_join(PaArgs a) {
+k_paged_join(const __grid_constant__ PaArgs a) {
+    constexpr int DL = D / 32, ROUND = PA_BLOCK / (2 * D) * PA_WARPS;
+    chain_release();
+    chain_wait();
+    const int lane = threadIdx.x & 31, seq = blockIdx.y;
+    const PaSeq s = pa_seq(a, seq);
+    if (s.n_new == 0) return;
+    const PaLine l = pa_line(a, ROUND, 0, seq, nullptr, nullptr);
+    const int rounds = max(1, (s.len + ROUND - 1) / ROUND), tiles = (s.n_new * a.group + PA_ROWS - 1) / PA_ROWS;
+    for (int64_t w = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 5); w < (int64_t) s.n_new * a.n_head; w += (int64_t) gridDim.x * 4) {
+        const int t = (int) (w / a.n_head), h = (int) (w - (int64_t) t * a.n_head), kvh = h / a.group, row = t * a.group + h % a.group;
+        const int64_t p0 = l.before + ((int64_t) kvh * tiles + row / PA_ROWS) * (rounds + PA_START) + PA_START;      // its first round
+        const int64_t c0 = ((p0 + 1) * a.stream - 1) / l.total, c1 = ((p0 + rounds) * a.stream - 1) / l.total;      // CTA c: from c * total / stream on
+        if (c0 == c1) continue;
+        const int n = (int) (c1 - c0 + 1);
+        auto part = [&](int i) { return a.part + (((c0 + i) * 2 + (i == 0)) * PA_ROWS + row % PA_ROWS) * (D + 4); };
+        float mx = -INFINITY;
+        auto some = [&](int i) { return (c0 + i + 1) * l.total / a.stream > (c0 + i) * l.total / a.stream; };       // fewer rounds than CTAs leave some without
+        for (int i = lane; i < n; i += 32) if (some(i)) mx = fmaxf(mx, part(i)[D]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        float sum = 0.0f, acc[DL] = {};
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            if (l.total < a.stream && !some(i)) continue;
+            const float * p = part(i);
+            const float f = exp2f(p[D] - base);
+            sum += f * p[D + 1];                          // NaN of a part without a finite maximum stays NaN
+#pragma unroll
+            for (int j = 0; j < DL; ++j) { const float v = p[lane * DL + j]; if (f != 0.0f) acc[j] += f * v; }
+        }
+        const int64_t out = (s.tok0 + t) * a.n_head + h;
+#pragma unroll
+        for (int j = 0; j < DL; ++j)
+            ((Q *) (a.dst + (s.tok0 + t) * a.nb_dst_tok + h * a.nb_dst_head))[lane * DL + j] = (Q) (sum == 0.0f ? 0.0f : acc[j] / sum);
+        if (a.lse && lane == 0) a.lse[out] = sum == 0.0f ? -INFINITY : mx * 0.69314718f + logf(sum);
+    }
+}
+
+// joins the splits of the tcgen05 form: one warp per row
+template <typename Q, int D>
+__global__ void __launch_bounds__(128)
+k_paged_join_tc(PaArgs a) {
     chain_release();
     chain_wait();
     constexpr int DL = D / 32;
@@ -454,23 +598,35 @@ static bool pa_args_ok(const b200_page_pool * p, const b200_paged_attn_args * a,
     return a->scale == a->scale && a->scale - a->scale == 0.0f;        // finite
 }
 
-// which kernel, keys per split and number of splits
-struct PaPlan { bool tc; int n_split, chunk; };
+// Which kernel, and how its work is dealt out.
+struct PaPlan { bool tc, store; int n_split, chunk, stream; };
 static PaPlan pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a) {
-    PaPlan r;
+    PaPlan r = {};
     const int64_t group = a->n_head / p->n_head_kv;
-    const int64_t rows = (a->max_new < a->n_tok ? a->max_new : a->n_tok) * group;
+    const int64_t new_max = a->max_new < a->n_tok ? a->max_new : a->n_tok, rows = new_max * group;
     r.tc = a->q_type != B200_TYPE_F32 && rows > PA_TC_MIN_ROWS;
-    const int64_t tile = r.tc ? PA_TC_ROWS : PA_ROWS;
-    const int64_t ctas = (rows + tile - 1) / tile * p->n_head_kv * a->n_seq;
-    const int64_t resident = 148 * (r.tc ? (p->head_dim == 64 ? 2 : 1) : 3);
-    const int64_t least = r.tc ? 512 : PA_MIN_CHUNK;
-    int64_t want = ((r.tc ? 1 : 3) * resident + ctas - 1) / ctas, most = (a->max_len + least - 1) / least;
-    if (r.tc && ctas * 2 > resident) want = 1;
+    r.n_split = 1;
+    if (!r.tc) {
+        r.store = a->k_new && new_max > PA_ROWS;           // few new rows are stored by the kernel itself
+        const int64_t tiles = (rows + PA_ROWS - 1) / PA_ROWS, items = tiles * p->n_head_kv * a->n_seq, round = PA_BLOCK / (2 * p->head_dim) * PA_WARPS;
+        const int64_t rounds = (a->max_len + round - 1) / round, resident = 148 * (a->q_type == B200_TYPE_F32 ? 2 : 3);
+        // Items of few rounds are not worth the join, and many tiles of a chunk fill the device by themselves (their reach differs, which
+        // the line does not know).
+        if (rounds >= PA_MIN_ROUNDS && (tiles == 1 || items < 2 * resident)) {
+            const int64_t want = items * rounds / (PA_MIN_ROUNDS / 2);
+            r.stream = (int) (want < resident ? want : resident);
+        }
+        return r;
+    }
+    r.store = a->k_new != nullptr;
+    const int64_t ctas = (rows + PA_TC_ROWS - 1) / PA_TC_ROWS * p->n_head_kv * a->n_seq;
+    const int64_t resident = 148 * (p->head_dim == 64 ? 2 : 1);
+    int64_t want = (resident + ctas - 1) / ctas, most = (a->max_len + 511) / 512;
+    if (ctas * 2 > resident) want = 1;
     if (want > most) want = most;
     if (want > 64) want = 64;
     if (want < 1) want = 1;
-    const int64_t step = 128;          // a multiple of the blocks of both kernels
+    const int64_t step = 128;          // a multiple of the blocks
     int64_t c = ((a->max_len + want - 1) / want + step - 1) / step * step;
     if (c < step) c = step;
     r.chunk = (int) c;
@@ -483,6 +639,7 @@ extern "C" int64_t b200_paged_attn_workspace(const b200_page_pool * pool, const 
     if (!a || !b200_pool_ok(pool, true) || a->n_tok < 1 || a->n_seq < 1 || a->max_new < 1 || a->max_len < 0 || a->max_len >= (1ll << 30) ||
         a->n_head < 1 || a->n_head % pool->n_head_kv) return 0;
     const PaPlan r = pa_plan(pool, a);
+    if (!r.tc) return (int64_t) r.stream * 2 * PA_ROWS * (pool->head_dim + 4) * 4;
     return r.n_split == 1 ? 0 : (int64_t) r.n_split * a->n_tok * a->n_head * (pool->head_dim + 4) * 4;
 }
 
@@ -520,24 +677,26 @@ extern "C" int b200_paged_store(const b200_page_pool * pool, const b200_paged_at
 }
 
 template <typename Q, typename KV, int D>
-static cudaError_t pa_launch(PaArgs & k, int n_seq, cudaStream_t st) {
+static cudaError_t pa_launch(PaArgs & k, const PaNew & x, int n_seq, cudaStream_t st) {
     cudaError_t e;
+    const int64_t rows = (int64_t) k.max_new * k.n_head;
+    const dim3 join((unsigned) (rows < 16384 ? (rows + 3) / 4 : 4096), (unsigned) n_seq);
     if (k.tile_rows == PA_TC_ROWS) {
         e = pa_tc_launch(k, D, std::is_same<KV, __half>::value ? B200_TYPE_F16 : B200_TYPE_BF16, n_seq, st);
-        if (e != cudaSuccess) return e;
+        if (e != cudaSuccess || k.n_split == 1) return e;
+        e = launch_chained(k_paged_join_tc<Q, D>, join, dim3(128), 0, st, k);
     } else {
-    const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
-    constexpr int smem = 4 * PA_WARPS * PA_BLOCK;
-    e = cudaFuncSetAttribute(k_paged_attn<Q, KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    e = launch_chained(k_paged_attn<Q, KV, D>, dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) (n_seq * k.n_split)), dim3(32 * PA_WARPS), smem, st, k);
-    if (e != cudaSuccess) return e;
-    B200_LAUNCHED();
+        constexpr int smem = 4 * PA_WARPS * PA_BLOCK;
+        e = cudaFuncSetAttribute(k_paged_attn<Q, KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
+        const dim3 grid = k.stream ? dim3((unsigned) k.stream) : dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) n_seq);
+        e = launch_chained(k_paged_attn<Q, KV, D>, grid, dim3(32 * PA_WARPS), smem, st, k, x);
+        if (e != cudaSuccess) return e;
+        B200_LAUNCHED();
+        if (!k.stream) return cudaGetLastError();
+        e = launch_chained(k_paged_join<Q, D>, join, dim3(128), 0, st, k);
     }
-    if (k.n_split == 1) return cudaGetLastError();
-    int64_t n = ((int64_t) k.max_new * k.n_head + 3) / 4;
-    if (n > 4096) n = 4096;
-    e = launch_chained(k_paged_join<Q, D>, dim3((unsigned) n, (unsigned) n_seq), dim3(128), 0, st, k);
     if (e == cudaSuccess) B200_LAUNCHED();
     return e;
 }
@@ -547,22 +706,23 @@ extern "C" int b200_paged_attn(const b200_page_pool * pool, const b200_paged_att
     if (a->n_seq == 0 || a->n_tok == 0 || a->max_new == 0) return 0;
     PaArgs k = pa_pack(pool, a);
     const PaPlan r = pa_plan(pool, a);
-    k.n_split = r.n_split; k.chunk = r.chunk; k.tile_rows = r.tc ? PA_TC_ROWS : PA_ROWS;
+    k.n_split = r.n_split; k.chunk = r.chunk; k.stream = r.stream; k.tile_rows = r.tc ? PA_TC_ROWS : PA_ROWS; k.n_seq = a->n_seq;
     const int64_t need = b200_paged_attn_workspace(pool, a);
     if (need && (!a->workspace || (uintptr_t) a->workspace % 16 || a->workspace_bytes < need)) return B200_ERR_ARG;
     if ((int64_t) a->n_seq * k.n_split > 65535) return B200_ERR_ARG;
-    if (a->k_new) {
+    if (r.store) {
         const int rc = b200_paged_store(pool, a, stream);
         if (rc) return rc;
     }
     const cudaStream_t st = as_stream(stream);
     const bool f32 = a->q_type == B200_TYPE_F32, h = pool->type == B200_TYPE_F16;
+    const PaNew x = { r.store ? nullptr : (const char *) a->k_new, (const char *) a->v_new, a->nb_new_tok, a->nb_new_head };
     cudaError_t e;
     if (pool->head_dim == 64)
-        e = f32 ? (h ? pa_launch<float, __half, 64>(k, a->n_seq, st) : pa_launch<float, __nv_bfloat16, 64>(k, a->n_seq, st))
-                : (h ? pa_launch<__half, __half, 64>(k, a->n_seq, st) : pa_launch<__nv_bfloat16, __nv_bfloat16, 64>(k, a->n_seq, st));
+        e = f32 ? (h ? pa_launch<float, __half, 64>(k, x, a->n_seq, st) : pa_launch<float, __nv_bfloat16, 64>(k, x, a->n_seq, st))
+                : (h ? pa_launch<__half, __half, 64>(k, x, a->n_seq, st) : pa_launch<__nv_bfloat16, __nv_bfloat16, 64>(k, x, a->n_seq, st));
     else
-        e = f32 ? (h ? pa_launch<float, __half, 128>(k, a->n_seq, st) : pa_launch<float, __nv_bfloat16, 128>(k, a->n_seq, st))
-                : (h ? pa_launch<__half, __half, 128>(k, a->n_seq, st) : pa_launch<__nv_bfloat16, __nv_bfloat16, 128>(k, a->n_seq, st));
+        e = f32 ? (h ? pa_launch<float, __half, 128>(k, x, a->n_seq, st) : pa_launch<float, __nv_bfloat16, 128>(k, x, a->n_seq, st))
+                : (h ? pa_launch<__half, __half, 128>(k, x, a->n_seq, st) : pa_launch<__nv_bfloat16, __nv_bfloat16, 128>(k, x, a->n_seq, st));
     return (int) e;
 }

@@ -172,9 +172,8 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
     using L = PtSmem<D, BN, NS>;
     constexpr int COLS = 2 * BN + 2 * D <= 256 ? 256 : 512, NC = D / 8;
     extern __shared__ __align__(16) char smem_raw[];
-    chain_release();
-    chain_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    chain_wait();                                         // no early release: this kernel wants whole SMs
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // the shuffle tells the compiler that the warp agrees
     const int seq = blockIdx.z / a.n_split, split = blockIdx.z % a.n_split, kvh = blockIdx.y;
     const int row0 = (gridDim.x - 1 - blockIdx.x) * PA_TC_ROWS;         // the longest tiles first
     const PaSeq s = pa_seq(a, seq);

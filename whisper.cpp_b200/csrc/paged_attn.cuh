@@ -9,9 +9,9 @@ struct PaArgs {
     const char * k; const char * v; int64_t nb_page, nb_tok, nb_head;
     const int32_t * tables; int64_t table_stride; const int32_t * lens; const int32_t * q_start;
     float * lse;
-    float * part;                   // [split][n_tok * n_head] x (head_dim + 4): sums, maximum, sum of weights, pad
+    float * part;                   // partial rows: head_dim sums, maximum, sum of weights, pad (head_dim + 4 floats)
     int64_t n_tok, max_len;
-    int n_pages, page_size, n_head, n_head_kv, group, max_new, causal, n_split, chunk, tile_rows;
+    int n_pages, page_size, n_head, n_head_kv, group, max_new, causal, n_split, chunk, tile_rows, stream, n_seq;
     float scale_log2;               // scale * log2(e): weights are powers of two
 };
 

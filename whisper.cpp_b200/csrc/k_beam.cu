@@ -8,15 +8,16 @@
 // score(b, v) = score[b] + (x - m) - log(sum exp(x - m)).  Within a row the order of the candidates is the order of the
 // logits, so a row's n_beam best logits are all it can contribute: pass 1 cuts every row into slices and leaves, per slice,
 // its maximum, its sum of exponentials and its n_beam best logits; pass 2 joins the slices of a sequence's rows and picks
-// the n_beam best of their sorted lists.  The logits are read once and stay in registers.  The n_beam-th best of the threads' maxima
-// bounds the slice's n_beam best from below, so that only logits that reach it are looked at one by one: about n_beam of them.  Where
-// equal logits make them many (more than SEL_CAP), the bound is taken once more with the index as the second part of the key; then the
-// n_beam threads that reach it hold all that do.  (A sorted list per warp, filled tile by tile, cost more in insertions: 65 us for 320
-// rows of 51866.)
+// the n_beam best of their sorted lists.  The logits are read once and stay in registers.  With the slice in 8 (or 32) groups, the n_beam-th
+// best of the groups' maxima bounds the slice's n_beam best from below, and about 7 logits reach it (5 beams, 8 groups: 8/8 + 8/7 + .. + 8/4):
+// only those are looked at one by one.  Where equal logits make them more than SEL_CAP, the bound is taken once more over the threads' maxima
+// with the index as the second part of the key; then the n_beam threads that reach it hold all that do.
+// 320 rows of 51866 (f32): 65 us with a sorted list per warp, filled tile by tile; 35 with the n_beam best thread maxima of every warp as the
+// bound and slices of four tiles (two CTAs an SM), 27 with two tiles (four CTAs).
 #define SEL_THREADS 256
 #define SEL_EPT     16                              // logits per thread and tile
 #define SEL_TILE    (SEL_THREADS * SEL_EPT)
-#define SEL_MANY    4                               // tiles of a slice where rows are many (64 logits per thread); one tile otherwise
+#define SEL_MANY    2                               // tiles of a slice where rows are many (32 logits per thread); one tile otherwise
 #define SEL_CAP     (B200_BEAM_MAX * SEL_EPT * SEL_MANY)
 #define SEL_LISTS   32768                           // slices of a sequence's rows that pass 2 can join (a byte of shared memory each)
 
@@ -37,6 +38,9 @@ __device__ __forceinline__ unsigned long long sel_max(uint32_t hi, uint32_t lo) 
     const uint32_t h = __reduce_max_sync(0xffffffffu, hi);
     return (unsigned long long) h << 32 | __reduce_max_sync(0xffffffffu, hi == h ? lo : 0u);
 }
+
+// 2^x; below 2^-126 it is 0 (the plain form spends four more instructions on those)
+__device__ __forceinline__ float sel_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // 16 consecutive bytes of logits with the widest loads that the row's alignment allows.  Which lane sums which logits does not depend
 // on the alignment, so equal rows give equal bits wherever they lie.
@@ -78,11 +82,12 @@ static inline SelSlices sel_layout(void * ws, int64_t rows, int64_t n_slice, int
 }
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(SEL_THREADS, NT == 1 ? 4 : 2)
+__global__ void __launch_bounds__(SEL_THREADS, 4)
 k_beam_scan(const char * logits, int64_t nb_row, int n_vocab, const float * score, const uint8_t * done,
             const uint32_t * banned, int64_t banned_stride, int n_beam, SelSlices out) {
     constexpr int VEC = 16 / sizeof(T), NV = NT * SEL_EPT / VEC, NW = SEL_THREADS / 32;
     __shared__ double s_s[NW];
+    __shared__ float s_grp[32];
     __shared__ unsigned long long s_top[NW * B200_BEAM_MAX], s_bound;
     __shared__ unsigned long long s_cand[SEL_CAP];
     __shared__ int s_n;
@@ -137,45 +142,40 @@ k_beam_scan(const char * logits, int64_t nb_row, int n_vocab, const float * scor
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) m = fmaxf(m, x[j][i]);
-    // the n_beam best thread maxima of each warp, best first, and from them the slice's maximum and its bound
-    auto tops = [&](uint32_t hi, uint32_t lo) {
-        for (int r = 0; r < n_beam; ++r) {
-            const unsigned long long top = sel_max(hi, lo);
-            if (lane == 0) s_top[warp * n_beam + r] = top;
-            if (hi == (uint32_t) (top >> 32) && lo == (uint32_t) top) hi = lo = 0;
-        }
-    };
-    const int n_top = NW * n_beam;
-    auto bound_of = [&]() {                     // the n_beam-th best of all; unique keys
-        if (tid < n_top) {
-            const unsigned long long k = s_top[tid];
-            int rank = 0;
-            for (int o = 0; o < n_top; ++o) rank += s_top[o] > k;
-            if (k && rank == n_beam - 1) s_bound = k;
-        }
-    };
-    // first with the thread as the second part of the key
-    tops(m > -INFINITY ? sel_key(m + 0.0f) : 0, m > -INFINITY ? ~(uint32_t) tid : 0);
-    if (tid == 0) { s_n = 0; s_bound = 0; }     // fewer candidates than beams: all that there are
-    __syncthreads();
-    unsigned long long best = s_top[0];
+    // groups: the warps, or eight lanes each
+    const int n_grp = n_beam <= NW ? NW : 32;
+    float g = m;
 #pragma unroll
-    for (int w = 1; w < NW; ++w) best = s_top[w * n_beam] > best ? s_top[w * n_beam] : best;
+    for (int o = 1; o < 8; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (n_beam <= NW) {
+        g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 8));
+        g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 16));
+        if (lane == 0) s_grp[warp] = g;
+    } else if ((lane & 7) == 0) s_grp[warp * 4 + (lane >> 3)] = g;
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    // every warp: the best group, and the n_beam-th best
+    const float mine = lane < n_grp ? s_grp[lane] : -INFINITY;
+    float mx = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     const int64_t at = row * n_slice + slice;
-    if (best == 0) {
+    if (mx == -INFINITY) {
         if (tid == 0) { out.m[at] = -INFINITY; out.s[at] = 0.0; }
         if (tid < n_beam) out.v[at * n_beam + tid] = -1;
         return;
     }
-    const float mx = sel_val((uint32_t) (best >> 32));
-    bound_of();
+    int rank = 0;
+    for (int o = 0; o < n_grp; ++o) { const float v = __shfl_sync(0xffffffffu, mine, o); rank += v > mine || (v == mine && o < lane); }
+    const unsigned who = __ballot_sync(0xffffffffu, lane < n_grp && rank == n_beam - 1);
+    const float bar = __shfl_sync(0xffffffffu, mine, __ffs(who) - 1);
     // sum of exp(x - mx): f32 within a thread, joined in f64
     float se = 0.0f;
     if (mx < INFINITY) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) se += __expf(x[j][i] - mx);
+            for (int i = 0; i < VEC; ++i) se += sel_exp2((x[j][i] - mx) * 1.44269504f);
     } else {                                     // infinite logits share the row
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -188,7 +188,6 @@ k_beam_scan(const char * logits, int64_t nb_row, int n_vocab, const float * scor
     if (lane == 0) s_s[warp] = sd;
     __syncthreads();
     auto key = [&](int j, int i) { return (unsigned long long) sel_key(x[j][i] + 0.0f) << 32 | ~(uint32_t) (first(j) + i); };      // one zero
-    const float bar = s_bound ? sel_val((uint32_t) (s_bound >> 32)) : -INFINITY;
     if (m >= bar && m > -INFINITY) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -206,20 +205,30 @@ k_beam_scan(const char * logits, int64_t nb_row, int n_vocab, const float * scor
         }
     }
     __syncthreads();
-    if (s_n > SEL_CAP) {                         // equal logits: the same once more with unique keys
-        unsigned long long mine = 0;
+    if (s_n > SEL_CAP) {                         // equal logits: once more with unique keys, over the n_beam best thread maxima of every warp
+        unsigned long long k = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) if (mine == 0 && x[j][i] == m && m > -INFINITY) mine = key(j, i);      // the lowest index: indices ascend
+            for (int i = 0; i < VEC; ++i) if (k == 0 && x[j][i] == m && m > -INFINITY) k = key(j, i);      // the lowest index: indices ascend
+        unsigned long long left = k;
+        for (int r = 0; r < n_beam; ++r) {
+            const unsigned long long top = sel_max((uint32_t) (left >> 32), (uint32_t) left);
+            if (lane == 0) s_top[warp * n_beam + r] = top;
+            if (left == top) left = 0;
+        }
         __syncthreads();
-        tops((uint32_t) (mine >> 32), (uint32_t) mine);
-        if (tid == 0) { s_n = 0; s_bound = 1; }
+        if (tid == 0) { s_n = 0; s_bound = 1; }  // fewer candidates than beams: all that there are
         __syncthreads();
-        bound_of();
+        if (tid < NW * n_beam) {
+            const unsigned long long t = s_top[tid];
+            int above = 0;
+            for (int o = 0; o < NW * n_beam; ++o) above += s_top[o] > t;
+            if (t && above == n_beam - 1) s_bound = t;
+        }
         __syncthreads();
         const unsigned long long bound = s_bound;
-        if (mine >= bound) {
+        if (k >= bound) {
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -246,9 +255,12 @@ k_beam_scan(const char * logits, int64_t nb_row, int n_vocab, const float * scor
     }
 }
 
-// One CTA per sequence.  The slices' sorted lists are the threads' (list l = beam * n_slice + slice belongs to thread l mod
-// blockDim): n_beam rounds of an arg-max over the lists' heads, each round one barrier.  Keys are (score as ordered 64-bit
-// integer, lowest beam * n_vocab + token).  Bound by latency; a warp per beam forms the logarithm of its sum.
+// One CTA per sequence: a warp per beam forms the logarithm of its sum, then n_beam rounds of an arg-max pick the best candidates.  Keys are
+// (score as ordered 64-bit integer, lowest beam * n_vocab + token).  Bound by latency: all candidates are loaded at once, before the sums are
+// known, and stay in registers (FLAT, up to SEL_HELD per thread); only where they are more, a thread holds the heads of its slices' sorted
+// lists (list l = beam * n_slice + slice belongs to thread l mod blockDim) and loads the next ones as they are taken.
+#define SEL_HELD 4
+template <bool FLAT>
 __global__ void __launch_bounds__(1024)
 k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam, int n_slice, int n_vocab, int eos,
             float * score_out, int32_t * token_out, int32_t * parent_out, uint8_t * done_out) {
@@ -259,11 +271,17 @@ k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam,
     __shared__ uint8_t s_done[B200_BEAM_MAX], s_live[B200_BEAM_MAX];
     __shared__ uint32_t s_hi[2][32], s_lo[2][32], s_ix[2][32];
     const int64_t row0 = (int64_t) blockIdx.x * n_beam;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warp = blockDim.x >> 5, n_list = n_beam * n_slice;
-    // heads of this thread's first list, under way while the sums are formed
-    float head_x = 0.0f;
-    int   head_v = -1;
-    if (tid < n_list) { const int64_t at = (row0 * n_slice + tid) * n_beam; head_x = in.x[at]; head_v = in.v[at]; }
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warp = blockDim.x >> 5, n_list = n_beam * n_slice, per_beam = n_slice * n_beam;
+    float held_x[SEL_HELD];
+    int   held_v[SEL_HELD];
+    if (FLAT) {
+#pragma unroll
+        for (int i = 0; i < SEL_HELD; ++i) {
+            const int c = i * blockDim.x + tid;
+            held_x[i] = 0.0f; held_v[i] = -1;
+            if (c < n_list * n_beam) { held_x[i] = in.x[row0 * per_beam + c]; held_v[i] = in.v[row0 * per_beam + c]; }
+        }
+    }
     for (int b = warp; b < n_beam; b += n_warp) {
         const float sc = score[row0 + b];
         const bool d = done && done[row0 + b], ok = sc > -INFINITY, live = ok && !d;
@@ -287,35 +305,51 @@ k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam,
             s_done[b] = d; s_live[b] = live && m > -INFINITY ? 1 : ok && d ? 2 : 0;
         }
     }
-    for (int l = tid; l < n_list; l += blockDim.x) s_head[l] = 0;
+    if (!FLAT) for (int l = tid; l < n_list; l += blockDim.x) s_head[l] = 0;
     __syncthreads();
 
-    unsigned long long mine = 0;
-    uint32_t mine_ix = 0;                    // ~(b * n_vocab + v) of this thread's best head, 0: none
-    int mine_l = -1;
-    auto look = [&](bool start) {            // best head among this thread's lists
-        mine = 0; mine_ix = 0; mine_l = -1;
-        for (int l = tid; l < n_list; l += blockDim.x) {
-            const int b = l / n_slice, sl = l - b * n_slice, h = s_head[l];
-            double v; int tok;
-            if (s_live[b] == 1) {
+    // key of the candidate (beam b, token, logit): 0 = none.  A done beam has one, in its first place
+    auto value = [&](int b, bool first, int tok, float x, uint32_t & ix) -> unsigned long long {
+        double v;
+        if (s_live[b] == 1) {
+            if (tok < 0) return 0;
+            v = s_score[b] + ((x == s_m[b] ? 0.0 : (double) x - s_m[b]) - s_log[b]);
+            if (!(v > -INFINITY)) return 0;
+        } else if (s_live[b] == 2 && first) {
+            tok = eos >= 0 && eos < n_vocab ? eos : 0;             // its place among equals; the token itself may be any number
+            v = s_score[b];
+        } else return 0;
+        ix = ~(uint32_t) (b * n_vocab + tok);
+        return sel_key(v + 0.0);                                   // one zero
+    };
+    unsigned long long keys[SEL_HELD] = {}, mine = 0;
+    uint32_t ixs[SEL_HELD] = {}, mine_ix = 0;                       // ~(b * n_vocab + token)
+    int mine_l = 0;
+    if (FLAT) {
+#pragma unroll
+        for (int i = 0; i < SEL_HELD; ++i) {
+            const int c = i * blockDim.x + tid;
+            if (c < n_list * n_beam) { const int b = c / per_beam; keys[i] = value(b, c == b * per_beam, held_v[i], held_x[i], ixs[i]); }
+        }
+    }
+    auto look = [&]() {                                            // best of what this thread holds
+        mine = 0; mine_ix = 0;
+        if (FLAT) {
+#pragma unroll
+            for (int i = 0; i < SEL_HELD; ++i)
+                if (keys[i] > mine || (keys[i] == mine && ixs[i] > mine_ix)) { mine = keys[i]; mine_ix = ixs[i]; mine_l = i; }
+        } else {
+            for (int l = tid; l < n_list; l += blockDim.x) {
+                const int b = l / n_slice, h = s_head[l];
                 if (h >= n_beam) continue;
-                const int64_t at = ((row0 + b) * n_slice + sl) * n_beam + h;
-                tok = start && l == tid ? head_v : in.v[at];
-                if (tok < 0) continue;
-                const double x = start && l == tid ? head_x : in.x[at];
-                v = s_score[b] + ((x == s_m[b] ? 0.0 : x - s_m[b]) - s_log[b]);
-                if (!(v > -INFINITY)) continue;
-            } else if (s_live[b] == 2 && sl == 0 && h == 0) {
-                tok = eos >= 0 && eos < n_vocab ? eos : 0;         // its place among equals; the token itself may be any number
-                v = s_score[b];
-            } else continue;
-            const unsigned long long k = sel_key(v + 0.0);         // one zero
-            const uint32_t ix = ~(uint32_t) (b * n_vocab + tok);
-            if (mine_l < 0 || k > mine || (k == mine && ix > mine_ix)) { mine = k; mine_ix = ix; mine_l = l; }
+                const int64_t at = (row0 * n_slice + l) * n_beam + h;
+                uint32_t ix = 0;
+                const unsigned long long k = value(b, l == b * n_slice && h == 0, in.v[at], in.x[at], ix);
+                if (k > mine || (k == mine && ix > mine_ix)) { mine = k; mine_ix = ix; mine_l = l; }
+            }
         }
     };
-    look(true);
+    look();
     for (int r = 0; r < n_beam; ++r) {
         const uint32_t h = (uint32_t) (mine >> 32), l = (uint32_t) mine;
         uint32_t bh = __reduce_max_sync(0xffffffffu, h);
@@ -329,19 +363,21 @@ k_beam_pick(SelSlices in, const float * score, const uint8_t * done, int n_beam,
             bl = __reduce_max_sync(0xffffffffu, wh == bh ? wl : 0u);
             bi = __reduce_max_sync(0xffffffffu, wh == bh && wl == bl ? wi : 0u);
         }
-        const bool none = bh == 0 && bl == 0;
-        if (!none && mine_l >= 0 && mine == ((unsigned long long) bh << 32 | bl) && mine_ix == bi) {
+        const unsigned long long top = (unsigned long long) bh << 32 | bl;
+        if (top != 0 && mine == top && mine_ix == bi) {
             const uint32_t flat = ~bi;
-            const int b = mine_l / n_slice;
-            const int tok = s_live[b] == 2 ? eos : (int) (flat - (uint32_t) b * (uint32_t) n_vocab);
-            score_out[row0 + r] = (float) sel_val(mine);
+            const int b = (int) (flat / (uint32_t) n_vocab), tok = s_live[b] == 2 ? eos : (int) (flat - (uint32_t) b * (uint32_t) n_vocab);
+            score_out[row0 + r] = (float) sel_val(top);
             token_out[row0 + r] = tok;
             parent_out[row0 + r] = b;
             done_out[row0 + r] = s_done[b] || tok == eos;
-            ++s_head[mine_l];
-            look(false);
+            if (FLAT) {
+#pragma unroll
+                for (int i = 0; i < SEL_HELD; ++i) if (i == mine_l) { keys[i] = 0; ixs[i] = 0; }
+            } else ++s_head[mine_l];
+            look();
         }
-        if (none && tid == 0) { score_out[row0 + r] = -INFINITY; token_out[row0 + r] = -1; parent_out[row0 + r] = -1; done_out[row0 + r] = 1; }
+        if (top == 0 && tid == 0) { score_out[row0 + r] = -INFINITY; token_out[row0 + r] = -1; parent_out[row0 + r] = -1; done_out[row0 + r] = 1; }
     }
 }
 
@@ -378,10 +414,13 @@ extern "C" int b200_beam_select(const b200_beam_select_args * a, void * stream) 
                                    a->banned, a->banned_stride, a->n_beam, ws);
     if (e != cudaSuccess) return (int) e;
     B200_LAUNCHED();
-    const int64_t n_list = n_slice * a->n_beam, lanes = n_list > 32 * a->n_beam ? n_list : 32 * a->n_beam;
+    const int64_t n_list = n_slice * a->n_beam, held = (n_list * a->n_beam + SEL_HELD - 1) / SEL_HELD;
+    const bool flat = held <= 1024;
+    int64_t lanes = flat ? held : n_list;
+    if (lanes < 32 * a->n_beam) lanes = 32 * a->n_beam;
     const unsigned threads = (unsigned) (lanes >= 1024 ? 1024 : (lanes + 31) / 32 * 32);
-    e = launch_chained(k_beam_pick, dim3((unsigned) a->n_seq), dim3(threads), (size_t) n_list, st, ws, a->score, a->done, a->n_beam, (int) n_slice,
-                       (int) a->n_vocab, (int) a->eos, a->score_out, a->token_out, a->parent_out, a->done_out);
+    e = launch_chained(flat ? k_beam_pick<true> : k_beam_pick<false>, dim3((unsigned) a->n_seq), dim3(threads), flat ? 0 : (size_t) n_list, st, ws, a->score, a->done,
+                       a->n_beam, (int) n_slice, (int) a->n_vocab, (int) a->eos, a->score_out, a->token_out, a->parent_out, a->done_out);
     if (e != cudaSuccess) return (int) e;
     B200_RETURN_LAST();
 }

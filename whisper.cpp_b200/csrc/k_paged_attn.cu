@@ -364,7 +364,7 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
         for (int of = 1; of < 4; of <<= 1) { xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, of)); xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, of)); }
         xa = fmaxf(xa, ma); xb = fmaxf(xb, mb);
         const float ba = xa == -INFINITY ? 0.0f : xa, bb = xb == -INFINITY ? 0.0f : xb;
-        const float ca = exp2f(ma - ba), cb = exp2f(mb - bb);
+        const float ca = pa_exp2(ma - ba), cb = pa_exp2(mb - bb);
         ma = xa; mb = xb;
         la *= ca; lb *= cb;
         uint32_t pf[NP][NK / 2][4];
@@ -372,7 +372,7 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
         for (int j = 0; j < NK; ++j) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                sc[j][e] = exp2f(sc[j][e] - ba); sc[j][e + 2] = exp2f(sc[j][e + 2] - bb);
+                sc[j][e] = pa_exp2(sc[j][e] - ba); sc[j][e + 2] = pa_exp2(sc[j][e + 2] - bb);
                 la += sc[j][e]; lb += sc[j][e + 2];
             }
             uint32_t w[NP];
@@ -462,7 +462,7 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
         float sum = 0.0f, x[4] = {};
 #pragma unroll
         for (int w = 0; w < PA_WARPS; ++w) {
-            const float f = exp2f(sm[w * PA_ROWS + r] - base);
+            const float f = pa_exp2(sm[w * PA_ROWS + r] - base);
             sum += f * sl[w * PA_ROWS + r];              // NaN of a warp without a finite maximum stays NaN
             if (f != 0.0f) {
                 const float4 v = *(const float4 *) (so + (w * PA_ROWS + r) * LD + d);
@@ -530,7 +530,7 @@ k_paged_join(const __grid_constant__ PaArgs a) {
         for (int i = 0; i < n; ++i) {
             if (l.total < a.stream && !some(i)) continue;
             const float * p = part(i);
-            const float f = exp2f(p[D] - base);
+            const float f = pa_exp2(p[D] - base);
             sum += f * p[D + 1];                          // NaN of a part without a finite maximum stays NaN
 #pragma unroll
             for (int j = 0; j < DL; ++j) { const float v = p[lane * DL + j]; if (f != 0.0f) acc[j] += f * v; }
@@ -567,7 +567,7 @@ k_paged_join_tc(PaArgs a) {
         const float base = mx == -INFINITY ? 0.0f : mx;
         float sum = 0.0f, acc[DL] = {};
         for (int i = 0; i < n; ++i) {
-            const float f = exp2f(p[i * step + D] - base);
+            const float f = pa_exp2(p[i * step + D] - base);
             sum += f * p[i * step + D + 1];                 // NaN of a split without a finite maximum stays NaN
             if (f == 0.0f) continue;
 #pragma unroll

@@ -128,7 +128,6 @@ __device__ __forceinline__ void pt_st16(uint32_t a, const uint32_t * v) {
 }
 __device__ __forceinline__ void pt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ float pt_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 template <typename T> __device__ __forceinline__ uint32_t pt_two(float a, float b);
 template <> __device__ __forceinline__ uint32_t pt_two<__half>(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *(const uint32_t *) &h; }
 template <> __device__ __forceinline__ uint32_t pt_two<__nv_bfloat16>(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *(const uint32_t *) &h; }
@@ -265,7 +264,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             mx = mx == -INFINITY ? mx : mx * scale;
             const bool grow = mx > m + 8.0f;                              // also when there was no key so far
             if (__any_sync(0xffffffffu, grow)) {
-                const float m1 = fmaxf(m, mx), f = m1 == -INFINITY ? 1.0f : pt_exp2(m - m1);
+                const float m1 = fmaxf(m, mx), f = m1 == -INFINITY ? 1.0f : pa_exp2(m - m1);
                 m = m1;
                 l *= f;
                 if (j > 0) {
@@ -291,7 +290,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                     float y0, y1;
                     pt_split(pt_fma2(pt_pair(__uint_as_float(x[c + 2 * i]), __uint_as_float(x[c + 2 * i + 1])), scale2, base2), y0, y1);
                     if (edge) { if (c + 2 * i >= seen) y0 = -INFINITY; if (c + 2 * i + 1 >= seen) y1 = -INFINITY; }       // -inf * 0 is not -inf
-                    y0 = pt_exp2(y0); y1 = pt_exp2(y1);
+                    y0 = pa_exp2(y0); y1 = pa_exp2(y1);
                     l2[i & 1] = pt_add2(l2[i & 1], pt_pair(y0, y1));
                     w[i] = pt_two<T>(y0, y1);
                 }

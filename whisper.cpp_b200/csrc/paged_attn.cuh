@@ -15,6 +15,9 @@ struct PaArgs {
     float scale_log2;               // scale * log2(e): weights are powers of two
 };
 
+// 2^x; below 2^-126 it is 0
+__device__ __forceinline__ float pa_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
 // the sequence's tokens: first query token, number of queries, keys in the pages (all cut to what the host was told)
 struct PaSeq { int64_t tok0; int n_new, len; };
 __device__ __forceinline__ PaSeq pa_seq(const PaArgs & a, int s) {

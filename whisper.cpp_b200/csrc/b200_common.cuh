@@ -34,6 +34,21 @@ static inline cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, di
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Dynamic shared memory above 48 KB (and clusters above 8 CTAs) have to be allowed once per kernel and device; asking every time costs
+// the host about a microsecond a call.
+template <auto KERNEL>
+static inline cudaError_t allow_once(int smem, bool big_cluster = false) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && big_cluster) e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return e;
+}
+
 // f32 -> f16 round-to-nearest-even -> f32, the F16C round trip of GGML_FP32_TO_FP16 / GGML_FP16_TO_FP32.
 // The packed conversion (cvt.rn.f16x2.f32) is used on purpose: the scalar f32->f16 conversion issues to the
 // quarter-rate conversion unit, which throttles the sequential F16 accumulation of the attention kernels.

@@ -687,7 +687,7 @@ static cudaError_t pa_launch(PaArgs & k, const PaNew & x, int n_seq, cudaStream_
         e = launch_chained(k_paged_join_tc<Q, D>, join, dim3(128), 0, st, k);
     } else {
         constexpr int smem = 4 * PA_WARPS * PA_BLOCK;
-        e = cudaFuncSetAttribute(k_paged_attn<Q, KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        e = allow_once<k_paged_attn<Q, KV, D>>(smem);
         if (e != cudaSuccess) return e;
         const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
         const dim3 grid = k.stream ? dim3((unsigned) k.stream) : dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) n_seq);

@@ -537,8 +537,8 @@ template <typename T, int D, int BN, int NS, int MIN_CTAS>
 static cudaError_t pt_go(const PaArgs & a, int n_seq, cudaStream_t st) {
     const int smem = PtSmem<D, BN, NS>::BYTES;
     const int64_t tiles = ((int64_t) a.max_new * a.group + PA_TC_ROWS - 1) / PA_TC_ROWS;
-    auto k = k_paged_attn_tc<T, D, BN, NS, MIN_CTAS>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    constexpr auto k = k_paged_attn_tc<T, D, BN, NS, MIN_CTAS>;
+    cudaError_t e = allow_once<k>(smem);
     if (e != cudaSuccess) return e;
     PtMaps maps;
     pt_make_maps(maps, a, D, BN, std::is_same<T, __half>::value);

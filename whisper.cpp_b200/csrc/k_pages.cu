@@ -5,15 +5,66 @@
 #include <cooperative_groups.h>
 namespace cg = cooperative_groups;
 
+// ---- copies --------------------------------------------------------------------------------------
+// CTA `me` of `ctas` takes its share of (copy, layer, K or V, tile of 16-byte vectors).  Bound by memory for long lists: the bytes are read
+// once and written once.
+#define PG_COPY_THREADS 256
+#define PG_COPY_UNROLL  4
+template <typename LIST>
+__device__ __forceinline__ void pg_copy(const b200_page_pool & pool, int n, int64_t me, int64_t ctas, LIST list) {
+    const unsigned vec_head = pool.head_dim / 8, vec_tok = vec_head * pool.n_head_kv, vec_page = vec_tok * pool.page_size;
+    const unsigned tiles = (vec_page + PG_COPY_THREADS * PG_COPY_UNROLL - 1) / (PG_COPY_THREADS * PG_COPY_UNROLL);
+    const int64_t items = (int64_t) n * pool.n_layer * 2 * tiles;
+    const int64_t row = pool.head_dim * 2;
+    const bool toks = (pool.n_head_kv == 1 || pool.nb_head == row) && (pool.page_size == 1 || pool.nb_tok == row * pool.n_head_kv);
+    const bool heads = (pool.page_size == 1 || pool.nb_tok == row) && (pool.n_head_kv == 1 || pool.nb_head == row * pool.page_size);
+    for (int64_t it = me; it < items; it += ctas) {
+        int64_t r = it;
+        const unsigned tile = (unsigned) (r % tiles); r /= tiles;
+        const int kv = (int) (r & 1); r >>= 1;
+        const int layer = (int) (r % pool.n_layer);
+        int src, dst, tokens;
+        list(r / pool.n_layer, src, dst, tokens);
+        const unsigned used = tokens * vec_tok;
+        if (src < 0 || dst < 0 || src >= pool.n_pages || dst >= pool.n_pages || used > vec_page) continue;
+        char * base = (char *) (kv ? pool.v : pool.k) + layer * pool.nb_layer;
+        const bool flat = toks || (heads && used == vec_page);      // what is copied is one piece of memory
+        uint4 v[PG_COPY_UNROLL];
+        int64_t off[PG_COPY_UNROLL];
+#pragma unroll
+        for (int u = 0; u < PG_COPY_UNROLL; ++u) {
+            const unsigned x = (tile * PG_COPY_UNROLL + u) * PG_COPY_THREADS + threadIdx.x;
+            off[u] = -1;
+            if (x < used && flat) {
+                off[u] = x * 16ll;
+                v[u] = *(const uint4 *) (base + src * pool.nb_page + off[u]);
+            } else if (x < used) {
+                // token-major pages: consecutive vectors walk the heads of a token; head-major: the tokens of a head come first
+                // in memory, so they are walked first
+                unsigned tok, h, i;
+                if (pool.nb_tok >= pool.nb_head) { tok = x / vec_tok; const unsigned y = x - tok * vec_tok; h = y / vec_head; i = y - h * vec_head; }
+                else { const unsigned per = tokens * vec_head; h = x / per; const unsigned y = x - h * per; tok = y / vec_head; i = y - tok * vec_head; }
+                off[u] = tok * pool.nb_tok + h * pool.nb_head + i * 16;
+                v[u] = *(const uint4 *) (base + src * pool.nb_page + off[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < PG_COPY_UNROLL; ++u) if (off[u] >= 0) *(uint4 *) (base + dst * pool.nb_page + off[u]) = v[u];
+    }
+}
+
 // ---- tables and reference counts -----------------------------------------------------------------
 // The steps depend on one another (counts -> who must copy -> which pages are taken), so all of them run in one launch.  A state that
-// fits shared memory (SMALL) is loaded once and worked on there by one CTA; what bounds it is the latency of that load.  A larger one
-// is the work of one cluster of CTAs on global memory: the hardware barrier of a cluster between the steps costs a fraction of a
+// fits shared memory (SMALL) is loaded once and worked on there; what bounds it is the latency of that load.  Up to PG_FUSED words of
+// state, every CTA of the launch does that for itself - the result is the same everywhere, CTA 0 writes it down - and then makes its share of
+// the page copies: one launch and no wait for a list.  A larger small state is the work of one CTA, and the copies are a launch of their
+// own.  A state that does not fit is the work of one cluster of CTAs on global memory: the hardware barrier of a cluster between the steps costs a fraction of a
 // launch.  All results are integers and independent of the order of the atomics; ranks come from prefix sums.
 #define PG_THREADS 1024
 #define PG_CLUSTER 16
 #define PG_MAX_ROWS 8192
 #define PG_SMALL   (160 * 1024)   // bytes of shared memory that a small state may take
+#define PG_FUSED   4096           // words of tables and counts up to which every CTA works them out for itself
 #define PG_HEADER  8              // workspace words before the lists: [0] copies, [1] tokens per whole page, [2] see k_pages_compact
 
 struct PgWork { int32_t * head; int32_t * copies; int32_t * a; int32_t * b; };    // copies: (src, dst, tokens) each
@@ -30,31 +81,28 @@ static inline int64_t pg_layout(PgWork * w, void * base, int64_t n_rows, int64_t
 
 struct PgState { int32_t * tables; int32_t * lens; int32_t * refs; };
 
-// exclusive prefix sum over the block (values and total in 32 bits); s_warp: 33 words
-__device__ __forceinline__ int pg_scan(int v, int * s_warp, int * total) {
+// exclusive prefix sum over the block; s_warp: 32 words
+template <typename V>
+__device__ __forceinline__ V pg_scan(V v, V * s_warp, V * total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int inc = v;
+    V inc = v;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += u; }
+    for (int o = 1; o < 32; o <<= 1) { const V u = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += u; }
     __syncthreads();                                   // s_warp may still be read from the scan before
     if (lane == 31) s_warp[warp] = inc;
     __syncthreads();
-    if (warp == 0) {
-        const int x = s_warp[lane];
-        int y = x;
+    // every warp adds up the warps before it
+    V y = lane < (int) (blockDim.x >> 5) ? s_warp[lane] : 0;
+    const V mine = y;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, y, o); if (lane >= o) y += u; }
-        s_warp[lane] = y - x;
-        if (lane == 31) s_warp[32] = y;
-    }
-    __syncthreads();
-    *total = s_warp[32];
-    return s_warp[warp] + inc - v;
+    for (int o = 1; o < 32; o <<= 1) { const V u = __shfl_up_sync(0xffffffffu, y, o); if (lane >= o) y += u; }
+    *total = __shfl_sync(0xffffffffu, y, 31);
+    return __shfl_sync(0xffffffffu, y - mine, warp) + inc - v;
 }
 
 __device__ __forceinline__ int pg_ceil(int n, int ps) { return n / ps + (n % ps != 0); }
 
-struct PgShared { int warp[33]; int n; int err; int pad; };
+struct PgShared { long long warp2[32]; int warp[32]; int n; int err; };
 
 // barrier over all threads of the launch
 template <bool SMALL> __device__ __forceinline__ void pg_sync(cg::cluster_group & cl) { if (SMALL) __syncthreads(); else cl.sync(); }
@@ -67,15 +115,13 @@ __device__ __forceinline__ void pg_across(cg::cluster_group & cl, PgShared & s, 
     pg_sync<SMALL>(cl);
     int b = 0, t = 0, e = 0;
     if (SMALL) { t = s.n; e = s.err; }
-    else {
-        const unsigned n = cl.num_blocks(), me = cl.block_rank();
-        for (unsigned r = 0; r < n; ++r) {
-            const PgShared * o = cl.map_shared_rank(&s, r);
-            const int v = o->n;
-            e |= o->err;
-            if (r < me) b += v;
-            t += v;
-        }
+    else {                                              // lane r asks CTA r (at most 16 of them)
+        const unsigned lane = threadIdx.x & 31, me = cl.block_rank();
+        int v = 0;
+        if (lane < cl.num_blocks()) { const PgShared * o = cl.map_shared_rank(&s, lane); v = o->n; e = o->err; }
+        e = __any_sync(0xffffffffu, e);
+        t = __reduce_add_sync(0xffffffffu, v);
+        b = __reduce_add_sync(0xffffffffu, lane < me ? v : 0);
     }
     *before = b; *all = t; *err = e;
 }
@@ -84,51 +130,52 @@ __device__ __forceinline__ void pg_across(cg::cluster_group & cl, PgShared & s, 
 // what they load as far as the compiler knows, and one value at a time costs a latency each (64 x 5 rows of 259 pages: 23 us).
 #define PG_BATCH 4
 
-// words of shared memory that a small state takes: tables, counts (as they are, and worked on), two lists of pages, columns of rows
+// words of shared memory that a small state takes: tables, counts (as they are, and worked on), two lists of pages, columns of rows, copies
 #define PG_COLUMNS 7
-static inline int64_t pg_small_words(int64_t n_rows, int64_t width, int64_t n_pages) { return n_rows * width + 4 * n_pages + PG_COLUMNS * n_rows; }
+static inline int64_t pg_small_words(int64_t n_rows, int64_t width, int64_t n_pages) { return n_rows * width + 4 * n_pages + (PG_COLUMNS + 3) * n_rows; }
 
 template <bool SMALL>
 __global__ void __launch_bounds__(PG_THREADS)
 k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int ps,
-               const int32_t * parent, const int32_t * keep, const int32_t * n_new, int32_t * status, PgWork w) {
+               const int32_t * parent, const int32_t * keep, const int32_t * n_new, int32_t * status, PgWork w, const __grid_constant__ b200_page_pool pool, bool fused) {
     cg::cluster_group cl = cg::this_cluster();
     __shared__ PgShared sh;
     extern __shared__ int32_t s_dyn[];
-    // per row, in every CTA: its parent; pages it had, keeps, will have; its length; tokens in its last kept page if that will be written, else 0;
-    // pages wanted by the rows before it (top bit: its last kept page is copied)
+    // per row, in every CTA: its parent; pages it had, keeps, will have; its length; tokens in its last kept page if that
+    // will be written, else 0; pages wanted by the rows before it (top bit: its last kept page is copied)
     int32_t * s_par = s_dyn, * s_old = s_par + n_rows, * s_kept = s_old + n_rows, * s_tot = s_kept + n_rows, * s_len = s_tot + n_rows, * s_mod = s_len + n_rows,
-            * s_off = s_mod + n_rows;
+            * s_off = s_mod + n_rows, * s_raw = s_off;      // the length as it was is needed only before the offsets
     chain_release();
     chain_wait();
-    const int tid = threadIdx.x, me = SMALL ? 0 : cl.block_rank(), n_cta = SMALL ? 1 : cl.num_blocks();
-    const int gtid = me * PG_THREADS + tid, all = n_cta * PG_THREADS, cells = n_rows * width;
+    const int tid = threadIdx.x, T = blockDim.x, me = SMALL ? 0 : cl.block_rank(), n_cta = SMALL ? 1 : cl.num_blocks();
+    const int gtid = me * T + tid, all = n_cta * T, cells = n_rows * width;
     const int32_t * tables = from.tables, * refs = from.refs;
     int32_t * held = to.refs;
+    const bool out = !SMALL || blockIdx.x == 0;        // whether this CTA writes the result down
+    int32_t * s_list = nullptr;                        // SMALL: the copies (src, dst, tokens), for this CTA's share of them
     if (tid == 0) sh.err = 0;
+    for (int i = tid; i < n_rows; i += T) { s_raw[i] = from.lens[i]; s_par[i] = parent ? parent[i] : i; s_kept[i] = keep[i]; s_tot[i] = n_new[i]; }
     if (SMALL) {                                       // everything comes in at once
         int32_t * t = s_off + n_rows, * r = t + cells;
-        held = r + n_pages; w.a = held + n_pages; w.b = w.a + n_pages;
+        held = r + n_pages; w.a = held + n_pages; w.b = w.a + n_pages; s_list = w.b + n_pages;
 #pragma unroll 4
-        for (int i = tid; i < cells; i += PG_THREADS) t[i] = tables[i];
+        for (int i = tid; i < cells; i += T) t[i] = tables[i];
 #pragma unroll 4
-        for (int i = tid; i < n_pages; i += PG_THREADS) r[i] = refs[i];
+        for (int i = tid; i < n_pages; i += T) r[i] = refs[i];
         tables = t; refs = r;
     }
-    __syncthreads();                                   // sh.err
-    for (int i = tid; i < n_rows; i += PG_THREADS) {
-        const int p = parent ? parent[i] : i, k = keep[i], n = n_new[i], len = from.lens[i];
-        const bool in = p >= 0 && p < n_rows;
-        const int have = in ? from.lens[p] : 0;
-        const bool ok = in && k >= 0 && n >= 0 && len >= 0 && (int64_t) k + n <= (int64_t) width * ps && len <= (int64_t) width * ps && k <= have;
+    __syncthreads();
+    // 1. requests checked, columns filled in; counts as they are, free pages by rank; pages that will be written announced
+    for (int i = tid; i < n_rows; i += T) {
+        const int p = s_par[i], k = s_kept[i], n = s_tot[i], len = s_raw[i];
+        const bool ok = p >= 0 && p < n_rows && k >= 0 && n >= 0 && len >= 0 && (int64_t) k + n <= (int64_t) width * ps && len <= (int64_t) width * ps && k <= s_raw[p];
         if (!ok) sh.err = 1;
-        s_par[i] = ok ? p : i; s_old[i] = ok ? pg_ceil(len, ps) : 0; s_kept[i] = ok ? pg_ceil(k, ps) : 0; s_tot[i] = ok ? pg_ceil(k + n, ps) : 0;
-        s_len[i] = ok ? k + n : 0; s_mod[i] = ok && n > 0 ? k % ps : 0;
+        const int full = k / ps, mod = k - full * ps;
+        s_par[i] = ok ? p : i; s_old[i] = ok ? pg_ceil(len, ps) : 0; s_kept[i] = ok ? full + (mod != 0) : 0; s_tot[i] = ok ? pg_ceil(k + n, ps) : 0;
+        s_len[i] = ok ? k + n : 0; s_mod[i] = ok && n > 0 ? mod : 0;
     }
-    // 1. counts as they are, free pages by rank; pages that will be written announced; every entry that is read below has to be a page
     const int per = (n_pages + all - 1) / all, p0 = min(n_pages, gtid * per), p1 = min(n_pages, p0 + per);
     int my_free = 0;
-    if (SMALL) __syncthreads();
     for (int p = p0; p < p1; p += PG_BATCH) {
         int r[PG_BATCH];
 #pragma unroll
@@ -144,47 +191,36 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
         const int s = page_written(i);
         if (s >= 0 && s < n_pages) { w.a[s] = 0x7fffffff; w.b[s] = 0; }
     }
+    pg_sync<SMALL>(cl);
+    // 2. old holders out, new ones in (what both have in the same column cancels); first writer and number of writers of a page.  Every entry
+    // that is used has to be a page; where one is not, `to` is made a copy of `from` in the end
     for (int c0 = gtid; c0 < cells; c0 += PG_BATCH * all) {
-        int t[PG_BATCH];
-#pragma unroll
-        for (int x = 0; x < PG_BATCH; ++x) t[x] = c0 + x * all < cells ? tables[c0 + x * all] : 0;
+        int o[PG_BATCH], n[PG_BATCH];
 #pragma unroll
         for (int x = 0; x < PG_BATCH; ++x) {
-            const int c = c0 + x * all, i = (unsigned) c / (unsigned) width;
-            if ((t[x] < 0 || t[x] >= n_pages) && c - i * width < s_old[i]) sh.err = 1;
+            const int c = c0 + x * all, i = (unsigned) c / (unsigned) width, j = c - i * width;
+            const bool in = c < cells;
+            o[x] = in && j < s_old[i] ? tables[c] : -1;
+            n[x] = in && j < s_kept[i] ? tables[s_par[i] * width + j] : -1;
+            if (in && j < s_old[i] && (o[x] < 0 || o[x] >= n_pages)) { sh.err = 1; o[x] = -1; }
         }
+#pragma unroll
+        for (int x = 0; x < PG_BATCH; ++x) if (o[x] != n[x]) {
+            if (o[x] >= 0) atomicSub(&held[o[x]], 1);
+            if (n[x] >= 0 && n[x] < n_pages) atomicAdd(&held[n[x]], 1);
+        }
+    }
+    for (int i = gtid; i < n_rows; i += all) {
+        const int s = page_written(i);
+        if (s >= 0 && s < n_pages) { atomicMin(&w.a[s], i); atomicAdd(&w.b[s], 1); }
     }
     int n_free, err;
     pg_across<SMALL>(cl, sh, &my_free, &n_free, &err);
     free_before += my_free;
-
-    if (!err) {
-        // 2. old holders out, new ones in (what both have in the same column cancels); first writer and number of writers of a page
-        for (int c0 = gtid; c0 < cells; c0 += PG_BATCH * all) {
-            int o[PG_BATCH], n[PG_BATCH];
-#pragma unroll
-            for (int x = 0; x < PG_BATCH; ++x) {
-                const int c = c0 + x * all, i = (unsigned) c / (unsigned) width, j = c - i * width;
-                const bool in = c < cells;
-                o[x] = in && j < s_old[i] ? tables[c] : -1;
-                n[x] = in && j < s_kept[i] ? tables[s_par[i] * width + j] : -1;
-            }
-#pragma unroll
-            for (int x = 0; x < PG_BATCH; ++x) if (o[x] != n[x]) {
-                if (o[x] >= 0) atomicSub(&held[o[x]], 1);
-                if (n[x] >= 0) atomicAdd(&held[n[x]], 1);
-            }
-        }
-        for (int i = gtid; i < n_rows; i += all) {
-            const int s = page_written(i);
-            if (s >= 0) { atomicMin(&w.a[s], i); atomicAdd(&w.b[s], 1); }
-        }
-    }
-    pg_sync<SMALL>(cl);
     // 3. who copies, what is wanted (every CTA for itself)
     int wanted = 0, n_copy = 0;
     if (!err) {
-        for (int i0 = 0; i0 < n_rows; i0 += PG_THREADS) {
+        for (int i0 = 0; i0 < n_rows; i0 += T) {
             const int i = i0 + tid;
             int want = 0, copy = 0, s = -1;
             if (i < n_rows) {
@@ -192,24 +228,22 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
                 copy = s >= 0 && (pg_get<SMALL>(&w.a[s]) != i || pg_get<SMALL>(&held[s]) > pg_get<SMALL>(&w.b[s]));
                 want = s_tot[i] - s_kept[i] + copy;
             }
-            int sum;
-            const int before = pg_scan(want, sh.warp, &sum);
-            if (i < n_rows) s_off[i] = (wanted + before) | copy << 31;
-            wanted += sum;                              // at most n_rows * (width + 1): checked to be below 2^31 by the host
-            if (me == 0) {
-                int copies;
-                const int c_before = pg_scan(copy, sh.warp, &copies);
-                if (copy) {                             // destination: filled in below, when the free pages are known
-                    const int c = n_copy + c_before;
-                    w.copies[3 * c] = s; w.copies[3 * c + 1] = wanted - sum + before; w.copies[3 * c + 2] = s_mod[i];
-                }
-                n_copy += copies;
+            long long sum;                              // pages wanted (at most n_rows * (width + 1): below 2^31 by the host's check), copies from bit 40 on
+            const long long at = pg_scan((long long) want | (long long) copy << 40, sh.warp2, &sum);
+            const int before = wanted + (int) (at & 0x7fffffff);
+            if (i < n_rows) s_off[i] = before | copy << 31;
+            if (me == 0 && copy) {                      // destination: filled in below, when the free pages are known
+                int32_t * l = (SMALL ? s_list : w.copies) + 3 * (n_copy + (int) (at >> 40));
+                l[0] = s; l[1] = before; l[2] = s_mod[i];
             }
+            wanted += (int) (sum & 0x7fffffff);
+            n_copy += (int) (sum >> 40);
         }
     }
     const int missing = err ? -1 : max(wanted - n_free, 0);
     pg_sync<SMALL>(cl);                                 // all have read the counts and the writers: w.a becomes the list of free pages
     if (missing != 0) {
+        if (!out) return;
         for (int p = gtid; p < n_pages; p += all) to.refs[p] = refs[p];
         for (int i = gtid; i < n_rows; i += all) to.lens[i] = from.lens[i];
         for (int c = gtid; c < cells; c += all) to.tables[c] = tables[c];
@@ -224,12 +258,12 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
         for (int x = 0; x < PG_BATCH; ++x) if (r[x] == 0 && f < wanted) { w.a[f++] = p + x; held[p + x] = 1; }
     }
     for (int i = gtid; i < n_rows; i += all) {
-        to.lens[i] = s_len[i];
+        if (out) to.lens[i] = s_len[i];
         if ((unsigned) s_off[i] >> 31) atomicSub(&held[page_written(i)], 1);
     }
     pg_sync<SMALL>(cl);
     // 4. the new tables
-    for (int c0 = gtid; c0 < cells; c0 += PG_BATCH * all) {
+    for (int c0 = gtid; out && c0 < cells; c0 += PG_BATCH * all) {
         int t[PG_BATCH];
 #pragma unroll
         for (int x = 0; x < PG_BATCH; ++x) {
@@ -243,36 +277,46 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
 #pragma unroll
         for (int x = 0; x < PG_BATCH; ++x) if (c0 + x * all < cells) to.tables[c0 + x * all] = t[x];
     }
-    if (SMALL) for (int p = tid; p < n_pages; p += PG_THREADS) to.refs[p] = held[p];
+    if (SMALL && out) for (int p = tid; p < n_pages; p += T) to.refs[p] = held[p];
     if (me == 0) {
-        for (int c = tid; c < n_copy; c += PG_THREADS) w.copies[3 * c + 1] = pg_get<SMALL>(&w.a[w.copies[3 * c + 1]]);
-        if (tid == 0) { status[0] = 0; status[1] = n_copy; w.head[0] = n_copy; w.head[1] = ps; }
+        for (int c = tid; c < n_copy; c += T) {
+            int32_t * l = (SMALL ? s_list : w.copies) + 3 * c;
+            l[1] = pg_get<SMALL>(&w.a[l[1]]);
+            if (SMALL && out) { w.copies[3 * c] = l[0]; w.copies[3 * c + 1] = l[1]; w.copies[3 * c + 2] = l[2]; }
+        }
+        if (tid == 0 && out) { status[0] = 0; status[1] = n_copy; w.head[0] = n_copy; w.head[1] = ps; }
+    }
+    if (SMALL && fused) {
+        __syncthreads();
+        pg_copy(pool, n_copy, blockIdx.x, gridDim.x, [&](int64_t c, int & src, int & dst, int & tokens) { src = s_list[3 * c]; dst = s_list[3 * c + 1]; tokens = s_list[3 * c + 2]; });
     }
 }
 
 template <bool SMALL>
 __global__ void __launch_bounds__(PG_THREADS)
-k_pages_compact(PgState from, PgState to, int n_rows, int width, int n_pages, int ps, int32_t * remap, int32_t * status, PgWork w) {
+k_pages_compact(PgState from, PgState to, int n_rows, int width, int n_pages, int ps, int32_t * remap, int32_t * status, PgWork w,
+                const __grid_constant__ b200_page_pool pool, bool fused) {
     cg::cluster_group cl = cg::this_cluster();
     __shared__ PgShared sh;
     __shared__ int s_low;
     extern __shared__ int32_t s_dyn[];
     chain_release();
     chain_wait();
-    const int tid = threadIdx.x, me = SMALL ? 0 : cl.block_rank(), n_cta = SMALL ? 1 : cl.num_blocks();
-    const int gtid = me * PG_THREADS + tid, all = n_cta * PG_THREADS;
+    const int tid = threadIdx.x, T = blockDim.x, me = SMALL ? 0 : cl.block_rank(), n_cta = SMALL ? 1 : cl.num_blocks();
+    const int gtid = me * T + tid, all = n_cta * T;
     const int cells = n_rows * width;
     const int32_t * tables = from.tables, * lens = from.lens, * refs = from.refs;
     int32_t * map = remap, * low_at = SMALL ? &s_low : &w.head[2];
+    const bool out = !SMALL || blockIdx.x == 0;        // whether this CTA writes the result down
     if (tid == 0) sh.err = 0;
     if (SMALL) {
         int32_t * t = s_dyn, * l = t + cells, * r = l + n_rows;
         map = r + n_pages; w.a = map + n_pages; w.b = w.a + n_pages;
-        for (int i = tid; i < n_rows; i += PG_THREADS) l[i] = lens[i];
+        for (int i = tid; i < n_rows; i += T) l[i] = lens[i];
 #pragma unroll 4
-        for (int i = tid; i < n_pages; i += PG_THREADS) r[i] = refs[i];
+        for (int i = tid; i < n_pages; i += T) r[i] = refs[i];
 #pragma unroll 4
-        for (int i = tid; i < cells; i += PG_THREADS) t[i] = tables[i];
+        for (int i = tid; i < cells; i += T) t[i] = tables[i];
         tables = t; lens = l; refs = r;
     }
     __syncthreads();
@@ -316,16 +360,16 @@ k_pages_compact(PgState from, PgState to, int n_rows, int width, int n_pages, in
             if (p >= n_live)   held = 0;
             else if (n == 0)   held = refs[pg_get<SMALL>(&w.a[low + p - r])];
         }
-        to.refs[p] = held;
+        if (out) to.refs[p] = held;
         map[p] = to_p;
-        if (SMALL) remap[p] = to_p;
+        if (SMALL && out) remap[p] = to_p;
         r += n != 0;
     }
-    for (int c = gtid; c < moves; c += all) { w.copies[3 * c] = pg_get<SMALL>(&w.a[low + c]); w.copies[3 * c + 1] = pg_get<SMALL>(&w.b[c]); w.copies[3 * c + 2] = ps; }
-    if (gtid == 0) { status[0] = err ? -1 : 0; status[1] = moves; w.head[0] = moves; w.head[1] = ps; }
+    for (int c = gtid; out && c < moves; c += all) { w.copies[3 * c] = pg_get<SMALL>(&w.a[low + c]); w.copies[3 * c + 1] = pg_get<SMALL>(&w.b[c]); w.copies[3 * c + 2] = ps; }
+    if (gtid == 0 && out) { status[0] = err ? -1 : 0; status[1] = moves; w.head[0] = moves; w.head[1] = ps; }
     pg_sync<SMALL>(cl);
-    for (int i = gtid; i < n_rows; i += all) to.lens[i] = lens[i];
-    for (int c0 = gtid; c0 < cells; c0 += PG_BATCH * all) {
+    for (int i = gtid; out && i < n_rows; i += all) to.lens[i] = lens[i];
+    for (int c0 = gtid; out && c0 < cells; c0 += PG_BATCH * all) {
         int t[PG_BATCH];
 #pragma unroll
         for (int x = 0; x < PG_BATCH; ++x) {
@@ -339,57 +383,16 @@ k_pages_compact(PgState from, PgState to, int n_rows, int width, int n_pages, in
 #pragma unroll
         for (int x = 0; x < PG_BATCH; ++x) if (c0 + x * all < cells) to.tables[c0 + x * all] = t[x];
     }
+    if (SMALL && fused) pg_copy(pool, moves, blockIdx.x, gridDim.x, [&](int64_t c, int & src, int & dst, int & tokens) { src = w.a[low + c]; dst = w.b[c]; tokens = ps; });
 }
 
-// ---- copies --------------------------------------------------------------------------------------
-// The list of copies is on the device, so its length is not known to the host: a fixed grid strides over
-// (copy, layer, K or V, 16-byte vector).  Bound by memory for long lists: the bytes are read once and written once.
-#define PG_COPY_THREADS 256
-#define PG_COPY_UNROLL  4
+// ---- host ----
+// The list of copies is on the device, so its length is not known to the host: a fixed grid strides over it.
 __global__ void __launch_bounds__(PG_COPY_THREADS)
 k_pages_copy(b200_page_pool pool, const int32_t * head, const int32_t * copies) {
     chain_release();
     chain_wait();
-    const int n = head[0];
-    const unsigned vec_head = pool.head_dim / 8, vec_tok = vec_head * pool.n_head_kv, vec_page = vec_tok * pool.page_size;
-    const unsigned tiles = (vec_page + PG_COPY_THREADS * PG_COPY_UNROLL - 1) / (PG_COPY_THREADS * PG_COPY_UNROLL);
-    const int64_t items = (int64_t) n * pool.n_layer * 2 * tiles;
-    const int64_t row = pool.head_dim * 2;
-    const bool toks = (pool.n_head_kv == 1 || pool.nb_head == row) && (pool.page_size == 1 || pool.nb_tok == row * pool.n_head_kv);
-    const bool heads = (pool.page_size == 1 || pool.nb_tok == row) && (pool.n_head_kv == 1 || pool.nb_head == row * pool.page_size);
-    for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-        int64_t r = it;
-        const unsigned tile = (unsigned) (r % tiles); r /= tiles;
-        const int kv = (int) (r & 1); r >>= 1;
-        const int layer = (int) (r % pool.n_layer);
-        const int64_t c = r / pool.n_layer;
-        const int32_t src = copies[3 * c], dst = copies[3 * c + 1];
-        const unsigned used = copies[3 * c + 2] * vec_tok;
-        if (src < 0 || dst < 0 || src >= pool.n_pages || dst >= pool.n_pages || used > vec_page) continue;
-        char * base = (char *) (kv ? pool.v : pool.k) + layer * pool.nb_layer;
-        const bool flat = toks || (heads && used == vec_page);      // what is copied is one piece of memory
-        uint4 v[PG_COPY_UNROLL];
-        int64_t off[PG_COPY_UNROLL];
-#pragma unroll
-        for (int u = 0; u < PG_COPY_UNROLL; ++u) {
-            const unsigned x = (tile * PG_COPY_UNROLL + u) * PG_COPY_THREADS + threadIdx.x;
-            off[u] = -1;
-            if (x < used && flat) {
-                off[u] = x * 16ll;
-                v[u] = *(const uint4 *) (base + src * pool.nb_page + off[u]);
-            } else if (x < used) {
-                // token-major pages: consecutive vectors walk the heads of a token; head-major: the tokens of a head come first
-                // in memory, so they are walked first
-                unsigned tok, h, i;
-                if (pool.nb_tok >= pool.nb_head) { tok = x / vec_tok; const unsigned y = x - tok * vec_tok; h = y / vec_head; i = y - h * vec_head; }
-                else { const unsigned per = copies[3 * c + 2] * vec_head; h = x / per; const unsigned y = x - h * per; tok = y / vec_head; i = y - tok * vec_head; }
-                off[u] = tok * pool.nb_tok + h * pool.nb_head + i * 16;
-                v[u] = *(const uint4 *) (base + src * pool.nb_page + off[u]);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < PG_COPY_UNROLL; ++u) if (off[u] >= 0) *(uint4 *) (base + dst * pool.nb_page + off[u]) = v[u];
-    }
+    pg_copy(pool, head[0], blockIdx.x, gridDim.x, [&](int64_t c, int & src, int & dst, int & tokens) { src = copies[3 * c]; dst = copies[3 * c + 1]; tokens = copies[3 * c + 2]; });
 }
 
 bool b200_pool_ok(const b200_page_pool * p, bool data) {
@@ -413,26 +416,31 @@ static int pg_launch_copy(const b200_page_pool * pool, const PgWork & w, int64_t
     return 0;
 }
 
-// SMALL or cluster form of a kernel, by the size of the state
-template <typename... KArgs, typename... Args>
-static cudaError_t pg_launch(void (*small)(KArgs...), void (*large)(KArgs...), int64_t n_rows, int64_t width, int64_t n_pages, cudaStream_t st, Args &&... args) {
+// SMALL or cluster form of a kernel, by the size of the state; *fused: it makes the copies too (max_copies at most)
+template <auto SMALL_KERNEL, auto LARGE_KERNEL, typename... Args>
+static cudaError_t pg_launch(int64_t n_rows, int64_t width, int64_t n_pages, const b200_page_pool * pool, bool data, int64_t max_copies, bool * fused, cudaStream_t st, Args &&... args) {
     const int64_t words = pg_small_words(n_rows, width, n_pages);
     const bool fits = words * 4 <= PG_SMALL;
-    auto kernel = fits ? small : large;
-    const size_t smem = fits ? words * 4 : 4 * PG_COLUMNS * (n_rows > 0 ? n_rows : 1);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fits ? PG_SMALL : 4 * PG_COLUMNS * PG_MAX_ROWS);
-    if (e == cudaSuccess && !fits) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    *fused = fits && data && n_rows * width + n_pages <= PG_FUSED && n_rows <= PG_COPY_THREADS;
+    cudaError_t e = fits ? allow_once<SMALL_KERNEL>(PG_SMALL) : allow_once<LARGE_KERNEL>(4 * PG_COLUMNS * PG_MAX_ROWS, true);
     if (e != cudaSuccess) return e;
+    int64_t ctas = 1;
+    if (*fused) {
+        ctas = max_copies * pool->n_layer * 2 * (((int64_t) pool->page_size * pool->n_head_kv * pool->head_dim / 8 + PG_COPY_THREADS * PG_COPY_UNROLL - 1) / (PG_COPY_THREADS * PG_COPY_UNROLL));
+        ctas = ctas < 1 ? 1 : ctas > 148 * 3 ? 148 * 3 : ctas;
+    }
     cudaLaunchConfig_t cfg = {};
-    const unsigned n = fits ? 1 : PG_CLUSTER;
-    cfg.gridDim = dim3(n); cfg.blockDim = dim3(PG_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.gridDim = dim3((unsigned) (fits ? ctas : PG_CLUSTER));
+    cfg.blockDim = dim3(*fused ? PG_COPY_THREADS : PG_THREADS);
+    cfg.dynamicSmemBytes = (size_t) (fits ? words * 4 : 4 * PG_COLUMNS * (n_rows > 0 ? n_rows : 1));
+    cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = n; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = fits ? 1 : PG_CLUSTER; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = b200_chained_launches() ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+    return cudaLaunchKernelEx(&cfg, fits ? SMALL_KERNEL : LARGE_KERNEL, std::forward<Args>(args)..., *pool, *fused);
 }
 
 // what update and compact ask of their states
@@ -465,10 +473,11 @@ extern "C" int b200_pages_update(const b200_page_pool * pool, const b200_page_st
     const PgState f = { from->tables, from->lens, from->refs }, t = { to->tables, to->lens, to->refs };
     const int width = from->n_rows ? (int) from->table_stride : 0;
     const cudaStream_t st = as_stream(stream);
-    cudaError_t e = pg_launch(k_pages_update<true>, k_pages_update<false>, from->n_rows, width, pool->n_pages, st, f, t, (int) from->n_rows, width, pool->n_pages, pool->page_size, parent, keep, n_new, status, w);
+    bool fused;
+    cudaError_t e = pg_launch<k_pages_update<true>, k_pages_update<false>>(from->n_rows, width, pool->n_pages, pool, data, from->n_rows, &fused, st, f, t, (int) from->n_rows, width, pool->n_pages, pool->page_size, parent, keep, n_new, status, w);
     if (e != cudaSuccess) return (int) e;
     B200_LAUNCHED();
-    if (data && from->n_rows) return pg_launch_copy(pool, w, from->n_rows, st);
+    if (data && !fused && from->n_rows) return pg_launch_copy(pool, w, from->n_rows, st);
     return (int) cudaGetLastError();
 }
 
@@ -482,10 +491,11 @@ extern "C" int b200_pages_compact(const b200_page_pool * pool, const b200_page_s
     const PgState f = { from->tables, from->lens, from->refs }, t = { to->tables, to->lens, to->refs };
     const int width = from->n_rows ? (int) from->table_stride : 0;
     const cudaStream_t st = as_stream(stream);
-    cudaError_t e = pg_launch(k_pages_compact<true>, k_pages_compact<false>, from->n_rows, width, pool->n_pages, st, f, t, (int) from->n_rows, width, pool->n_pages, pool->page_size, remap, status, w);
+    bool fused;
+    cudaError_t e = pg_launch<k_pages_compact<true>, k_pages_compact<false>>(from->n_rows, width, pool->n_pages, pool, data, pool->n_pages / 2 + 1, &fused, st, f, t, (int) from->n_rows, width, pool->n_pages, pool->page_size, remap, status, w);
     if (e != cudaSuccess) return (int) e;
     B200_LAUNCHED();
-    if (data) return pg_launch_copy(pool, w, pool->n_pages / 2 + 1, st);
+    if (data && !fused) return pg_launch_copy(pool, w, pool->n_pages / 2 + 1, st);
     return (int) cudaGetLastError();
 }
 

@@ -142,9 +142,9 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
     __shared__ PgShared sh;
     extern __shared__ int32_t s_dyn[];
     // per row, in every CTA: its parent; pages it had, keeps, will have; its length; tokens in its last kept page if that
-    // will be written, else 0; pages wanted by the rows before it (top bit: its last kept page is copied)
+    // will be written, else 0, and that page; pages wanted by the rows before it (top bit: its last kept page is copied)
     int32_t * s_par = s_dyn, * s_old = s_par + n_rows, * s_kept = s_old + n_rows, * s_tot = s_kept + n_rows, * s_len = s_tot + n_rows, * s_mod = s_len + n_rows,
-            * s_off = s_mod + n_rows, * s_raw = s_off;      // the length as it was is needed only before the offsets
+            * s_off = s_mod + n_rows, * s_raw = s_off, * s_page = s_old;     // the length as it was is needed only before the offsets
     chain_release();
     chain_wait();
     const int tid = threadIdx.x, T = blockDim.x, me = SMALL ? 0 : cl.block_rank(), n_cta = SMALL ? 1 : cl.num_blocks();
@@ -186,9 +186,8 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
     int cta_free;
     int free_before = pg_scan(my_free, sh.warp, &cta_free);            // (its barriers publish the columns)
     if (tid == 0) sh.n = cta_free;
-    auto page_written = [&](int i) { return s_mod[i] ? tables[s_par[i] * width + s_kept[i] - 1] : -1; };
     for (int i = gtid; i < n_rows; i += all) {
-        const int s = page_written(i);
+        const int s = s_mod[i] ? tables[s_par[i] * width + s_kept[i] - 1] : -1;
         if (s >= 0 && s < n_pages) { w.a[s] = 0x7fffffff; w.b[s] = 0; }
     }
     pg_sync<SMALL>(cl);
@@ -210,9 +209,11 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
             if (n[x] >= 0 && n[x] < n_pages) atomicAdd(&held[n[x]], 1);
         }
     }
-    for (int i = gtid; i < n_rows; i += all) {
-        const int s = page_written(i);
-        if (s >= 0 && s < n_pages) { atomicMin(&w.a[s], i); atomicAdd(&w.b[s], 1); }
+    __syncthreads();                                    // s_page takes the place of s_old
+    for (int i = tid; i < n_rows; i += T) {
+        const int s = s_mod[i] ? tables[s_par[i] * width + s_kept[i] - 1] : -1;
+        s_page[i] = s;
+        if (i % n_cta == me && s >= 0 && s < n_pages) { atomicMin(&w.a[s], i); atomicAdd(&w.b[s], 1); }
     }
     int n_free, err;
     pg_across<SMALL>(cl, sh, &my_free, &n_free, &err);
@@ -224,7 +225,7 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
             const int i = i0 + tid;
             int want = 0, copy = 0, s = -1;
             if (i < n_rows) {
-                s = page_written(i);
+                s = s_page[i];
                 copy = s >= 0 && (pg_get<SMALL>(&w.a[s]) != i || pg_get<SMALL>(&held[s]) > pg_get<SMALL>(&w.b[s]));
                 want = s_tot[i] - s_kept[i] + copy;
             }
@@ -259,7 +260,7 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
     }
     for (int i = gtid; i < n_rows; i += all) {
         if (out) to.lens[i] = s_len[i];
-        if ((unsigned) s_off[i] >> 31) atomicSub(&held[page_written(i)], 1);
+        if ((unsigned) s_off[i] >> 31) atomicSub(&held[s_page[i]], 1);
     }
     pg_sync<SMALL>(cl);
     // 4. the new tables

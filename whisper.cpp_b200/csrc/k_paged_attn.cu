@@ -35,30 +35,36 @@ template <> __device__ __forceinline__ void pa_unpack8<__nv_bfloat16>(uint4 q, f
 }
 
 
-// one thread per 8 values; f32 is rounded to the pool's type (to nearest even: the cache's precision), 16-bit values are copied
+// a warp per token, 16 bytes of the pool a lane; f32 is rounded to the pool's type (to nearest even: the cache's precision), 16-bit values are
+// copied.  Bound by memory: every value is read and written once
 template <typename KV, bool F32>
 __global__ void __launch_bounds__(256)
-k_paged_store(PaArgs a, PaNew x, int vec_head) {
+k_paged_store(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew x, int log_vec) {
     chain_release();
     chain_wait();
     const PaSeq s = pa_seq(a, blockIdx.y);
-    const int per_tok = 2 * a.n_head_kv * vec_head;
-    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < (int64_t) s.n_new * per_tok; i += (int64_t) gridDim.x * 256) {
-        const int t = (int) (i / per_tok), r = (int) (i - (int64_t) t * per_tok), c = r % vec_head, h = r / vec_head % a.n_head_kv;
-        const bool v = r >= per_tok / 2;
+    const int lane = threadIdx.x & 31, per_tok = 2 * a.n_head_kv << log_vec, mask = (1 << log_vec) - 1;
+    for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < s.n_new; t += gridDim.x * 8) {
         const int pos = s.len - s.n_new + t;
         if (pos < 0) continue;
         const int page = a.tables[blockIdx.y * a.table_stride + pos / a.page_size];
         if (page < 0 || page >= a.n_pages) continue;
-        const char * src = (v ? x.v : x.k) + (s.tok0 + t) * x.nb_tok + h * x.nb_head;
-        uint4 q;
-        if (F32) {
-            float f[8];
-            *(float4 *) f = ((const float4 *) src)[2 * c];
-            *(float4 *) (f + 4) = ((const float4 *) src)[2 * c + 1];
-            q = pa_pack8<KV>(f);
-        } else q = ((const uint4 *) src)[c];
-        *(uint4 *) ((char *) (v ? a.v : a.k) + page * a.nb_page + (pos % a.page_size) * a.nb_tok + h * a.nb_head + c * 16) = q;
+        const int64_t at = page * a.nb_page + (pos % a.page_size) * a.nb_tok, from = (s.tok0 + t) * x.nb_tok;
+#pragma unroll 4
+        for (int r = lane; r < per_tok; r += 32) {
+            const int c = r & mask, hv = r >> log_vec;
+            const bool v = hv >= a.n_head_kv;
+            const int h = v ? hv - a.n_head_kv : hv;
+            const char * src = (v ? x.v : x.k) + from + h * x.nb_head;
+            uint4 q;
+            if (F32) {
+                float f[8];
+                *(float4 *) f = ((const float4 *) src)[2 * c];
+                *(float4 *) (f + 4) = ((const float4 *) src)[2 * c + 1];
+                q = pa_pack8<KV>(f);
+            } else q = ((const uint4 *) src)[c];
+            *(uint4 *) ((char *) (v ? a.v : a.k) + at + h * a.nb_head + c * 16) = q;
+        }
     }
 }
 
@@ -619,8 +625,8 @@ static PaPlan pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a) 
         return r;
     }
     r.store = a->k_new != nullptr;
-    const int64_t ctas = (rows + PA_TC_ROWS - 1) / PA_TC_ROWS * p->n_head_kv * a->n_seq;
-    const int64_t resident = 148 * (p->head_dim == 64 ? 2 : 1);
+    const int64_t ctas = (rows + PA_TC_ROWS(p->head_dim) - 1) / PA_TC_ROWS(p->head_dim) * p->n_head_kv * a->n_seq;
+    const int64_t resident = 148 * (p->head_dim == 64 ? 4 : 1);
     int64_t want = (resident + ctas - 1) / ctas, most = (a->max_len + 511) / 512;
     if (ctas * 2 > resident) want = 1;
     if (want > most) want = most;
@@ -665,13 +671,12 @@ extern "C" int b200_paged_store(const b200_page_pool * pool, const b200_paged_at
     if (b.n_head < 1) b.n_head = pool->n_head_kv;
     const PaArgs k = pa_pack(pool, &b);
     const PaNew x = { (const char *) a->k_new, (const char *) a->v_new, a->nb_new_tok, a->nb_new_head };
-    const int vec_head = pool->head_dim / 8;
-    int64_t n = ((int64_t) k.max_new * 2 * pool->n_head_kv * vec_head + 255) / 256;
+    int64_t n = (k.max_new + 7) / 8;
     const int64_t most = (148 * 8 + a->n_seq - 1) / a->n_seq;
     if (n > most) n = most;
     const bool f32 = a->q_type == B200_TYPE_F32, h = pool->type == B200_TYPE_F16;
     auto f = h ? (f32 ? k_paged_store<__half, true> : k_paged_store<__half, false>) : (f32 ? k_paged_store<__nv_bfloat16, true> : k_paged_store<__nv_bfloat16, false>);
-    const cudaError_t e = launch_chained(f, dim3((unsigned) n, (unsigned) a->n_seq), dim3(256), 0, as_stream(stream), k, x, vec_head);
+    const cudaError_t e = launch_chained(f, dim3((unsigned) n, (unsigned) a->n_seq), dim3(256), 0, as_stream(stream), k, x, pool->head_dim == 64 ? 3 : 4);
     if (e != cudaSuccess) return (int) e;
     B200_RETURN_LAST();
 }
@@ -681,7 +686,7 @@ static cudaError_t pa_launch(PaArgs & k, const PaNew & x, int n_seq, cudaStream_
     cudaError_t e;
     const int64_t rows = (int64_t) k.max_new * k.n_head;
     const dim3 join((unsigned) (rows < 16384 ? (rows + 3) / 4 : 4096), (unsigned) n_seq);
-    if (k.tile_rows == PA_TC_ROWS) {
+    if (k.tile_rows != PA_ROWS) {
         e = pa_tc_launch(k, D, std::is_same<KV, __half>::value ? B200_TYPE_F16 : B200_TYPE_BF16, n_seq, st);
         if (e != cudaSuccess || k.n_split == 1) return e;
         e = launch_chained(k_paged_join_tc<Q, D>, join, dim3(128), 0, st, k);
@@ -706,7 +711,7 @@ extern "C" int b200_paged_attn(const b200_page_pool * pool, const b200_paged_att
     if (a->n_seq == 0 || a->n_tok == 0 || a->max_new == 0) return 0;
     PaArgs k = pa_pack(pool, a);
     const PaPlan r = pa_plan(pool, a);
-    k.n_split = r.n_split; k.chunk = r.chunk; k.stream = r.stream; k.tile_rows = r.tc ? PA_TC_ROWS : PA_ROWS; k.n_seq = a->n_seq;
+    k.n_split = r.n_split; k.chunk = r.chunk; k.stream = r.stream; k.tile_rows = r.tc ? PA_TC_ROWS(pool->head_dim) : PA_ROWS; k.n_seq = a->n_seq;
     const int64_t need = b200_paged_attn_workspace(pool, a);
     if (need && (!a->workspace || (uintptr_t) a->workspace % 16 || a->workspace_bytes < need)) return B200_ERR_ARG;
     if ((int64_t) a->n_seq * k.n_split > 65535) return B200_ERR_ARG;

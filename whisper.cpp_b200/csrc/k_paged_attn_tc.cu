@@ -33,11 +33,11 @@ extern "C" int b200_paged_attn_status(void) {
     return e == cudaSuccess ? v : (int) e;
 }
 
-#define PT_THREADS 352
+#define PT_THREADS(NTILE) (128 * (NTILE) + 96)
 
-template <int D, int BN, int NS> struct PtSmem {
+template <int D, int BN, int NS, int NTILE> struct PtSmem {
     static constexpr int TILE = BN * D * 2, QT = 128 * D * 2;
-    static constexpr int Q = 0, K = 2 * QT, V = K + NS * TILE, BAR = V + NS * TILE;
+    static constexpr int Q = 0, K = NTILE * QT, V = K + NS * TILE, BAR = V + NS * TILE;
     static constexpr int N_BAR = 5 * NS + 7;             // k_full, k_empty, v_full, v_empty, v_here [NS]; q_full; s_full, p_full, o_full [2]
     static constexpr int MISC = BAR + N_BAR * 8;         // tensor-memory address, abort flag, odd-value flag
     static constexpr int BYTES = MISC + 16 + 1024;       // the dynamic array starts on 16 bytes: tiles are moved to 1024
@@ -165,31 +165,31 @@ template <typename T> __device__ __forceinline__ float pt_zero_times(uint4 x, fl
     return any + __uint_as_float(pt_odd<T>(z) ? 0x7fffffffu : 0u);
 }
 
-template <typename T, int D, int BN, int NS, int MIN_CTAS>
-__global__ void __launch_bounds__(PT_THREADS, MIN_CTAS)
+template <typename T, int D, int BN, int NS, int NTILE, int MIN_CTAS>
+__global__ void __launch_bounds__(PT_THREADS(NTILE), MIN_CTAS)
 k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps maps) {
-    using L = PtSmem<D, BN, NS>;
-    constexpr int COLS = 2 * BN + 2 * D <= 256 ? 256 : 512, NC = D / 8;
+    using L = PtSmem<D, BN, NS, NTILE>;
+    constexpr int COLS = NTILE * (BN + D) <= 128 ? 128 : NTILE * (BN + D) <= 256 ? 256 : 512, NC = D / 8, ROWS = 128 * NTILE, W_MMA = 4 * NTILE;
     extern __shared__ __align__(16) char smem_raw[];
     chain_wait();                                         // no early release: this kernel wants whole SMs
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // the shuffle tells the compiler that the warp agrees
     const int seq = blockIdx.z / a.n_split, split = blockIdx.z % a.n_split, kvh = blockIdx.y;
-    const int row0 = (gridDim.x - 1 - blockIdx.x) * PA_TC_ROWS;         // the longest tiles first
+    const int row0 = (gridDim.x - 1 - blockIdx.x) * ROWS;         // the longest tiles first
     const PaSeq s = pa_seq(a, seq);
     const int n_rows = s.n_new * a.group;
     if (row0 >= n_rows) return;
     const int k0 = split * a.chunk, k1 = min(pa_reach(a, s, row0), k0 + a.chunk);
     if (k0 >= k1 && split != 0) return;                  // an empty split: the join does not read it
     // blocks of each tile; a tile without rows has none
-    int n_blk[2], sure[2];                               // sure: keys below are seen by every row of the tile
+    int n_blk[NTILE], sure[NTILE];                               // sure: keys below are seen by every row of the tile
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < NTILE; ++t) {
         const int r0 = row0 + t * 128, r1 = min(r0 + 128, n_rows);
         const int reach = r0 >= n_rows ? 0 : a.causal ? min(s.len, max(s.len - s.n_new + (r1 - 1) / a.group + 1, 0)) : s.len;
         n_blk[t] = (max(min(reach, k0 + a.chunk) - k0, 0) + BN - 1) / BN;
         sure[t] = a.causal ? s.len - s.n_new + r0 / a.group + 1 : s.len;
     }
-    const int n = max(n_blk[0], n_blk[1]);
+    const int n = NTILE == 1 ? n_blk[0] : max(n_blk[0], n_blk[NTILE - 1]);
     char * smem = smem_raw + ((1024 - ((uint32_t) __cvta_generic_to_shared(smem_raw) & 1023)) & 1023);
     const uint32_t sb = (uint32_t) __cvta_generic_to_shared(smem);
     const uint32_t k_full = sb + L::BAR, k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS, v_here = v_empty + 8 * NS,
@@ -200,13 +200,13 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
     if (tid == 0) {
         auto init = [](uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count)); };
         for (int i = 0; i < 5 * NS; ++i) init(k_full + 8 * i, 1);
-        init(q_full, 8);
-        for (int t = 0; t < 2; ++t) { init(s_full + 8 * t, 1); init(p_full + 8 * t, 4); init(o_full + 8 * t, 1); }
+        init(q_full, 4 * NTILE);
+        for (int t = 0; t < NTILE; ++t) { init(s_full + 8 * t, 1); init(p_full + 8 * t, 4); init(o_full + 8 * t, 1); }
         *abort_flag = 0;
         *odd_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == W_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(sb + L::MISC), "n"(COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -215,9 +215,9 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
     pt_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp < 8) {
+    if (warp < W_MMA) {
         // ================= softmax =================
-        const int t = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + t * 128 + r;
+        const int t = NTILE == 1 ? 0 : warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + t * 128 + r;
         const bool valid = row < n_rows;
         const int tok = valid ? row / a.group : 0, head = kvh * a.group + (valid ? row % a.group : 0);
         {
@@ -237,28 +237,33 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
         const float scale = fabsf(a.scale_log2);
         const int last = !valid ? -1 : a.causal ? s.len - s.n_new + tok : s.len - 1;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;              // 32 lanes per warp, in bits 16 and up
-        const uint32_t ts = tmem + lanes + t * BN, to = tmem + lanes + 2 * BN + t * D;
+        const uint32_t ts = tmem + lanes + t * BN, to = tmem + lanes + NTILE * BN + t * D;
         float m = -INFINITY, l = 0.0f;
         for (int j = 0; j < n_blk[t]; ++j) {
             if (!pt_wait_warp(s_full + 8 * t, j & 1, abort_flag, 1)) goto done;
             pt_after();
             const int seen = last + 1 - (k0 + j * BN);                   // this row sees the block's first `seen` keys
             const bool edge = k0 + (j + 1) * BN > sure[t];
-            uint32_t x[BN];
+            constexpr bool TWICE = MIN_CTAS > 1;                          // few registers: the scores are read once for the maximum, once for the weights
+            uint32_t x[TWICE ? 32 : BN];
+            if (!TWICE) {
 #pragma unroll
-            for (int c = 0; c < BN; c += 32) pt_ld32(x + c, ts + c);
+                for (int c = 0; c < BN; c += 32) pt_ld32(x + (TWICE ? 0 : c), ts + c);
+            }
             float m4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
-                pt_wait32(x + c);
+                uint32_t * y = x + (TWICE ? 0 : c);
+                if (TWICE) pt_ld32(y, ts + c);
+                pt_wait32(y);
                 if (edge) {
 #pragma unroll
-                    for (int i = c; i < c + 32; ++i) if (i >= seen) x[i] = 0xff800000u;
+                    for (int i = 0; i < 32; ++i) if (c + i >= seen) y[i] = 0xff800000u;
                 }
 #pragma unroll
-                for (int i = c; i < c + 32; i += 8)
+                for (int i = 0; i < 32; i += 8)
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], fmaxf(__uint_as_float(x[i + u]), __uint_as_float(x[i + 4 + u])));
+                    for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], fmaxf(__uint_as_float(y[i + u]), __uint_as_float(y[i + 4 + u])));
             }
             float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
             mx = mx == -INFINITY ? mx : mx * scale;
@@ -284,11 +289,12 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             const pt_f2 scale2 = pt_pair(scale, scale), base2 = pt_pair(base, base);
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
-                uint32_t w[16];
+                uint32_t w[16], * y = x + (TWICE ? 0 : c);
+                if (TWICE) { pt_ld32(y, ts + c); pt_wait32(y); }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     float y0, y1;
-                    pt_split(pt_fma2(pt_pair(__uint_as_float(x[c + 2 * i]), __uint_as_float(x[c + 2 * i + 1])), scale2, base2), y0, y1);
+                    pt_split(pt_fma2(pt_pair(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), scale2, base2), y0, y1);
                     if (edge) { if (c + 2 * i >= seen) y0 = -INFINITY; if (c + 2 * i + 1 >= seen) y1 = -INFINITY; }       // -inf * 0 is not -inf
                     y0 = pa_exp2(y0); y1 = pa_exp2(y1);
                     l2[i & 1] = pt_add2(l2[i & 1], pt_pair(y0, y1));
@@ -344,7 +350,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
         }
         if (valid && a.n_split > 1) { part[D] = m; part[D + 1] = l; }
         if (valid && a.n_split == 1 && a.lse) a.lse[out] = l == 0.0f ? -INFINITY : m * 0.69314718f + logf(l);
-    } else if (warp == 8) {
+    } else if (warp == W_MMA) {
         // ================= MMA issue =================
         if (lane == 0 && n > 0) {
             constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u << 7 | 1u << 10 : 0u;
@@ -359,18 +365,18 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             };
             if (!pt_wait(q_full, 0, abort_flag, 3) || !pt_wait(k_full, 0, abort_flag, 4)) goto done;
             pt_after();
-            for (int t = 0; t < 2; ++t) if (n_blk[t] > 0) scores(t, 0);
+            for (int t = 0; t < NTILE; ++t) if (n_blk[t] > 0) scores(t, 0);
             pt_commit(k_empty);
             for (int j = 0; j < n; ++j) {
                 if (!pt_wait(v_full + 8 * (j % NS), j / NS & 1, abort_flag, 5)) goto done;
                 if (j + 1 < n && !pt_wait(k_full + 8 * ((j + 1) % NS), (j + 1) / NS & 1, abort_flag, 6)) goto done;
-                for (int t = 0; t < 2; ++t) {
+                for (int t = 0; t < NTILE; ++t) {
                     if (j >= n_blk[t]) continue;
                     if (!pt_wait(p_full + 8 * t, j & 1, abort_flag, 7)) goto done;
                     pt_after();
                     const uint32_t v = sb + L::V + (j % NS) * L::TILE;
 #pragma unroll
-                    for (int i = 0; i < BN / 16; ++i) pt_mma_ts(tmem + 2 * BN + t * D, tmem + t * BN + i * 8, pt_desc(v + i * 2048, BN * 128), id_o, j > 0 || i > 0);
+                    for (int i = 0; i < BN / 16; ++i) pt_mma_ts(tmem + NTILE * BN + t * D, tmem + t * BN + i * 8, pt_desc(v + i * 2048, BN * 128), id_o, j > 0 || i > 0);
                     if (j + 1 < n_blk[t]) scores(t, j + 1);
                     else pt_commit(o_full + 8 * t);
                 }
@@ -380,7 +386,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
         }
     } else {
         // ================= K and V =================
-        const bool is_v = warp == 10;
+        const bool is_v = warp == W_MMA + 2;
         const char * base = (is_v ? a.v : a.k) + kvh * a.nb_head;
         const uint32_t ring = sb + (is_v ? L::V : L::K), full = is_v ? v_full : k_full, empty = is_v ? v_empty : k_empty;
         const int32_t * table = a.tables + seq * a.table_stride;
@@ -500,7 +506,7 @@ done:
     __syncwarp();
     pt_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == W_MMA) {
         pt_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "n"(COLS) : "memory");
     }
@@ -533,21 +539,21 @@ static void pt_make_maps(PtMaps & m, const PaArgs & a, int D, int BN, bool f16) 
     m.box = box;
 }
 
-template <typename T, int D, int BN, int NS, int MIN_CTAS>
+template <typename T, int D, int BN, int NS, int NTILE, int MIN_CTAS>
 static cudaError_t pt_go(const PaArgs & a, int n_seq, cudaStream_t st) {
-    const int smem = PtSmem<D, BN, NS>::BYTES;
-    const int64_t tiles = ((int64_t) a.max_new * a.group + PA_TC_ROWS - 1) / PA_TC_ROWS;
-    constexpr auto k = k_paged_attn_tc<T, D, BN, NS, MIN_CTAS>;
+    const int smem = PtSmem<D, BN, NS, NTILE>::BYTES;
+    const int64_t tiles = ((int64_t) a.max_new * a.group + 128 * NTILE - 1) / (128 * NTILE);
+    constexpr auto k = k_paged_attn_tc<T, D, BN, NS, NTILE, MIN_CTAS>;
     cudaError_t e = allow_once<k>(smem);
     if (e != cudaSuccess) return e;
     PtMaps maps;
     pt_make_maps(maps, a, D, BN, std::is_same<T, __half>::value);
-    e = launch_chained(k, dim3((unsigned) tiles, (unsigned) a.n_head_kv, (unsigned) (n_seq * a.n_split)), dim3(PT_THREADS), smem, st, a, maps);
+    e = launch_chained(k, dim3((unsigned) tiles, (unsigned) a.n_head_kv, (unsigned) (n_seq * a.n_split)), dim3(PT_THREADS(NTILE)), smem, st, a, maps);
     if (e == cudaSuccess) B200_LAUNCHED();
     return e;
 }
 
 cudaError_t pa_tc_launch(const PaArgs & a, int head_dim, int type, int n_seq, cudaStream_t st) {
-    if (head_dim == 64) return type == B200_TYPE_F16 ? pt_go<__half, 64, 64, 4, 2>(a, n_seq, st) : pt_go<__nv_bfloat16, 64, 64, 4, 2>(a, n_seq, st);
-    return type == B200_TYPE_F16 ? pt_go<__half, 128, 128, 2, 1>(a, n_seq, st) : pt_go<__nv_bfloat16, 128, 128, 2, 1>(a, n_seq, st);
+    if (head_dim == 64) return type == B200_TYPE_F16 ? pt_go<__half, 64, 64, 2, 1, 4>(a, n_seq, st) : pt_go<__nv_bfloat16, 64, 64, 2, 1, 4>(a, n_seq, st);
+    return type == B200_TYPE_F16 ? pt_go<__half, 128, 128, 2, 2, 1>(a, n_seq, st) : pt_go<__nv_bfloat16, 128, 128, 2, 2, 1>(a, n_seq, st);
 }

@@ -40,5 +40,5 @@ __device__ __forceinline__ int pa_reach(const PaArgs & a, const PaSeq & s, int r
 }
 
 // the tcgen05 form (k_paged_attn_tc.cu); rows of a tile, and its launch: a.n_split, a.chunk (a multiple of 128) and a.tile_rows are set
-#define PA_TC_ROWS 256
+#define PA_TC_ROWS(head_dim) ((head_dim) == 64 ? 128 : 256)
 cudaError_t pa_tc_launch(const PaArgs & a, int head_dim, int type, int n_seq, cudaStream_t st);

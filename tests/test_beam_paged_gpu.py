@@ -446,6 +446,9 @@ SHAPES = [
     ([(16, 100), (9, 9), (2, 300), (0, 7), (16, 17)], 2, 4, 64, 16),
     ([(1, 5000), (1, 1), (0, 0), (1, 777), (1, 4096), (1, 64)], 3, 2, 128, 16),
     ([(4, 3001), (1, 3), (3, 2500)], 2, 7, 64, 24),
+    ([(300, 2000), (129, 1300), (0, 0), (1, 900)], 2, 4, 128, 64),
+    ([(200, 1500), (70, 700), (5, 9), (3, 2)], 3, 3, 64, 16),
+    ([(150, 1200), (0, 0), (40, 2100)], 2, 2, 128, 24),
 ]
 
 

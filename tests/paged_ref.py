@@ -112,16 +112,25 @@ def attention(q, k, v, n_new, length, scale, causal):
     g = H // k.shape[1] if k.shape[1] else 1
     out, mag, lse = np.zeros(q.shape), np.zeros(q.shape), np.full(q.shape[:2], -np.inf)
     reach = np.zeros(q.shape[:2])
-    for t in range(n_new):
-        n = length - n_new + t + 1 if causal else length
-        if n <= 0:
-            continue
-        for h in range(H):
-            s = k[:n, h // g] @ q[t, h] * scale
-            m = s.max()
-            w = np.exp(s - m)
-            lse[t, h] = m + np.log(w.sum())
-            out[t, h] = w @ v[:n, h // g] / w.sum()
-            mag[t, h] = w @ np.abs(v[:n, h // g]) / w.sum()
-            reach[t, h] = (np.abs(k[:n, h // g]) @ np.abs(q[t, h])).max() * abs(scale)      # largest sum of |products| behind a score
+    seen = np.array([length - n_new + t + 1 if causal else length for t in range(n_new)])
+    hidden = np.arange(length)[None, :] >= seen[:, None]
+    rows = seen > 0
+    if length == 0 or not rows.any():
+        return out, lse, mag, reach
+    for h in range(H):
+        kh, vh = k[:, h // g], v[:, h // g]
+        with np.errstate(invalid="ignore"):
+            s = q[:, h] @ kh.T * scale
+        s[hidden] = -np.inf
+        s, hid = s[rows], hidden[rows]
+        m = s.max(1, keepdims=True)
+        w = np.exp(s - m)
+        w[hid] = 0
+        total = w.sum(1)
+        lse[rows, h] = m[:, 0] + np.log(total)
+        out[rows, h] = w @ vh / total[:, None]
+        mag[rows, h] = w @ np.abs(vh) / total[:, None]
+        a = np.abs(q[rows, h]) @ np.abs(kh).T                   # largest sum of |products| behind a score
+        a[hid] = 0
+        reach[rows, h] = a.max(1) * abs(scale)
     return out, lse, mag, reach

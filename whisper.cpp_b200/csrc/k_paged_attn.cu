@@ -147,9 +147,10 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     chain_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // the shuffle tells the compiler that the warp agrees
     PaDealer deal;
-    if (!pa_deal_init(a, ROUND, deal)) return;
+    if (!pa_deal_init(a, ROUND, deal, nullptr)) return;       // (no whole items before the line here: a.whole is 0)
     PaSeg g;
-    while (pa_deal_next(a, ROUND, deal, g)) {
+    int taken = 0;
+    while (pa_deal_next(a, ROUND, deal, g, nullptr, &taken)) {
     const PaSeq s = g.s;
     const int seq = g.seq, kvh = g.kvh, tile = g.tile, n_rows = g.n_rows, row0 = g.row0, k0 = g.k0, k1 = g.k1;
 
@@ -434,32 +435,30 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     }
 }
 
-// Joins the partial items: one warp per row of a sequence.  An item's rounds lie in CTAs c0 .. c1 of the line; the first left its part in
-// slot 1, the others in slot 0.
-template <typename Q, int D>
+// Joins the partial items.  CTA c of the line can have begun one item that it did not end: the one that holds the first step of CTA c + 1.
+// Block (c, y) joins rows of that item, a warp a row: CTA c left its part in slot 1, the CTAs up to the item's end theirs in slot 0.
+template <typename Q, int D, int round>
 __global__ void __launch_bounds__(128)
-k_paged_join(const __grid_constant__ PaArgs a, int round) {
+k_paged_join(const __grid_constant__ PaArgs a) {
     constexpr int DL = D / 32;
     chain_release();
     chain_wait();
-    const int lane = threadIdx.x & 31, seq = blockIdx.y;
-    const PaSeq s = pa_seq(a, seq);
-    if (s.n_new == 0) return;
-    const PaLine l = pa_line(a, round, 0, seq, nullptr, nullptr);
-    const int64_t head_steps = pa_head_steps(a, s, round);
-    int tile_at = -1;
-    int64_t tile_steps = 0;                               // steps of the tiles before tile_at
-    for (int64_t w = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 5); w < (int64_t) s.n_new * a.n_head; w += (int64_t) gridDim.x * 4) {
-        const int t = (int) (w / a.n_head), h = (int) (w - (int64_t) t * a.n_head), kvh = h / a.group, row = t * a.group + h % a.group, tile = row / a.tile_rows;
-        if (tile < tile_at) { tile_at = -1; tile_steps = 0; }       // a token's heads may lie in two tiles
-        for (; tile_at < tile; ++tile_at) if (tile_at >= 0) tile_steps += pa_tile_steps(a, s, tile_at, round);
-        const int64_t p0 = l.before + kvh * head_steps + tile_steps + PA_START, rounds = pa_tile_steps(a, s, tile, round) - PA_START;      // its first round
-        const int64_t c0 = ((p0 + 1) * a.stream - 1) / l.total, c1 = ((p0 + rounds) * a.stream - 1) / l.total;      // CTA c: from c * total / stream on
-        if (c0 == c1) continue;
-        const int n = (int) (c1 - c0 + 1);
-        auto part = [&](int i) { return a.part + (((c0 + i) * 2 + (i == 0)) * a.tile_rows + row % a.tile_rows) * (D + 4); };
+    const int lane = threadIdx.x & 31;
+    const int64_t c = blockIdx.x;
+    const PaLine l = pa_line(a, round);
+    const int64_t w0 = c * l.total / a.stream, w1 = (c + 1) * l.total / a.stream;
+    if (w0 == w1 || w1 >= l.total) return;
+    const PaPlace p = pa_locate(a, round, l, w1);
+    if (p.seq >= a.n_seq || p.at == 0) return;
+    const int64_t first = w1 - p.at + PA_START;           // the item's first round
+    if (first >= w1 || first < w0) return;
+    const PaSeq s = pa_seq(a, p.seq);
+    const int64_t c1 = ((w1 - p.at + pa_steps(s, round)) * a.stream - 1) / l.total;      // the CTA that has its last one
+    const int n = (int) (c1 - c + 1), row0 = p.tile * a.tile_rows, rows = min(a.tile_rows, s.n_new * a.group - row0);
+    auto some = [&](int i) { return l.total >= a.stream || (c + i + 1) * l.total / a.stream > (c + i) * l.total / a.stream; };       // fewer steps than CTAs leave some without
+    for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 4) {
+        auto part = [&](int i) { return a.part + (((c + i) * 2 + (i == 0)) * a.tile_rows + r) * (D + 4); };
         float mx = -INFINITY;
-        auto some = [&](int i) { return (c0 + i + 1) * l.total / a.stream > (c0 + i) * l.total / a.stream; };       // fewer steps than CTAs leave some without
         for (int i = lane; i < n; i += 32) if (some(i)) mx = fmaxf(mx, part(i)[D]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -467,13 +466,14 @@ k_paged_join(const __grid_constant__ PaArgs a, int round) {
         float sum = 0.0f, acc[DL] = {};
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
-            if (l.total < a.stream && !some(i)) continue;
-            const float * p = part(i);
-            const float f = pa_exp2(p[D] - base);
-            sum += f * p[D + 1];                          // NaN of a part without a finite maximum stays NaN
+            if (!some(i)) continue;
+            const float * q = part(i);
+            const float f = pa_exp2(q[D] - base);
+            sum += f * q[D + 1];                          // NaN of a part without a finite maximum stays NaN
 #pragma unroll
-            for (int j = 0; j < DL; ++j) { const float v = p[lane * DL + j]; if (f != 0.0f) acc[j] += f * v; }
+            for (int j = 0; j < DL; ++j) { const float v = q[lane * DL + j]; if (f != 0.0f) acc[j] += f * v; }
         }
+        const int t = (row0 + r) / a.group, h = p.kvh * a.group + (row0 + r) % a.group;
         const int64_t out = (s.tok0 + t) * a.n_head + h;
 #pragma unroll
         for (int j = 0; j < DL; ++j)
@@ -501,7 +501,7 @@ static bool pa_args_ok(const b200_page_pool * p, const b200_paged_attn_args * a,
 }
 
 // Which kernel, and how its work is dealt out.
-struct PaPlan { bool tc, store; int stream, round, tile_rows; };
+struct PaPlan { bool tc, store, whole; int stream, round, tile_rows; };
 static PaPlan pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a) {
     PaPlan r = {};
     const int64_t group = a->n_head / p->n_head_kv;
@@ -513,9 +513,10 @@ static PaPlan pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a) 
     const int64_t tiles = (rows + r.tile_rows - 1) / r.tile_rows, items = tiles * p->n_head_kv * a->n_seq, rounds = (a->max_len + r.round - 1) / r.round;
     const int64_t resident = 148 * (r.tc ? PA_TC_CTAS(p->head_dim) : a->q_type == B200_TYPE_F32 ? 2 : 3);
     // Items of few rounds are not worth the join, and items that fill the device many times over end together well enough by themselves.
-    if (rounds >= PA_MIN_ROUNDS && (tiles == 1 || (items < 8 * resident && tiles <= 64))) {
+    if (rounds >= PA_MIN_ROUNDS && (tiles == 1 || (items < (r.tc ? PA_WHOLE : 1) * resident && tiles <= 64))) {
         const int64_t want = items * rounds / (PA_MIN_ROUNDS / 2);
         r.stream = (int) (want < resident ? want : resident);
+        r.whole = r.tc && items >= r.stream;
     }
     return r;
 }
@@ -562,15 +563,10 @@ extern "C" int b200_paged_store(const b200_page_pool * pool, const b200_paged_at
 template <typename Q, typename KV, int D>
 static cudaError_t pa_launch(PaArgs & k, const PaNew & x, int n_seq, cudaStream_t st) {
     cudaError_t e;
-    const int64_t rows = (int64_t) k.max_new * k.n_head;
-    const dim3 join((unsigned) (rows < 16384 ? (rows + 3) / 4 : 4096), (unsigned) n_seq);
-    int round;
     if (k.tile_rows != PA_ROWS) {
-        round = PA_TC_KEYS(D);
         e = pa_tc_launch(k, D, std::is_same<KV, __half>::value ? B200_TYPE_F16 : B200_TYPE_BF16, n_seq, st);
     } else {
         constexpr int smem = 4 * PA_WARPS * PA_BLOCK;
-        round = PA_BLOCK / (2 * D) * PA_WARPS;
         e = allow_once<k_paged_attn<Q, KV, D>>(smem);
         if (e != cudaSuccess) return e;
         const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
@@ -579,7 +575,8 @@ static cudaError_t pa_launch(PaArgs & k, const PaNew & x, int n_seq, cudaStream_
         if (e == cudaSuccess) B200_LAUNCHED();
     }
     if (e != cudaSuccess || !k.stream) return e;
-    e = launch_chained(k_paged_join<Q, D>, join, dim3(128), 0, st, k, round);
+    e = k.tile_rows == PA_ROWS ? launch_chained(k_paged_join<Q, D, PA_BLOCK / (2 * D) * PA_WARPS>, dim3((unsigned) k.stream, 4), dim3(128), 0, st, k)
+                               : launch_chained(k_paged_join<Q, D, PA_TC_KEYS(D)>, dim3((unsigned) k.stream, 16), dim3(128), 0, st, k);
     if (e == cudaSuccess) B200_LAUNCHED();
     return e;
 }
@@ -589,7 +586,7 @@ extern "C" int b200_paged_attn(const b200_page_pool * pool, const b200_paged_att
     if (a->n_seq == 0 || a->n_tok == 0 || a->max_new == 0) return 0;
     PaArgs k = pa_pack(pool, a);
     const PaPlan r = pa_plan(pool, a);
-    k.stream = r.stream; k.tile_rows = r.tile_rows; k.n_seq = a->n_seq;
+    k.stream = r.stream; k.whole = r.whole; k.tile_rows = r.tile_rows; k.n_seq = a->n_seq;
     const int64_t need = b200_paged_attn_workspace(pool, a);
     if (need && (!a->workspace || (uintptr_t) a->workspace % 16 || a->workspace_bytes < need)) return B200_ERR_ARG;
     if (r.store) {

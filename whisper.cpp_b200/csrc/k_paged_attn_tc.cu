@@ -40,7 +40,8 @@ template <int D, int BN, int NS, int NTILE> struct PtSmem {
     static constexpr int Q = 0, K = NTILE * QT, V = K + NS * TILE, BAR = V + NS * TILE;
     static constexpr int N_BAR = 5 * NS + 8;             // k_full, k_empty, v_full, v_empty, v_here [NS]; q_full, s_full, p_full, o_full [2]
     static constexpr int MISC = BAR + N_BAR * 8;         // tensor-memory address, abort flag, odd-value flags [4]
-    static constexpr int BYTES = MISC + 32 + 1024;       // the dynamic array starts on 16 bytes: tiles are moved to 1024
+    static constexpr int ITEMS = MISC + 32, PIECES = ITEMS + PA_WHOLE * 12;       // whole items; a piece and a dealer per warp
+    static constexpr int BYTES = PIECES + (4 * NTILE + 3) * (int) (sizeof(PaSeg) + sizeof(PaDealer)) + 1024;       // the dynamic array starts on 16 bytes: tiles are moved to 1024
 };
 
 __device__ __forceinline__ bool pt_try(uint32_t bar, uint32_t parity) {
@@ -169,14 +170,22 @@ template <typename T, int D, int BN, int NS, int NTILE, int MIN_CTAS>
 __global__ void __launch_bounds__(PT_THREADS(NTILE), MIN_CTAS)
 k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps maps) {
     using L = PtSmem<D, BN, NS, NTILE>;
-    constexpr int COLS = NTILE * (BN + D) <= 128 ? 128 : NTILE * (BN + D) <= 256 ? 256 : 512, NC = D / 8, ROWS = 128 * NTILE, W_MMA = 4 * NTILE;
+    constexpr int COLS = NTILE * (BN + D) <= 128 ? 128 : NTILE * (BN + D) <= 256 ? 256 : 512, NC = D / 8, ROWS = 128 * NTILE, W_MMA = 4 * NTILE, W_ALL = W_MMA + 3;
     extern __shared__ __align__(16) char smem_raw[];
     chain_wait();                                         // no early release: this kernel wants whole SMs
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // the shuffle tells the compiler that the warp agrees
-    PaDealer deal;
-    if (!pa_deal_init(a, BN, deal)) return;
-    if (!a.stream && deal.tile * ROWS >= pa_seq(a, deal.seq).n_new * a.group) return;
     char * smem = smem_raw + ((1024 - ((uint32_t) __cvta_generic_to_shared(smem_raw) & 1023)) & 1023);
+    PaItem * items = (PaItem *) (smem + L::ITEMS);
+    // The current piece of work and the dealer's state of every warp live in shared memory: in registers they are spilled in the loop
+    volatile PaSeg * g = (volatile PaSeg *) (smem + L::PIECES) + warp;
+    PaDealer * deal_at = (PaDealer *) (smem + L::PIECES + W_ALL * sizeof(PaSeg)) + warp;
+    {
+        PaDealer deal;
+        if (!pa_deal_init(a, BN, deal, items)) return;
+        if (!a.stream && deal.tile * ROWS >= pa_seq(a, deal.seq).n_new * a.group) return;
+        if (lane == 0) *deal_at = deal;
+        __syncwarp();
+    }
     const uint32_t sb = (uint32_t) __cvta_generic_to_shared(smem);
     const uint32_t k_full = sb + L::BAR, k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS, v_here = v_empty + 8 * NS,
                    q_full = v_here + 8 * NS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16;
@@ -202,17 +211,26 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
 
     // Every role walks through the same pieces of work.  n_blk: blocks of a piece for each tile (a tile without rows has none); sure: keys below
     // are seen by every row of the tile; active: pieces so far that had blocks
-    PaSeg g;
-    int n_blk[NTILE], sure[NTILE], n, active = -1;
-    auto next = [&]() {
-        if (!pa_deal_next(a, BN, deal, g)) return false;
+    int n_blk[NTILE], sure[NTILE], n, active = -1, taken = 0;
+    auto next = [&](unsigned lanes) {                     // the given lanes of a warp together; lane 0 keeps the state
+        PaDealer deal = *deal_at;
+        PaSeg p;
+        const bool more = pa_deal_next(a, BN, deal, p, items, &taken);
+        if (!more) return false;
+        __syncwarp(lanes);
+        if (lane == 0) {
+            *deal_at = deal;
+            g->s.tok0 = p.s.tok0; g->s.n_new = p.s.n_new; g->s.len = p.s.len; g->seq = p.seq; g->kvh = p.kvh; g->row0 = p.row0; g->n_rows = p.n_rows;
+            g->k0 = p.k0; g->k1 = p.k1; g->whole = p.whole;
+        }
+        __syncwarp(lanes);
         n = 0;
 #pragma unroll
         for (int t = 0; t < NTILE; ++t) {
-            const int r0 = g.row0 + t * 128, r1 = min(r0 + 128, g.n_rows);
-            const int reach = r0 >= g.n_rows ? 0 : a.causal ? min(g.s.len, max(g.s.len - g.s.n_new + (r1 - 1) / a.group + 1, 0)) : g.s.len;
-            n_blk[t] = (max(min(reach, g.k1) - g.k0, 0) + BN - 1) / BN;
-            sure[t] = a.causal ? g.s.len - g.s.n_new + r0 / a.group + 1 : g.s.len;
+            const int r0 = p.row0 + t * 128, r1 = min(r0 + 128, p.n_rows);
+            const int reach = r0 >= p.n_rows ? 0 : a.causal ? min(p.s.len, max(p.s.len - p.s.n_new + (r1 - 1) / a.group + 1, 0)) : p.s.len;
+            n_blk[t] = (max(min(reach, p.k1) - p.k0, 0) + BN - 1) / BN;
+            sure[t] = a.causal ? p.s.len - p.s.n_new + r0 / a.group + 1 : p.s.len;
             n = max(n, n_blk[t]);
         }
         active += n > 0;
@@ -227,15 +245,14 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;              // 32 lanes per warp, in bits 16 and up
         const uint32_t ts = tmem + lanes + t * BN, to = tmem + lanes + NTILE * BN + t * D;
         uint32_t turn = 0, block = 0;                                     // this tile's pieces and blocks so far: the barriers' phases
-        while (next()) {
-        const PaSeq & s = g.s;
-        const int k0 = g.k0, nb = NTILE == 1 ? n_blk[0] : t ? n_blk[NTILE - 1] : n_blk[0], row = g.row0 + t * 128 + r;
+        while (next(0xffffffffu)) {
+        const int k0 = g->k0, nb = NTILE == 1 ? n_blk[0] : t ? n_blk[NTILE - 1] : n_blk[0], row = g->row0 + t * 128 + r;
         const int all_see = NTILE == 1 ? sure[0] : t ? sure[NTILE - 1] : sure[0];
-        const bool valid = row < g.n_rows;
-        const int tok = valid ? row / a.group : 0, head = g.kvh * a.group + (valid ? row % a.group : 0);
+        const bool valid = row < g->n_rows;
+        const int tok = valid ? row / a.group : 0, head = g->kvh * a.group + (valid ? row % a.group : 0);
         if (nb > 0) {
             // (the scores of the last piece are done: its o_full said so)
-            const char * q = a.q + (s.tok0 + tok) * a.nb_q_tok + head * a.nb_q_head;
+            const char * q = a.q + (g->s.tok0 + tok) * a.nb_q_tok + head * a.nb_q_head;
             char * dst = smem + L::Q + t * L::QT + r * 128;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -248,7 +265,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             __syncwarp();
             if (lane == 0) pt_arrive(q_full + 8 * t);
         }
-        const int last = !valid ? -1 : a.causal ? s.len - s.n_new + tok : s.len - 1;
+        const int last = !valid ? -1 : a.causal ? g->s.len - g->s.n_new + tok : g->s.len - 1;
         float m = -INFINITY, l = 0.0f;
         for (int j = 0; j < nb; ++j, ++block) {
             if (!pt_wait_warp(s_full + 8 * t, block & 1, abort_flag, 1)) goto done;
@@ -326,10 +343,11 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             pt_after();
             ++turn;
         }
-        const int64_t out = (s.tok0 + tok) * a.n_head + head;
+        const int64_t out = (g->s.tok0 + tok) * a.n_head + head;
         const bool odd = nb > 0 && odd_flag[active & 3] == active;
-        const float inv = !g.whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-        char * dst = a.dst + (s.tok0 + tok) * a.nb_dst_tok + head * a.nb_dst_head;
+        const bool whole = g->whole;
+        const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+        char * dst = a.dst + (g->s.tok0 + tok) * a.nb_dst_tok + head * a.nb_dst_head;
         float * part = a.part + (((int64_t) blockIdx.x * 2 + (k0 == 0)) * ROWS + t * 128 + r) * (D + 4);
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
@@ -341,15 +359,15 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             }
             if (odd && valid) {                                           // values that were taken out of V tiles, for the rows that see them
                 for (int key = k0 + max(0, sure[0] - k0) / BN * BN; key <= min(last, k0 + nb * BN - 1); ++key) {
-                    const int page = a.tables[g.seq * a.table_stride + key / a.page_size];
+                    const int page = a.tables[g->seq * a.table_stride + key / a.page_size];
                     if (page < 0 || page >= a.n_pages) continue;
-                    const T * v = (const T *) (a.v + page * a.nb_page + (key % a.page_size) * a.nb_tok + g.kvh * a.nb_head) + c;
+                    const T * v = (const T *) (a.v + page * a.nb_page + (key % a.page_size) * a.nb_tok + g->kvh * a.nb_head) + c;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) { const float y = (float) v[i]; if (!(fabsf(y) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + y); }
                 }
             }
             if (!valid) continue;
-            if (!g.whole) {
+            if (!whole) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) *(uint4 *) (part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             } else {
@@ -360,8 +378,8 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                 *(uint4 *) (dst + c * 2 + 16) = make_uint4(w[4], w[5], w[6], w[7]);
             }
         }
-        if (valid && !g.whole) { part[D] = m; part[D + 1] = l; }
-        if (valid && g.whole && a.lse) a.lse[out] = l == 0.0f ? -INFINITY : m * 0.69314718f + logf(l);
+        if (valid && !whole) { part[D] = m; part[D + 1] = l; }
+        if (valid && whole && a.lse) a.lse[out] = l == 0.0f ? -INFINITY : m * 0.69314718f + logf(l);
         }
     } else if (warp == W_MMA) {
         // ================= MMA issue =================
@@ -377,7 +395,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                     pt_mma_ss(tmem + t * BN, pt_desc(q + (i >> 2) * 128 * 128 + (i & 3) * 32, 16), pt_desc(k + (i >> 2) * BN * 128 + (i & 3) * 32, 16), id_s, i > 0);
                 pt_commit(s_full + 8 * t);
             };
-            while (next()) {
+            while (next(1u)) {
                 if (n == 0) continue;
                 if (!pt_wait(k_full + 8 * (u % NS), u / NS & 1, abort_flag, 4)) goto done;
 #pragma unroll
@@ -414,9 +432,9 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
         constexpr int G = BN / 32;
         const int box = maps.box;
         uint32_t u = 0;                                                   // blocks so far
-        while (next()) {
-        const int k0 = g.k0, k1 = g.k1;
-        const int32_t * table = a.tables + g.seq * a.table_stride;
+        while (next(0xffffffffu)) {
+        const int k0 = g->k0, k1 = g->k1, kvh = g->kvh;
+        const int32_t * table = a.tables + g->seq * a.table_stride;
         // V's non-finite values, in blocks that are not wholly seen, are taken out; a lane looks at the same 16-byte chunks that it copies
         auto clean = [&](int j) {
             auto place = [&](int q, int c) {
@@ -470,7 +488,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                 if (lane < per) {
                     const int tok = (k0 + j * BN + lane * box) % a.page_size;
 #pragma unroll
-                    for (int h = 0; h < D / 64; ++h) pt_tma(dst + h * BN * 128, is_v ? &maps.v : &maps.k, h * 64, g.kvh, tok, now, bar);
+                    for (int h = 0; h < D / 64; ++h) pt_tma(dst + h * BN * 128, is_v ? &maps.v : &maps.k, h * 64, kvh, tok, now, bar);
                 }
                 __syncwarp();
                 if (is_v) {
@@ -481,7 +499,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                 }
             }
         } else {
-            const char * base = (is_v ? a.v : a.k) + g.kvh * a.nb_head;
+            const char * base = (is_v ? a.v : a.k) + kvh * a.nb_head;
             int page[G];
             auto look = [&](int j) {
 #pragma unroll

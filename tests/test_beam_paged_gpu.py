@@ -449,7 +449,7 @@ SHAPES = [
     ([(300, 2000), (129, 1300), (0, 0), (1, 900)], 2, 4, 128, 64),
     ([(200, 1500), (70, 700), (5, 9), (3, 2)], 3, 3, 64, 16),
     ([(150, 1200), (0, 0), (40, 2100)], 2, 2, 128, 24),
-    ([(300, 1100), (280, 1030), (0, 0), (290, 1200), (257, 1025)], 20, 1, 128, 32),
+    ([(300, 1100), (280, 1030), (0, 0), (290, 1200), (257, 1025)], 20, 2, 128, 32),
     ([(260, 520)] * 3 + [(500, 700), (0, 3), (390, 1000)] + [(257, 514)] * 6, 20, 1, 64, 16),
 ]
 

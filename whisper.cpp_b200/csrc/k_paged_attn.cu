@@ -134,6 +134,48 @@ __device__ __forceinline__ void pa_ldm_t(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3},[%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 
+// How the work is dealt out.  Items are (sequence, key/value head, tile of 16 rows), numbered in that order; an item of a sequence of n keys
+// is ceil(n / round) rounds of PA_WARPS blocks, at least one.  Either a CTA takes one item (a.stream = 0), or the rounds of all items are one
+// line that is cut into a.stream equal parts, one per CTA: whatever the lengths, all CTAs end together.  On the line an item begins with
+// PA_START rounds of nothing, the time that it takes to get its first keys.  A CTA then has up to two partial items, at the ends of its
+// part; it leaves them in slots 0 (an item begun by another CTA) and 1, and k_paged_join puts them together.
+// (64 sequences of 1 to 8192 keys: 224 us without it, 183 with 2, 181 with 4 or 8.)
+#define PA_START 3
+struct PaLine { int64_t total, before; };                 // rounds of all sequences, and of those before a given one
+__device__ __forceinline__ int64_t pa_rounds(const PaArgs & a, const PaSeq & s, int round) {
+    return (int64_t) ((s.n_new * a.group + PA_ROWS - 1) / PA_ROWS) * a.n_head_kv * (max(1, (s.len + round - 1) / round) + PA_START);
+}
+// this warp's lanes go over the sequences, a run of them each
+__device__ __forceinline__ PaLine pa_line(const PaArgs & a, int round, int64_t target, int upto, int * seq_at, int64_t * rest) {
+    const int lane = threadIdx.x & 31, per = (a.n_seq + 31) / 32, s0 = min(a.n_seq, lane * per), s1 = min(a.n_seq, s0 + per);
+    int64_t mine = 0;
+    for (int s = s0; s < s1; ++s) mine += pa_rounds(a, pa_seq(a, s), round);
+    int64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int64_t u = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += u; }
+    PaLine l;
+    l.total = __shfl_sync(0xffffffffu, inc, 31);
+    l.before = 0;
+    if (upto >= 0) {                                       // rounds before sequence `upto`
+        int64_t b = inc - mine;
+        if (upto >= s0 && upto < s1) for (int s = s0; s < upto; ++s) b += pa_rounds(a, pa_seq(a, s), round);
+        l.before = __shfl_sync(0xffffffffu, b, upto / per);
+    }
+    if (seq_at) {                                          // the sequence that holds round target * total / a.stream
+        const int64_t w = target * l.total / a.stream;
+        const bool here = w >= inc - mine && w < inc;
+        int s = s0;
+        int64_t left = w - (inc - mine);
+        if (here) for (; s < s1; ++s) { const int64_t r = pa_rounds(a, pa_seq(a, s), round); if (left < r) break; left -= r; }
+        const unsigned who = __ballot_sync(0xffffffffu, here);
+        const int src = who ? __ffs(who) - 1 : 0;
+        *seq_at = who ? __shfl_sync(0xffffffffu, s, src) : a.n_seq;
+        *rest = __shfl_sync(0xffffffffu, left, src);
+    }
+    return l;
+}
+
+
 template <typename Q, typename KV, int D>
 __global__ void __launch_bounds__(32 * PA_WARPS, PaParts<Q, KV>::n == 1 ? 3 : 2)
 k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw) {
@@ -146,13 +188,29 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     // own (111 sequences of 4096 keys: 121 us a call, 85 without).
     chain_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // the shuffle tells the compiler that the warp agrees
-    PaDealer deal;
-    if (!pa_deal_init(a, ROUND, deal, nullptr)) return;       // (no whole items before the line here: a.whole is 0)
-    PaSeg g;
-    int taken = 0;
-    while (pa_deal_next(a, ROUND, deal, g, nullptr, &taken)) {
-    const PaSeq s = g.s;
-    const int seq = g.seq, kvh = g.kvh, tile = g.tile, n_rows = g.n_rows, row0 = g.row0, k0 = g.k0, k1 = g.k1;
+    int seq, kvh, tile, at = 0;                           // the item, and where in it (on the line) this CTA begins
+    int64_t todo = 1ll << 60;                             // what is left of this CTA's part
+    if (a.stream) {
+        int64_t rest;
+        const PaLine l = pa_line(a, ROUND, blockIdx.x, -1, &seq, &rest);
+        todo = ((int64_t) blockIdx.x + 1) * l.total / a.stream - (int64_t) blockIdx.x * l.total / a.stream;
+        if (seq >= a.n_seq || todo == 0) return;
+        const PaSeq s = pa_seq(a, seq);
+        const int rounds = max(1, (s.len + ROUND - 1) / ROUND), tiles = (s.n_new * a.group + PA_ROWS - 1) / PA_ROWS;
+        const int64_t item = rest / (rounds + PA_START);
+        at = (int) (rest - item * (rounds + PA_START));
+        kvh = (int) (item / tiles);
+        tile = (int) (item - (int64_t) kvh * tiles);
+    } else { seq = blockIdx.z; kvh = blockIdx.y; tile = gridDim.x - 1 - blockIdx.x; }      // the longest tiles first
+    for (;;) {
+    const PaSeq s = pa_seq(a, seq);
+    const int n_rows = s.n_new * a.group, row0 = tile * PA_ROWS;
+    if (!a.stream && row0 >= n_rows) return;
+    const int rounds = max(1, (s.len + ROUND - 1) / ROUND), steps = (int) min((int64_t) (rounds + PA_START - at), todo);
+    const int first_round = max(0, at - PA_START), n_round = max(0, at + steps - PA_START) - first_round;
+    const int k0 = first_round * ROUND, k1 = min(pa_reach(a, s, row0), k0 + n_round * ROUND);
+    const bool whole = n_round == rounds;
+    if (n_round > 0) {
 
     const char * kp = a.k + kvh * a.nb_head, * vp = a.v + kvh * a.nb_head;
     const int32_t * table = a.tables + seq * a.table_stride;
@@ -419,46 +477,56 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
         }
         const int t = row / a.group, h = kvh * a.group + row % a.group;
         const int64_t out = (s.tok0 + t) * a.n_head + h;
-        if (g.whole) {
+        if (whole) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             char * dst = a.dst + (s.tok0 + t) * a.nb_dst_tok + h * a.nb_dst_head + d * sizeof(Q);
             if constexpr (NP == 1) *(uint2 *) dst = make_uint2(P::two(x[0] * inv, x[1] * inv), P::two(x[2] * inv, x[3] * inv));
             else *(float4 *) dst = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
             if (a.lse && d == 0) a.lse[out] = sum == 0.0f ? -INFINITY : mx * 0.69314718f + logf(sum);
         } else {
-            float * p = a.part + (((int64_t) blockIdx.x * 2 + (g.k0 == 0)) * PA_ROWS + r) * (D + 4);
+            float * p = a.part + (((int64_t) blockIdx.x * 2 + (first_round == 0)) * PA_ROWS + r) * (D + 4);
             *(float4 *) (p + d) = make_float4(x[0], x[1], x[2], x[3]);
             if (d == 0) { p[D] = mx; p[D + 1] = sum; }
+        }
+    }
+    }
+    // the next item of this CTA's part
+    todo -= steps;
+    if (!a.stream || todo == 0) return;
+    at = 0;
+    if (++tile * PA_ROWS >= n_rows) {
+        tile = 0;
+        if (++kvh == a.n_head_kv) {
+            kvh = 0;
+            do { if (++seq >= a.n_seq) return; } while (pa_seq(a, seq).n_new == 0);
         }
     }
     __syncthreads();                                      // the accumulators are read before the ring is filled again
     }
 }
 
-// Joins the partial items.  CTA c of the line can have begun one item that it did not end: the one that holds the first step of CTA c + 1.
-// Block (c, y) joins rows of that item, a warp a row: CTA c left its part in slot 1, the CTAs up to the item's end theirs in slot 0.
-template <typename Q, int D, int round>
+// Joins the partial items: one warp per row of a sequence.  An item's rounds lie in CTAs c0 .. c1 of the line; the first left its part in
+// slot 1, the others in slot 0.
+template <typename Q, int D>
 __global__ void __launch_bounds__(128)
 k_paged_join(const __grid_constant__ PaArgs a) {
-    constexpr int DL = D / 32;
+    constexpr int DL = D / 32, ROUND = PA_BLOCK / (2 * D) * PA_WARPS;
     chain_release();
     chain_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t c = blockIdx.x;
-    const PaLine l = pa_line(a, round);
-    const int64_t w0 = c * l.total / a.stream, w1 = (c + 1) * l.total / a.stream;
-    if (w0 == w1 || w1 >= l.total) return;
-    const PaPlace p = pa_locate(a, round, l, w1);
-    if (p.seq >= a.n_seq || p.at == 0) return;
-    const int64_t first = w1 - p.at + PA_START;           // the item's first round
-    if (first >= w1 || first < w0) return;
-    const PaSeq s = pa_seq(a, p.seq);
-    const int64_t c1 = ((w1 - p.at + pa_steps(s, round)) * a.stream - 1) / l.total;      // the CTA that has its last one
-    const int n = (int) (c1 - c + 1), row0 = p.tile * a.tile_rows, rows = min(a.tile_rows, s.n_new * a.group - row0);
-    auto some = [&](int i) { return l.total >= a.stream || (c + i + 1) * l.total / a.stream > (c + i) * l.total / a.stream; };       // fewer steps than CTAs leave some without
-    for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 4) {
-        auto part = [&](int i) { return a.part + (((c + i) * 2 + (i == 0)) * a.tile_rows + r) * (D + 4); };
+    const int lane = threadIdx.x & 31, seq = blockIdx.y;
+    const PaSeq s = pa_seq(a, seq);
+    if (s.n_new == 0) return;
+    const PaLine l = pa_line(a, ROUND, 0, seq, nullptr, nullptr);
+    const int rounds = max(1, (s.len + ROUND - 1) / ROUND), tiles = (s.n_new * a.group + PA_ROWS - 1) / PA_ROWS;
+    for (int64_t w = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 5); w < (int64_t) s.n_new * a.n_head; w += (int64_t) gridDim.x * 4) {
+        const int t = (int) (w / a.n_head), h = (int) (w - (int64_t) t * a.n_head), kvh = h / a.group, row = t * a.group + h % a.group;
+        const int64_t p0 = l.before + ((int64_t) kvh * tiles + row / PA_ROWS) * (rounds + PA_START) + PA_START;      // its first round
+        const int64_t c0 = ((p0 + 1) * a.stream - 1) / l.total, c1 = ((p0 + rounds) * a.stream - 1) / l.total;      // CTA c: from c * total / stream on
+        if (c0 == c1) continue;
+        const int n = (int) (c1 - c0 + 1);
+        auto part = [&](int i) { return a.part + (((c0 + i) * 2 + (i == 0)) * PA_ROWS + row % PA_ROWS) * (D + 4); };
         float mx = -INFINITY;
+        auto some = [&](int i) { return (c0 + i + 1) * l.total / a.stream > (c0 + i) * l.total / a.stream; };       // fewer rounds than CTAs leave some without
         for (int i = lane; i < n; i += 32) if (some(i)) mx = fmaxf(mx, part(i)[D]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -466,14 +534,51 @@ k_paged_join(const __grid_constant__ PaArgs a) {
         float sum = 0.0f, acc[DL] = {};
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
-            if (!some(i)) continue;
-            const float * q = part(i);
-            const float f = pa_exp2(q[D] - base);
-            sum += f * q[D + 1];                          // NaN of a part without a finite maximum stays NaN
+            if (l.total < a.stream && !some(i)) continue;
+            const float * p = part(i);
+            const float f = pa_exp2(p[D] - base);
+            sum += f * p[D + 1];                          // NaN of a part without a finite maximum stays NaN
 #pragma unroll
-            for (int j = 0; j < DL; ++j) { const float v = q[lane * DL + j]; if (f != 0.0f) acc[j] += f * v; }
+            for (int j = 0; j < DL; ++j) { const float v = p[lane * DL + j]; if (f != 0.0f) acc[j] += f * v; }
         }
-        const int t = (row0 + r) / a.group, h = p.kvh * a.group + (row0 + r) % a.group;
+        const int64_t out = (s.tok0 + t) * a.n_head + h;
+#pragma unroll
+        for (int j = 0; j < DL; ++j)
+            ((Q *) (a.dst + (s.tok0 + t) * a.nb_dst_tok + h * a.nb_dst_head))[lane * DL + j] = (Q) (sum == 0.0f ? 0.0f : acc[j] / sum);
+        if (a.lse && lane == 0) a.lse[out] = sum == 0.0f ? -INFINITY : mx * 0.69314718f + logf(sum);
+    }
+}
+
+// Joins the splits of the tcgen05 form's last items: a warp a row, block (item, y).
+template <typename Q, int D>
+__global__ void __launch_bounds__(128)
+k_paged_join_tc(const __grid_constant__ PaArgs a) {
+    chain_release();
+    chain_wait();
+    constexpr int DL = D / 32;
+    const int lane = threadIdx.x & 31;
+    const PaItem item = pa_item(a, a.n_whole + blockIdx.x * a.n_split);
+    const PaSeq s = pa_seq(a, item.seq);
+    const int row0 = item.tile * a.tile_rows, rows = min(a.tile_rows, s.n_new * a.group - row0);
+    if (rows <= 0) return;
+    const int n = min(a.n_split, max(1, (pa_reach(a, s, row0) + a.chunk - 1) / a.chunk));
+    const int64_t step = (int64_t) a.tile_rows * (D + 4);
+    for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 4) {
+        const float * p = a.part + (item.slot * a.tile_rows + r) * (D + 4);
+        float mx = -INFINITY;
+        for (int i = lane; i < n; i += 32) mx = fmaxf(mx, p[i * step + D]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        float sum = 0.0f, acc[DL] = {};
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float f = pa_exp2(p[i * step + D] - base);
+            sum += f * p[i * step + D + 1];               // NaN of a split without a finite maximum stays NaN
+#pragma unroll
+            for (int j = 0; j < DL; ++j) { const float v = p[i * step + lane * DL + j]; if (f != 0.0f) acc[j] += f * v; }
+        }
+        const int t = (row0 + r) / a.group, h = item.kvh * a.group + (row0 + r) % a.group;
         const int64_t out = (s.tok0 + t) * a.n_head + h;
 #pragma unroll
         for (int j = 0; j < DL; ++j)
@@ -501,23 +606,34 @@ static bool pa_args_ok(const b200_page_pool * p, const b200_paged_attn_args * a,
 }
 
 // Which kernel, and how its work is dealt out.
-struct PaPlan { bool tc, store, whole; int stream, round, tile_rows; };
+struct PaPlan { bool tc, store; int stream, tiles, n_whole, n_split, chunk; int64_t items; };
 static PaPlan pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a) {
     PaPlan r = {};
     const int64_t group = a->n_head / p->n_head_kv;
     const int64_t new_max = a->max_new < a->n_tok ? a->max_new : a->n_tok, rows = new_max * group;
     r.tc = a->q_type != B200_TYPE_F32 && rows > PA_TC_MIN_ROWS;
     r.store = a->k_new && (r.tc || new_max > PA_ROWS);     // few new rows are stored by the kernel itself
-    r.round = r.tc ? PA_TC_KEYS(p->head_dim) : PA_BLOCK / (2 * p->head_dim) * PA_WARPS;
-    r.tile_rows = r.tc ? PA_TC_ROWS(p->head_dim) : PA_ROWS;
-    const int64_t tiles = (rows + r.tile_rows - 1) / r.tile_rows, items = tiles * p->n_head_kv * a->n_seq, rounds = (a->max_len + r.round - 1) / r.round;
+    const int64_t tile = r.tc ? PA_TC_ROWS(p->head_dim) : PA_ROWS, tiles = (rows + tile - 1) / tile;
+    const int64_t round = r.tc ? PA_TC_KEYS(p->head_dim) : PA_BLOCK / (2 * p->head_dim) * PA_WARPS, rounds = (a->max_len + round - 1) / round;
     const int64_t resident = 148 * (r.tc ? PA_TC_CTAS(p->head_dim) : a->q_type == B200_TYPE_F32 ? 2 : 3);
-    // Items of few rounds are not worth the join, and items that fill the device many times over end together well enough by themselves.
-    if (rounds >= PA_MIN_ROUNDS && (tiles == 1 || (items < (r.tc ? PA_WHOLE : 1) * resident && tiles <= 64))) {
-        const int64_t want = items * rounds / (PA_MIN_ROUNDS / 2);
-        r.stream = (int) (want < resident ? want : resident);
-        r.whole = r.tc && items >= r.stream;
+    r.items = tiles * p->n_head_kv * a->n_seq;
+    r.tiles = (int) tiles;
+    if (!r.tc) {
+        // Items of few rounds are not worth the join, and many tiles of a chunk fill the device by themselves (their reach differs, which
+        // the line does not know).
+        if (rounds >= PA_MIN_ROUNDS && (tiles == 1 || r.items < 2 * resident)) {
+            const int64_t want = r.items * rounds / (PA_MIN_ROUNDS / 2);
+            r.stream = (int) (want < resident ? want : resident);
+        }
+        return r;
     }
+    const int64_t whole = r.items / resident * resident, rest = r.items - whole;
+    int64_t split = rest ? resident / rest : 1;
+    if (split > rounds / (PA_MIN_ROUNDS / 2)) split = rounds / (PA_MIN_ROUNDS / 2);
+    if (whole > 8 * resident || split < 1) split = 1;      // the last of many waves is not worth the join
+    r.n_whole = (int) (split == 1 ? r.items : whole);
+    r.chunk = split == 1 ? 0 : (int) ((rounds + split - 1) / split * round);
+    r.n_split = split == 1 ? 1 : (int) ((a->max_len + r.chunk - 1) / r.chunk);
     return r;
 }
 
@@ -525,7 +641,7 @@ extern "C" int64_t b200_paged_attn_workspace(const b200_page_pool * pool, const 
     if (!a || !b200_pool_ok(pool, true) || a->n_tok < 1 || a->n_seq < 1 || a->max_new < 1 || a->max_len < 0 || a->max_len >= (1ll << 30) ||
         a->n_head < 1 || a->n_head % pool->n_head_kv) return 0;
     const PaPlan r = pa_plan(pool, a);
-    return (int64_t) r.stream * 2 * r.tile_rows * (pool->head_dim + 4) * 4;
+    return (r.tc ? (r.items - r.n_whole) * r.n_split * PA_TC_ROWS(pool->head_dim) : (int64_t) r.stream * 2 * PA_ROWS) * (pool->head_dim + 4) * 4;
 }
 
 static PaArgs pa_pack(const b200_page_pool * p, const b200_paged_attn_args * a) {
@@ -561,10 +677,14 @@ extern "C" int b200_paged_store(const b200_page_pool * pool, const b200_paged_at
 }
 
 template <typename Q, typename KV, int D>
-static cudaError_t pa_launch(PaArgs & k, const PaNew & x, int n_seq, cudaStream_t st) {
+static cudaError_t pa_launch(PaArgs & k, const PaNew & x, int n_seq, int64_t n_items, cudaStream_t st) {
     cudaError_t e;
+    const int64_t rows = (int64_t) k.max_new * k.n_head;
+    const dim3 join((unsigned) (rows < 16384 ? (rows + 3) / 4 : 4096), (unsigned) n_seq);
     if (k.tile_rows != PA_ROWS) {
-        e = pa_tc_launch(k, D, std::is_same<KV, __half>::value ? B200_TYPE_F16 : B200_TYPE_BF16, n_seq, st);
+        e = pa_tc_launch(k, D, std::is_same<KV, __half>::value ? B200_TYPE_F16 : B200_TYPE_BF16, n_items, st);
+        if (e != cudaSuccess || k.n_split == 1) return e;
+        e = launch_chained(k_paged_join_tc<Q, D>, dim3((unsigned) (n_items - k.n_whole), (unsigned) k.tile_rows / 16), dim3(128), 0, st, k);
     } else {
         constexpr int smem = 4 * PA_WARPS * PA_BLOCK;
         e = allow_once<k_paged_attn<Q, KV, D>>(smem);
@@ -572,11 +692,11 @@ static cudaError_t pa_launch(PaArgs & k, const PaNew & x, int n_seq, cudaStream_
         const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
         const dim3 grid = k.stream ? dim3((unsigned) k.stream) : dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) n_seq);
         e = launch_chained(k_paged_attn<Q, KV, D>, grid, dim3(32 * PA_WARPS), smem, st, k, x);
-        if (e == cudaSuccess) B200_LAUNCHED();
+        if (e != cudaSuccess) return e;
+        B200_LAUNCHED();
+        if (!k.stream) return cudaGetLastError();
+        e = launch_chained(k_paged_join<Q, D>, join, dim3(128), 0, st, k);
     }
-    if (e != cudaSuccess || !k.stream) return e;
-    e = k.tile_rows == PA_ROWS ? launch_chained(k_paged_join<Q, D, PA_BLOCK / (2 * D) * PA_WARPS>, dim3((unsigned) k.stream, 4), dim3(128), 0, st, k)
-                               : launch_chained(k_paged_join<Q, D, PA_TC_KEYS(D)>, dim3((unsigned) k.stream, 16), dim3(128), 0, st, k);
     if (e == cudaSuccess) B200_LAUNCHED();
     return e;
 }
@@ -586,7 +706,9 @@ extern "C" int b200_paged_attn(const b200_page_pool * pool, const b200_paged_att
     if (a->n_seq == 0 || a->n_tok == 0 || a->max_new == 0) return 0;
     PaArgs k = pa_pack(pool, a);
     const PaPlan r = pa_plan(pool, a);
-    k.stream = r.stream; k.whole = r.whole; k.tile_rows = r.tile_rows; k.n_seq = a->n_seq;
+    k.n_split = r.n_split; k.chunk = r.chunk; k.stream = r.stream; k.tile_rows = r.tc ? PA_TC_ROWS(pool->head_dim) : PA_ROWS; k.n_seq = a->n_seq;
+    k.tiles = r.tiles; k.n_whole = r.n_whole;
+    if (r.items > 0x7fffffff || (r.items - r.n_whole) * r.n_split > 0x7fffffff - r.n_whole) return B200_ERR_ARG;
     const int64_t need = b200_paged_attn_workspace(pool, a);
     if (need && (!a->workspace || (uintptr_t) a->workspace % 16 || a->workspace_bytes < need)) return B200_ERR_ARG;
     if (r.store) {
@@ -598,10 +720,10 @@ extern "C" int b200_paged_attn(const b200_page_pool * pool, const b200_paged_att
     const PaNew x = { r.store ? nullptr : (const char *) a->k_new, (const char *) a->v_new, a->nb_new_tok, a->nb_new_head };
     cudaError_t e;
     if (pool->head_dim == 64)
-        e = f32 ? (h ? pa_launch<float, __half, 64>(k, x, a->n_seq, st) : pa_launch<float, __nv_bfloat16, 64>(k, x, a->n_seq, st))
-                : (h ? pa_launch<__half, __half, 64>(k, x, a->n_seq, st) : pa_launch<__nv_bfloat16, __nv_bfloat16, 64>(k, x, a->n_seq, st));
+        e = f32 ? (h ? pa_launch<float, __half, 64>(k, x, a->n_seq, r.items, st) : pa_launch<float, __nv_bfloat16, 64>(k, x, a->n_seq, r.items, st))
+                : (h ? pa_launch<__half, __half, 64>(k, x, a->n_seq, r.items, st) : pa_launch<__nv_bfloat16, __nv_bfloat16, 64>(k, x, a->n_seq, r.items, st));
     else
-        e = f32 ? (h ? pa_launch<float, __half, 128>(k, x, a->n_seq, st) : pa_launch<float, __nv_bfloat16, 128>(k, x, a->n_seq, st))
-                : (h ? pa_launch<__half, __half, 128>(k, x, a->n_seq, st) : pa_launch<__nv_bfloat16, __nv_bfloat16, 128>(k, x, a->n_seq, st));
+        e = f32 ? (h ? pa_launch<float, __half, 128>(k, x, a->n_seq, r.items, st) : pa_launch<float, __nv_bfloat16, 128>(k, x, a->n_seq, r.items, st))
+                : (h ? pa_launch<__half, __half, 128>(k, x, a->n_seq, r.items, st) : pa_launch<__nv_bfloat16, __nv_bfloat16, 128>(k, x, a->n_seq, r.items, st));
     return (int) e;
 }

@@ -38,10 +38,9 @@ extern "C" int b200_paged_attn_status(void) {
 template <int D, int BN, int NS, int NTILE> struct PtSmem {
     static constexpr int TILE = BN * D * 2, QT = 128 * D * 2;
     static constexpr int Q = 0, K = NTILE * QT, V = K + NS * TILE, BAR = V + NS * TILE;
-    static constexpr int N_BAR = 5 * NS + 8;             // k_full, k_empty, v_full, v_empty, v_here [NS]; q_full, s_full, p_full, o_full [2]
-    static constexpr int MISC = BAR + N_BAR * 8;         // tensor-memory address, abort flag, odd-value flags [4]
-    static constexpr int ITEMS = MISC + 32, PIECES = ITEMS + PA_WHOLE * 12;       // whole items; a piece and a dealer per warp
-    static constexpr int BYTES = PIECES + (4 * NTILE + 3) * (int) (sizeof(PaSeg) + sizeof(PaDealer)) + 1024;       // the dynamic array starts on 16 bytes: tiles are moved to 1024
+    static constexpr int N_BAR = 5 * NS + 7;             // k_full, k_empty, v_full, v_empty, v_here [NS]; q_full; s_full, p_full, o_full [2]
+    static constexpr int MISC = BAR + N_BAR * 8;         // tensor-memory address, abort flag, odd-value flag
+    static constexpr int BYTES = MISC + 16 + 1024;       // the dynamic array starts on 16 bytes: tiles are moved to 1024
 };
 
 __device__ __forceinline__ bool pt_try(uint32_t bar, uint32_t parity) {
@@ -170,34 +169,41 @@ template <typename T, int D, int BN, int NS, int NTILE, int MIN_CTAS>
 __global__ void __launch_bounds__(PT_THREADS(NTILE), MIN_CTAS)
 k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps maps) {
     using L = PtSmem<D, BN, NS, NTILE>;
-    constexpr int COLS = NTILE * (BN + D) <= 128 ? 128 : NTILE * (BN + D) <= 256 ? 256 : 512, NC = D / 8, ROWS = 128 * NTILE, W_MMA = 4 * NTILE, W_ALL = W_MMA + 3;
+    constexpr int COLS = NTILE * (BN + D) <= 128 ? 128 : NTILE * (BN + D) <= 256 ? 256 : 512, NC = D / 8, ROWS = 128 * NTILE, W_MMA = 4 * NTILE;
     extern __shared__ __align__(16) char smem_raw[];
     chain_wait();                                         // no early release: this kernel wants whole SMs
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // the shuffle tells the compiler that the warp agrees
-    char * smem = smem_raw + ((1024 - ((uint32_t) __cvta_generic_to_shared(smem_raw) & 1023)) & 1023);
-    PaItem * items = (PaItem *) (smem + L::ITEMS);
-    // The current piece of work and the dealer's state of every warp live in shared memory: in registers they are spilled in the loop
-    volatile PaSeg * g = (volatile PaSeg *) (smem + L::PIECES) + warp;
-    PaDealer * deal_at = (PaDealer *) (smem + L::PIECES + W_ALL * sizeof(PaSeg)) + warp;
-    {
-        PaDealer deal;
-        if (!pa_deal_init(a, BN, deal, items)) return;
-        if (!a.stream && deal.tile * ROWS >= pa_seq(a, deal.seq).n_new * a.group) return;
-        if (lane == 0) *deal_at = deal;
-        __syncwarp();
+    const PaItem item = pa_item(a, blockIdx.x);
+    const int seq = item.seq, split = max(item.split, 0), kvh = item.kvh, row0 = item.tile * ROWS, chunk = item.split < 0 ? 1 << 30 : a.chunk;
+    const PaSeq s = pa_seq(a, seq);
+    const int n_rows = s.n_new * a.group;
+    if (row0 >= n_rows) return;
+    const int k0 = split * chunk, k1 = min(pa_reach(a, s, row0), k0 + chunk);
+    if (k0 >= k1 && split != 0) return;                  // an empty split: the join does not read it
+    // blocks of each tile; a tile without rows has none
+    int n_blk[NTILE], sure[NTILE];                               // sure: keys below are seen by every row of the tile
+#pragma unroll
+    for (int t = 0; t < NTILE; ++t) {
+        const int r0 = row0 + t * 128, r1 = min(r0 + 128, n_rows);
+        const int reach = r0 >= n_rows ? 0 : a.causal ? min(s.len, max(s.len - s.n_new + (r1 - 1) / a.group + 1, 0)) : s.len;
+        n_blk[t] = (max(min(reach, k0 + chunk) - k0, 0) + BN - 1) / BN;
+        sure[t] = a.causal ? s.len - s.n_new + r0 / a.group + 1 : s.len;
     }
+    const int n = NTILE == 1 ? n_blk[0] : max(n_blk[0], n_blk[NTILE - 1]);
+    char * smem = smem_raw + ((1024 - ((uint32_t) __cvta_generic_to_shared(smem_raw) & 1023)) & 1023);
     const uint32_t sb = (uint32_t) __cvta_generic_to_shared(smem);
     const uint32_t k_full = sb + L::BAR, k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS, v_here = v_empty + 8 * NS,
-                   q_full = v_here + 8 * NS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16;
+                   q_full = v_here + 8 * NS, s_full = q_full + 8, p_full = s_full + 16, o_full = p_full + 16;
     uint32_t * tmem_slot = (uint32_t *) (smem + L::MISC);
     volatile int * abort_flag = (volatile int *) (smem + L::MISC + 4);
     volatile int * odd_flag = (volatile int *) (smem + L::MISC + 8);
     if (tid == 0) {
         auto init = [](uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count)); };
         for (int i = 0; i < 5 * NS; ++i) init(k_full + 8 * i, 1);
-        for (int t = 0; t < NTILE; ++t) { init(q_full + 8 * t, 4); init(s_full + 8 * t, 1); init(p_full + 8 * t, 4); init(o_full + 8 * t, 1); }
+        init(q_full, 4 * NTILE);
+        for (int t = 0; t < NTILE; ++t) { init(s_full + 8 * t, 1); init(p_full + 8 * t, 4); init(o_full + 8 * t, 1); }
         *abort_flag = 0;
-        for (int i = 0; i < 4; ++i) odd_flag[i] = -1;
+        *odd_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == W_MMA) {
@@ -209,50 +215,14 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
     pt_after();
     const uint32_t tmem = *tmem_slot;
 
-    // Every role walks through the same pieces of work.  n_blk: blocks of a piece for each tile (a tile without rows has none); sure: keys below
-    // are seen by every row of the tile; active: pieces so far that had blocks
-    int n_blk[NTILE], sure[NTILE], n, active = -1, taken = 0;
-    auto next = [&](unsigned lanes) {                     // the given lanes of a warp together; lane 0 keeps the state
-        PaDealer deal = *deal_at;
-        PaSeg p;
-        const bool more = pa_deal_next(a, BN, deal, p, items, &taken);
-        if (!more) return false;
-        __syncwarp(lanes);
-        if (lane == 0) {
-            *deal_at = deal;
-            g->s.tok0 = p.s.tok0; g->s.n_new = p.s.n_new; g->s.len = p.s.len; g->seq = p.seq; g->kvh = p.kvh; g->row0 = p.row0; g->n_rows = p.n_rows;
-            g->k0 = p.k0; g->k1 = p.k1; g->whole = p.whole;
-        }
-        __syncwarp(lanes);
-        n = 0;
-#pragma unroll
-        for (int t = 0; t < NTILE; ++t) {
-            const int r0 = p.row0 + t * 128, r1 = min(r0 + 128, p.n_rows);
-            const int reach = r0 >= p.n_rows ? 0 : a.causal ? min(p.s.len, max(p.s.len - p.s.n_new + (r1 - 1) / a.group + 1, 0)) : p.s.len;
-            n_blk[t] = (max(min(reach, p.k1) - p.k0, 0) + BN - 1) / BN;
-            sure[t] = a.causal ? p.s.len - p.s.n_new + r0 / a.group + 1 : p.s.len;
-            n = max(n, n_blk[t]);
-        }
-        active += n > 0;
-        return true;
-    };
-
     if (warp < W_MMA) {
         // ================= softmax =================
-        const int t = NTILE == 1 ? 0 : warp >> 2, r = (warp & 3) * 32 + lane;
-        const uint32_t flip = a.scale_log2 < 0 ? 0x80008000u : 0;        // a negative scale goes into the signs of Q: the maximum is then one of S
-        const float scale = fabsf(a.scale_log2);
-        const uint32_t lanes = (uint32_t) (warp & 3) << 21;              // 32 lanes per warp, in bits 16 and up
-        const uint32_t ts = tmem + lanes + t * BN, to = tmem + lanes + NTILE * BN + t * D;
-        uint32_t turn = 0, block = 0;                                     // this tile's pieces and blocks so far: the barriers' phases
-        while (next(0xffffffffu)) {
-        const int k0 = g->k0, nb = NTILE == 1 ? n_blk[0] : t ? n_blk[NTILE - 1] : n_blk[0], row = g->row0 + t * 128 + r;
-        const int all_see = NTILE == 1 ? sure[0] : t ? sure[NTILE - 1] : sure[0];
-        const bool valid = row < g->n_rows;
-        const int tok = valid ? row / a.group : 0, head = g->kvh * a.group + (valid ? row % a.group : 0);
-        if (nb > 0) {
-            // (the scores of the last piece are done: its o_full said so)
-            const char * q = a.q + (g->s.tok0 + tok) * a.nb_q_tok + head * a.nb_q_head;
+        const int t = NTILE == 1 ? 0 : warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + t * 128 + r;
+        const bool valid = row < n_rows;
+        const int tok = valid ? row / a.group : 0, head = kvh * a.group + (valid ? row % a.group : 0);
+        {
+            const uint32_t flip = a.scale_log2 < 0 ? 0x80008000u : 0;   // a negative scale goes into the signs of Q: the maximum is then one of S
+            const char * q = a.q + (s.tok0 + tok) * a.nb_q_tok + head * a.nb_q_head;
             char * dst = smem + L::Q + t * L::QT + r * 128;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -261,17 +231,19 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                 *(uint4 *) (dst + (c >> 3) * 128 * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
             }
             pt_proxy_fence();
-            pt_before();                                                  // the last piece's O has been read
             __syncwarp();
-            if (lane == 0) pt_arrive(q_full + 8 * t);
+            if (lane == 0) pt_arrive(q_full);
         }
-        const int last = !valid ? -1 : a.causal ? g->s.len - g->s.n_new + tok : g->s.len - 1;
+        const float scale = fabsf(a.scale_log2);
+        const int last = !valid ? -1 : a.causal ? s.len - s.n_new + tok : s.len - 1;
+        const uint32_t lanes = (uint32_t) (warp & 3) << 21;              // 32 lanes per warp, in bits 16 and up
+        const uint32_t ts = tmem + lanes + t * BN, to = tmem + lanes + NTILE * BN + t * D;
         float m = -INFINITY, l = 0.0f;
-        for (int j = 0; j < nb; ++j, ++block) {
-            if (!pt_wait_warp(s_full + 8 * t, block & 1, abort_flag, 1)) goto done;
+        for (int j = 0; j < n_blk[t]; ++j) {
+            if (!pt_wait_warp(s_full + 8 * t, j & 1, abort_flag, 1)) goto done;
             pt_after();
             const int seen = last + 1 - (k0 + j * BN);                   // this row sees the block's first `seen` keys
-            const bool edge = k0 + (j + 1) * BN > all_see;
+            const bool edge = k0 + (j + 1) * BN > sure[t];
             constexpr bool TWICE = MIN_CTAS > 1;                          // few registers: the scores are read once for the maximum, once for the weights
             uint32_t x[TWICE ? 32 : BN];
             if (!TWICE) {
@@ -338,30 +310,29 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             __syncwarp();
             if (lane == 0) pt_arrive(p_full + 8 * t);
         }
-        if (nb > 0) {
-            if (!pt_wait_warp(o_full + 8 * t, turn & 1, abort_flag, 2)) goto done;
+        if (n_blk[t] > 0) {
+            if (!pt_wait_warp(o_full + 8 * t, 0, abort_flag, 2)) goto done;
             pt_after();
-            ++turn;
         }
-        const int64_t out = (g->s.tok0 + tok) * a.n_head + head;
-        const bool odd = nb > 0 && odd_flag[active & 3] == active;
-        const bool whole = g->whole;
+        const int64_t out = (s.tok0 + tok) * a.n_head + head;
+        const bool odd = n_blk[t] > 0 && *odd_flag;
+        const bool whole = item.split < 0;
         const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-        char * dst = a.dst + (g->s.tok0 + tok) * a.nb_dst_tok + head * a.nb_dst_head;
-        float * part = a.part + (((int64_t) blockIdx.x * 2 + (k0 == 0)) * ROWS + t * 128 + r) * (D + 4);
+        char * dst = a.dst + (s.tok0 + tok) * a.nb_dst_tok + head * a.nb_dst_head;
+        float * part = a.part + (item.slot * ROWS + t * 128 + r) * (D + 4);
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
             uint32_t o[16];
-            if (nb > 0) { pt_ld16(o, to + c); pt_wait16(o); }
+            if (n_blk[t] > 0) { pt_ld16(o, to + c); pt_wait16(o); }
             else {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[i] = 0;
             }
             if (odd && valid) {                                           // values that were taken out of V tiles, for the rows that see them
-                for (int key = k0 + max(0, sure[0] - k0) / BN * BN; key <= min(last, k0 + nb * BN - 1); ++key) {
-                    const int page = a.tables[g->seq * a.table_stride + key / a.page_size];
+                for (int key = k0 + max(0, sure[0] - k0) / BN * BN; key <= min(last, k0 + n_blk[t] * BN - 1); ++key) {
+                    const int page = a.tables[seq * a.table_stride + key / a.page_size];
                     if (page < 0 || page >= a.n_pages) continue;
-                    const T * v = (const T *) (a.v + page * a.nb_page + (key % a.page_size) * a.nb_tok + g->kvh * a.nb_head) + c;
+                    const T * v = (const T *) (a.v + page * a.nb_page + (key % a.page_size) * a.nb_tok + kvh * a.nb_head) + c;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) { const float y = (float) v[i]; if (!(fabsf(y) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + y); }
                 }
@@ -380,87 +351,74 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
         }
         if (valid && !whole) { part[D] = m; part[D + 1] = l; }
         if (valid && whole && a.lse) a.lse[out] = l == 0.0f ? -INFINITY : m * 0.69314718f + logf(l);
-        }
     } else if (warp == W_MMA) {
         // ================= MMA issue =================
-        if (lane == 0) {
+        if (lane == 0 && n > 0) {
             constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u << 7 | 1u << 10 : 0u;
             constexpr uint32_t id_s = 1u << 4 | type | (uint32_t) (BN >> 3) << 17 | 128u >> 4 << 24;
             constexpr uint32_t id_o = 1u << 4 | type | 1u << 16 | (uint32_t) (D >> 3) << 17 | 128u >> 4 << 24;
-            uint32_t u = 0, turn[NTILE] = {}, block[NTILE] = {};          // blocks of K and V so far; pieces and blocks of each tile: the barriers' phases
-            auto scores = [&](int t, uint32_t v) {
-                const uint32_t q = sb + L::Q + t * L::QT, k = sb + L::K + (v % NS) * L::TILE;
+            auto scores = [&](int t, int j) {
+                const uint32_t q = sb + L::Q + t * L::QT, k = sb + L::K + (j % NS) * L::TILE;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
                     pt_mma_ss(tmem + t * BN, pt_desc(q + (i >> 2) * 128 * 128 + (i & 3) * 32, 16), pt_desc(k + (i >> 2) * BN * 128 + (i & 3) * 32, 16), id_s, i > 0);
                 pt_commit(s_full + 8 * t);
             };
-            while (next(1u)) {
-                if (n == 0) continue;
-                if (!pt_wait(k_full + 8 * (u % NS), u / NS & 1, abort_flag, 4)) goto done;
-#pragma unroll
+            if (!pt_wait(q_full, 0, abort_flag, 3) || !pt_wait(k_full, 0, abort_flag, 4)) goto done;
+            pt_after();
+            for (int t = 0; t < NTILE; ++t) if (n_blk[t] > 0) scores(t, 0);
+            pt_commit(k_empty);
+            for (int j = 0; j < n; ++j) {
+                if (!pt_wait(v_full + 8 * (j % NS), j / NS & 1, abort_flag, 5)) goto done;
+                if (j + 1 < n && !pt_wait(k_full + 8 * ((j + 1) % NS), (j + 1) / NS & 1, abort_flag, 6)) goto done;
                 for (int t = 0; t < NTILE; ++t) {
-                    if (n_blk[t] == 0) continue;
-                    if (!pt_wait(q_full + 8 * t, turn[t]++ & 1, abort_flag, 3)) goto done;
+                    if (j >= n_blk[t]) continue;
+                    if (!pt_wait(p_full + 8 * t, j & 1, abort_flag, 7)) goto done;
                     pt_after();
-                    scores(t, u);
-                }
-                pt_commit(k_empty + 8 * (u % NS));
-                for (int j = 0; j < n; ++j, ++u) {
-                    if (!pt_wait(v_full + 8 * (u % NS), u / NS & 1, abort_flag, 5)) goto done;
-                    if (j + 1 < n && !pt_wait(k_full + 8 * ((u + 1) % NS), (u + 1) / NS & 1, abort_flag, 6)) goto done;
+                    const uint32_t v = sb + L::V + (j % NS) * L::TILE;
 #pragma unroll
-                    for (int t = 0; t < NTILE; ++t) {
-                        if (j >= n_blk[t]) continue;
-                        if (!pt_wait(p_full + 8 * t, block[t]++ & 1, abort_flag, 7)) goto done;
-                        pt_after();
-                        const uint32_t v = sb + L::V + (u % NS) * L::TILE;
-#pragma unroll
-                        for (int i = 0; i < BN / 16; ++i) pt_mma_ts(tmem + NTILE * BN + t * D, tmem + t * BN + i * 8, pt_desc(v + i * 2048, BN * 128), id_o, j > 0 || i > 0);
-                        if (j + 1 < n_blk[t]) scores(t, u + 1);
-                        else pt_commit(o_full + 8 * t);
-                    }
-                    pt_commit(v_empty + 8 * (u % NS));
-                    if (j + 1 < n) pt_commit(k_empty + 8 * ((u + 1) % NS));
+                    for (int i = 0; i < BN / 16; ++i) pt_mma_ts(tmem + NTILE * BN + t * D, tmem + t * BN + i * 8, pt_desc(v + i * 2048, BN * 128), id_o, j > 0 || i > 0);
+                    if (j + 1 < n_blk[t]) scores(t, j + 1);
+                    else pt_commit(o_full + 8 * t);
                 }
+                pt_commit(v_empty + 8 * (j % NS));
+                if (j + 1 < n) pt_commit(k_empty + 8 * ((j + 1) % NS));
             }
         }
     } else {
         // ================= K and V =================
         const bool is_v = warp == W_MMA + 2;
+        const char * base = (is_v ? a.v : a.k) + kvh * a.nb_head;
         const uint32_t ring = sb + (is_v ? L::V : L::K), full = is_v ? v_full : k_full, empty = is_v ? v_empty : k_empty;
-        constexpr int G = BN / 32;
+        const int32_t * table = a.tables + seq * a.table_stride;
+        constexpr int G = BN / 32, LAG = NS - 2;
         const int box = maps.box;
-        uint32_t u = 0;                                                   // blocks so far
-        while (next(0xffffffffu)) {
-        const int k0 = g->k0, k1 = g->k1, kvh = g->kvh;
-        const int32_t * table = a.tables + g->seq * a.table_stride;
         // V's non-finite values, in blocks that are not wholly seen, are taken out; a lane looks at the same 16-byte chunks that it copies
-        auto clean = [&](int j) {
-            auto place = [&](int q, int c) {
+        auto clean = [&](int jj) {
+            auto place = [&](int g, int c) {
                 const int i = c * 32 + lane, r = i / NC, ch = i % NC;
-                return (uint4 *) (smem + L::V + (u % NS) * L::TILE + (ch >> 3) * BN * 128 + (q * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                return (uint4 *) (smem + L::V + (jj % NS) * L::TILE + (ch >> 3) * BN * 128 + (g * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4));
             };
             float any = 0.0f;                                             // NaN as soon as a value is infinite or NaN: x * 0
-            const int rows = k1 - (k0 + j * BN);                          // behind them nobody looks: zeros, whatever the page holds
+            const int rows = k1 - (k0 + jj * BN);                         // behind them nobody looks: zeros, whatever the page holds
 #pragma unroll
-            for (int q = 0; q < G; ++q)
+            for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
-                    if (q * 32 + (c * 32 + lane) / NC < rows) any = pt_zero_times<T>(*place(q, c), any);
-                    else *place(q, c) = make_uint4(0, 0, 0, 0);
+                    if (g * 32 + (c * 32 + lane) / NC < rows) any = pt_zero_times<T>(*place(g, c), any);
+                    else *place(g, c) = make_uint4(0, 0, 0, 0);
                 }
             if (any != any) {
 #pragma unroll 1
-                for (int q = 0; q < G; ++q)
+                for (int g = 0; g < G; ++g)
 #pragma unroll 1
                     for (int c = 0; c < NC; ++c) {
-                        uint4 * p = place(q, c);
+                        uint4 * p = place(g, c);
                         uint4 x = *p;
                         x.x &= ~pt_odd<T>(x.x); x.y &= ~pt_odd<T>(x.y); x.z &= ~pt_odd<T>(x.z); x.w &= ~pt_odd<T>(x.w);
                         *p = x;
                     }
-                odd_flag[active & 3] = active;                            // (V is at most two blocks ahead of the rows that ask for it)
+                *odd_flag = 1;
             }
             pt_proxy_fence();
         };
@@ -475,68 +433,74 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                 return p < 0 || p > a.n_pages ? a.n_pages : p;
             };
             int page = page_of(0);
-            for (int j = 0; j < n; ++j, ++u) {
-                const int now = page;
-                page = page_of(j + 1);
-                if (!pt_wait_warp(empty + 8 * (u % NS), (u / NS & 1) ^ 1, abort_flag, 8)) {
-                    for (uint32_t i = u < NS ? 0 : u - NS; i < u; ++i) pt_poll((is_v ? v_here : k_full) + 8 * (i % NS), i / NS & 1);       // copies under way
-                    goto done;
-                }
-                const uint32_t bar = (is_v ? v_here : k_full) + 8 * (u % NS), dst = ring + (u % NS) * L::TILE + lane * box * 128;
-                if (lane == 0) pt_expect(bar, L::TILE);
-                __syncwarp();
-                if (lane < per) {
-                    const int tok = (k0 + j * BN + lane * box) % a.page_size;
-#pragma unroll
-                    for (int h = 0; h < D / 64; ++h) pt_tma(dst + h * BN * 128, is_v ? &maps.v : &maps.k, h * 64, kvh, tok, now, bar);
-                }
-                __syncwarp();
-                if (is_v) {
-                    if (!pt_wait_warp(v_here + 8 * (u % NS), u / NS & 1, abort_flag, 9)) goto done;
-                    if (k0 + (j + 1) * BN > sure[0]) clean(j);
+            for (int j = 0; j < n + LAG; ++j) {
+                if (j < n) {
+                    const int now = page;
+                    page = page_of(j + 1);
+                    if (!pt_wait_warp(empty + 8 * (j % NS), (j / NS & 1) ^ 1, abort_flag, 8)) {
+                        for (int i = max(0, j - NS); i < j; ++i) pt_poll((is_v ? v_here : k_full) + 8 * (i % NS), i / NS & 1);       // copies under way
+                        goto done;
+                    }
+                    const uint32_t bar = (is_v ? v_here : k_full) + 8 * (j % NS), dst = ring + (j % NS) * L::TILE + lane * box * 128;
+                    if (lane == 0) pt_expect(bar, L::TILE);
                     __syncwarp();
-                    if (lane == 0) pt_arrive(v_full + 8 * (u % NS));
+                    if (lane < per) {
+                        const int tok = (k0 + j * BN + lane * box) % a.page_size;
+#pragma unroll
+                        for (int h = 0; h < D / 64; ++h) pt_tma(dst + h * BN * 128, is_v ? &maps.v : &maps.k, h * 64, kvh, tok, now, bar);
+                    }
+                    __syncwarp();
+                }
+                if (is_v && j >= LAG) {
+                    const int jj = j - LAG;
+                    if (!pt_wait_warp(v_here + 8 * (jj % NS), jj / NS & 1, abort_flag, 9)) goto done;
+                    if (k0 + (jj + 1) * BN > sure[0]) clean(jj);
+                    __syncwarp();
+                    if (lane == 0) pt_arrive(v_full + 8 * (jj % NS));
                 }
             }
-        } else {
-            const char * base = (is_v ? a.v : a.k) + kvh * a.nb_head;
-            int page[G];
-            auto look = [&](int j) {
+            if (!is_v)                                                    // nothing may be under way when the CTA ends
+                for (int j = max(0, n - NS); j < n; ++j) if (!pt_wait_warp(k_full + 8 * (j % NS), j / NS & 1, abort_flag, 10)) break;
+            goto done;
+        }
+        int page[G];
+        auto look = [&](int j) {
 #pragma unroll
-                for (int q = 0; q < G; ++q) { const int key = k0 + j * BN + q * 32 + lane; page[q] = j < n && key < k1 ? table[key / a.page_size] : -1; }
-            };
-            look(0);
-            for (int j = 0; j < n; ++j, ++u) {
-                const uint32_t dst = ring + (u % NS) * L::TILE;
+            for (int g = 0; g < G; ++g) { const int key = k0 + j * BN + g * 32 + lane; page[g] = j < n && key < k1 ? table[key / a.page_size] : -1; }
+        };
+        look(0);
+        for (int j = 0; j < n + LAG; ++j) {
+            if (j < n) {
+                const uint32_t dst = ring + (j % NS) * L::TILE;
                 int64_t at[G];
 #pragma unroll
-                for (int q = 0; q < G; ++q) {
-                    const int key = k0 + j * BN + q * 32 + lane;
-                    at[q] = page[q] >= 0 && page[q] < a.n_pages ? page[q] * a.nb_page + (key % a.page_size) * a.nb_tok : -1;
-                    asm volatile("" : "+l"(at[q]));       // kept: the compiler computes it again for every chunk otherwise, division included
+                for (int g = 0; g < G; ++g) {
+                    const int key = k0 + j * BN + g * 32 + lane;
+                    at[g] = page[g] >= 0 && page[g] < a.n_pages ? page[g] * a.nb_page + (key % a.page_size) * a.nb_tok : -1;
+                    asm volatile("" : "+l"(at[g]));       // kept: computed again for every chunk otherwise, division included (30 000 cycles a block)
                 }
                 look(j + 1);
-                if (!pt_wait_warp(empty + 8 * (u % NS), (u / NS & 1) ^ 1, abort_flag, 8)) goto done;
+                if (!pt_wait_warp(empty + 8 * (j % NS), (j / NS & 1) ^ 1, abort_flag, 8)) goto done;
 #pragma unroll
-                for (int q = 0; q < G; ++q)
+                for (int g = 0; g < G; ++g)
 #pragma unroll
                     for (int c = 0; c < NC; ++c) {
                         const int i = c * 32 + lane, r = i / NC, ch = i % NC;        // row of the group, 16-byte chunk of the row
-                        const int64_t off = __shfl_sync(0xffffffffu, at[q], r);
-                        const uint32_t d = dst + (ch >> 3) * BN * 128 + (q * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                        const int64_t off = __shfl_sync(0xffffffffu, at[g], r);
+                        const uint32_t d = dst + (ch >> 3) * BN * 128 + (g * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4);
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(d), "l"(base + (off < 0 ? 0 : off + ch * 16)), "r"(off < 0 ? 0 : 16) : "memory");
                     }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                if (is_v && k0 + (j + 1) * BN > sure[0]) clean(j);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (j >= LAG) {
+                const int jj = j - LAG;
+                asm volatile("cp.async.wait_group %0;" :: "n"(LAG) : "memory");
+                if (is_v && k0 + (jj + 1) * BN > sure[0]) clean(jj);
                 pt_proxy_fence();
                 __syncwarp();
-                if (lane == 0) pt_arrive(full + 8 * (u % NS));
+                if (lane == 0) pt_arrive(full + 8 * (jj % NS));
             }
         }
-        }
-        if (box && !is_v)                                                 // nothing may be under way when the CTA ends
-            for (uint32_t i = u < NS ? 0 : u - NS; i < u; ++i) if (!pt_wait_warp(k_full + 8 * (i % NS), i / NS & 1, abort_flag, 10)) break;
     }
 done:
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -577,20 +541,21 @@ static void pt_make_maps(PtMaps & m, const PaArgs & a, int D, int BN, bool f16) 
 }
 
 template <typename T, int D, int BN, int NS, int NTILE, int MIN_CTAS>
-static cudaError_t pt_go(const PaArgs & a, int n_seq, cudaStream_t st) {
-    const int smem = PtSmem<D, BN, NS, NTILE>::BYTES;
-    const int64_t tiles = ((int64_t) a.max_new * a.group + 128 * NTILE - 1) / (128 * NTILE);
+static cudaError_t pt_go(const PaArgs & a, int64_t n_items, cudaStream_t st) {
+    static_assert(128 * NTILE == PA_TC_ROWS(D) && BN == PA_TC_KEYS(D) && MIN_CTAS == PA_TC_CTAS(D), "what the plan counts with");
     constexpr auto k = k_paged_attn_tc<T, D, BN, NS, NTILE, MIN_CTAS>;
+    constexpr int smem = PtSmem<D, BN, NS, NTILE>::BYTES;
     cudaError_t e = allow_once<k>(smem);
     if (e != cudaSuccess) return e;
     PtMaps maps;
     pt_make_maps(maps, a, D, BN, std::is_same<T, __half>::value);
-    e = launch_chained(k, a.stream ? dim3((unsigned) a.stream) : dim3((unsigned) tiles, (unsigned) a.n_head_kv, (unsigned) n_seq), dim3(PT_THREADS(NTILE)), smem, st, a, maps);
+    const int64_t ctas = a.n_whole + (n_items - a.n_whole) * a.n_split;
+    e = launch_chained(k, dim3((unsigned) ctas), dim3(PT_THREADS(NTILE)), smem, st, a, maps);
     if (e == cudaSuccess) B200_LAUNCHED();
     return e;
 }
 
-cudaError_t pa_tc_launch(const PaArgs & a, int head_dim, int type, int n_seq, cudaStream_t st) {
-    if (head_dim == 64) return type == B200_TYPE_F16 ? pt_go<__half, 64, 64, 2, 1, 4>(a, n_seq, st) : pt_go<__nv_bfloat16, 64, 64, 2, 1, 4>(a, n_seq, st);
-    return type == B200_TYPE_F16 ? pt_go<__half, 128, 128, 2, 2, 1>(a, n_seq, st) : pt_go<__nv_bfloat16, 128, 128, 2, 2, 1>(a, n_seq, st);
+cudaError_t pa_tc_launch(const PaArgs & a, int head_dim, int type, int64_t n_items, cudaStream_t st) {
+    if (head_dim == 64) return type == B200_TYPE_F16 ? pt_go<__half, 64, 64, 2, 1, 4>(a, n_items, st) : pt_go<__nv_bfloat16, 64, 64, 2, 1, 4>(a, n_items, st);
+    return type == B200_TYPE_F16 ? pt_go<__half, 128, 128, 2, 2, 1>(a, n_items, st) : pt_go<__nv_bfloat16, 128, 128, 2, 2, 1>(a, n_items, st);
 }

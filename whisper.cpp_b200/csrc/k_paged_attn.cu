@@ -176,13 +176,13 @@ __device__ __forceinline__ PaLine pa_line(const PaArgs & a, int round, int64_t t
 }
 
 
-template <typename Q, typename KV, int D>
-__global__ void __launch_bounds__(32 * PA_WARPS, PaParts<Q, KV>::n == 1 ? 3 : 2)
+template <typename Q, typename KV, int D, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, WARPS > PA_WARPS ? 1 : PaParts<Q, KV>::n == 1 ? 3 : 2)
 k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw) {
     using P = PaPack<KV>;
     constexpr int NP = PaParts<Q, KV>::n, NC = D / 8, KS = D / 16;      // parts, 16-byte chunks and MMA steps of a head
     constexpr float LIFT = PaParts<Q, KV>::lift;
-    constexpr int BLOCK = PA_BLOCK, KEYS = BLOCK / (2 * D), NK = KEYS / 8, ROUND = KEYS * PA_WARPS;      // keys of a block, MMA columns of its scores
+    constexpr int BLOCK = PA_BLOCK, KEYS = BLOCK / (2 * D), NK = KEYS / 8, ROUND = KEYS * WARPS;      // keys of a block, MMA columns of its scores
     extern __shared__ __align__(16) char smem[];
     // The successor is let in only when CTAs end: brought in early, the CTAs of the join and of the next call took the places of this kernel's
     // own (111 sequences of 4096 keys: 121 us a call, 85 without).
@@ -215,8 +215,8 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     const char * kp = a.k + kvh * a.nb_head, * vp = a.v + kvh * a.nb_head;
     const int32_t * table = a.tables + seq * a.table_stride;
     const uint32_t ring = pa_smem(smem) + warp * 4 * BLOCK;             // K0 K1 V0 V1
-    const int n_block = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0, n_mine = (n_block - warp + PA_WARPS - 1) / PA_WARPS;
-    auto key_of = [&](int i) { return k0 + (i * PA_WARPS + warp) * KEYS + lane; };
+    const int n_block = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0, n_mine = (n_block - warp + WARPS - 1) / WARPS;
+    auto key_of = [&](int i) { return k0 + (i * WARPS + warp) * KEYS + lane; };
     auto page_of = [&](int i) { const int key = key_of(i); return i < n_mine && lane < KEYS && key < k1 ? table[key / a.page_size] : -1; };
     const int new0 = nw.k ? s.len - s.n_new : 1 << 30;    // from here on K and V come from the new rows
     auto at_of = [&](int i, int page) -> int64_t {       // this lane's key's place in the pool, -1: none
@@ -229,7 +229,7 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     auto load = [&](int i, int64_t at, bool is_v, uint32_t dst) {
         if (i < n_mine) {
             const char * base = is_v ? vp : kp;
-            const int key0 = k0 + (i * PA_WARPS + warp) * KEYS;
+            const int key0 = k0 + (i * WARPS + warp) * KEYS;
             if (key0 + KEYS <= new0) {
 #pragma unroll
                 for (int c = 0; c < NC * KEYS / 32; ++c) {
@@ -319,7 +319,7 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     float o[NC][4] = {}, ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
     for (int i = 0; i < n_mine; ++i) {
         const uint32_t kb = ring + (i & 1) * BLOCK, vb = kb + 2 * BLOCK;
-        const int key0 = k0 + (i * PA_WARPS + warp) * KEYS;
+        const int key0 = k0 + (i * WARPS + warp) * KEYS;
         at_next = at_of(i + 2, page_next);
         page_next = page_of(i + 3);
         pa_wait<3>();
@@ -446,7 +446,7 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     for (int of = 1; of < 4; of <<= 1) { la += __shfl_xor_sync(0xffffffffu, la, of); lb += __shfl_xor_sync(0xffffffffu, lb, of); }
     __syncthreads();
     // join of the four warps: [warp][row] maxima and sums, [warp][row][D + 4] accumulators over the rings
-    float * sm = (float *) smem, * sl = sm + PA_WARPS * PA_ROWS, * so = sl + PA_WARPS * PA_ROWS;
+    float * sm = (float *) smem, * sl = sm + WARPS * PA_ROWS, * so = sl + WARPS * PA_ROWS;
     constexpr int LD = D + 4;
     {
         const int wa = warp * PA_ROWS + (lane >> 2), wb = wa + 8;
@@ -459,15 +459,15 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     }
     __syncthreads();
     const int rows = min(PA_ROWS, n_rows - row0);
-    for (int i = tid; i < rows * (D / 4); i += 32 * PA_WARPS) {
+    for (int i = tid; i < rows * (D / 4); i += 32 * WARPS) {
         const int r = i / (D / 4), d = i % (D / 4) * 4, row = row0 + r;
         float mx = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < PA_WARPS; ++w) mx = fmaxf(mx, sm[w * PA_ROWS + r]);
+        for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, sm[w * PA_ROWS + r]);
         const float base = mx == -INFINITY ? 0.0f : mx;
         float sum = 0.0f, x[4] = {};
 #pragma unroll
-        for (int w = 0; w < PA_WARPS; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const float f = pa_exp2(sm[w * PA_ROWS + r] - base);
             sum += f * sl[w * PA_ROWS + r];              // NaN of a warp without a finite maximum stays NaN
             if (f != 0.0f) {
@@ -686,12 +686,16 @@ static cudaError_t pa_launch(PaArgs & k, const PaNew & x, int n_seq, int64_t n_i
         if (e != cudaSuccess || k.n_split == 1) return e;
         e = launch_chained(k_paged_join_tc<Q, D>, dim3((unsigned) (n_items - k.n_whole), (unsigned) k.tile_rows / 16), dim3(128), 0, st, k);
     } else {
-        constexpr int smem = 4 * PA_WARPS * PA_BLOCK;
-        e = allow_once<k_paged_attn<Q, KV, D>>(smem);
-        if (e != cudaSuccess) return e;
         const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
         const dim3 grid = k.stream ? dim3((unsigned) k.stream) : dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) n_seq);
-        e = launch_chained(k_paged_attn<Q, KV, D>, grid, dim3(32 * PA_WARPS), smem, st, k, x);
+        // few items, one CTA per SM at most: eight warps share an item's blocks (5 beams of 20 heads, 431 keys, f32: 11.2 -> 8.8 us)
+        if (!k.stream && n_items <= 148) {
+            e = allow_once<k_paged_attn<Q, KV, D, 8>>(4 * 8 * PA_BLOCK);
+            if (e == cudaSuccess) e = launch_chained(k_paged_attn<Q, KV, D, 8>, grid, dim3(256), 4 * 8 * PA_BLOCK, st, k, x);
+        } else {
+            e = allow_once<k_paged_attn<Q, KV, D, PA_WARPS>>(4 * PA_WARPS * PA_BLOCK);
+            if (e == cudaSuccess) e = launch_chained(k_paged_attn<Q, KV, D, PA_WARPS>, grid, dim3(32 * PA_WARPS), 4 * PA_WARPS * PA_BLOCK, st, k, x);
+        }
         if (e != cudaSuccess) return e;
         B200_LAUNCHED();
         if (!k.stream) return cudaGetLastError();

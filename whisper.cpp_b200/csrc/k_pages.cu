@@ -388,7 +388,8 @@ k_pages_compact(PgState from, PgState to, int n_rows, int width, int n_pages, in
 }
 
 // ---- host ----
-// The list of copies is on the device, so its length is not known to the host: a fixed grid strides over it.
+// The list of copies is on the device, so its length is not known to the host: a grid of fixed size strides over it (18 000 pages of 64 KB:
+// 211 us with 8 CTAs per SM in the grid, 193 with 64: 6.1 TB/s).
 __global__ void __launch_bounds__(PG_COPY_THREADS)
 k_pages_copy(b200_page_pool pool, const int32_t * head, const int32_t * copies) {
     chain_release();
@@ -410,7 +411,7 @@ bool b200_pool_ok(const b200_page_pool * p, bool data) {
 static int pg_launch_copy(const b200_page_pool * pool, const PgWork & w, int64_t max_copies, cudaStream_t st) {
     const int64_t tiles = ((int64_t) pool->page_size * pool->n_head_kv * pool->head_dim / 8 + PG_COPY_THREADS * PG_COPY_UNROLL - 1) / (PG_COPY_THREADS * PG_COPY_UNROLL);
     const int64_t items = max_copies * pool->n_layer * 2 * tiles;
-    const unsigned grid = (unsigned) (items < 148 * 8 ? items : 148 * 8);
+    const unsigned grid = (unsigned) (items < 148 * 64 ? items : 148 * 64);
     const cudaError_t e = launch_chained(k_pages_copy, dim3(grid), dim3(PG_COPY_THREADS), 0, st, *pool, (const int32_t *) w.head, (const int32_t *) w.copies);
     if (e != cudaSuccess) return (int) e;
     B200_LAUNCHED();

@@ -1,22 +1,28 @@
 // Attention of many rows over a paged key/value cache on the fifth-generation tensor cores (tcgen05.mma, scores, weights and
 // accumulators in tensor memory).  Operator and row numbering as in k_paged_attn.cu; 16-bit queries only.
 //
-// A CTA takes 256 rows - two tiles of 128, so that one tile's softmax runs while the tensor core works for the other - of one
-// sequence and key/value head over one split of the keys, in blocks of BN keys:
+// A CTA takes one or two tiles of 128 rows of one sequence and key/value head over one split of the keys, in blocks of BN keys:
 //     S_t = Q_t K^T   (M 128, N BN, K head_dim)   both operands K-major in shared memory, 128-byte swizzle
 //     O_t += P_t V    (M 128, N head_dim, K BN)   P_t from tensor memory (over S_t, 16-bit), V as stored: N-major, 128-byte swizzle
-// Roles (352 threads):
-//   warps 0-3, 4-7   softmax of tile 0, 1: a thread owns a row.  It reads its scores (tcgen05.ld), masks only blocks that some row
-//                    does not see wholly, and writes the weights back as P.  The reference point of the exponentials is the running
-//                    maximum, but it follows it only when the maximum has grown by more than 2^8: the weights stay below 256, the
-//                    sums are exact in the same sense, and the rescaling of O (a read and a write of tensor memory) is rare.  All
-//                    exponentials go to the exponential unit: two to five of eight pairs as a polynomial on the FMA pipe made a chunk of
-//                    2048 over 16k keys slower (1.11 -> 1.41 .. 1.83 ms).
-//   warp 8           one thread issues all MMAs.  S_t(j+1) follows P_t V(j) in issue order, so the commit behind S_t(j+1) also says that
+// While the softmax of one tile runs the tensor core has to have other work.  head_dim 128: two tiles in a CTA of 352 threads, which fill
+// tensor memory (2 x (128 + 128) columns) and shared memory (192 KB), one CTA on an SM, BN = 128.  head_dim 64: one tile in a CTA of 224
+// threads and four CTAs on an SM, BN = 64, so that short prompts do not leave half of a CTA's rows empty.
+// Roles (NTILE tiles):
+//   4 NTILE warps    softmax: a thread owns a row.  It reads its scores (tcgen05.ld), masks only blocks that some row does not see wholly,
+//                    and writes the weights back as P.  The reference point of the exponentials is the running maximum, but it follows it
+//                    only when the maximum has grown by more than 2^8: the weights stay below 256, the sums are exact in the same sense,
+//                    and the rescaling of O (a read and a write of tensor memory) is rare.  All exponentials go to the exponential unit:
+//                    one of eight pairs as a polynomial on the FMA pipe made a chunk of 2048 over 16k keys slower (932 -> 966 us), one
+//                    of four more so (1004 us).
+//   1 warp           one thread issues all MMAs.  S_t(j+1) follows P_t V(j) in issue order, so the commit behind S_t(j+1) also says that
 //                    O_t is at rest and that P_t may be overwritten; no further barrier is needed for either.
-//   warps 9, 10      bring K and V by TMA, page by page into the swizzled tile, where pages fit into blocks or blocks into pages (page
+//   2 warps          bring K and V by TMA, page by page into the swizzled tile, where pages fit into blocks or blocks into pages (page
 //                    sizes 8, 16, 32, .. and multiples of BN); otherwise per key one page lookup and 16-byte cp.async.  Zeros for keys
 //                    out of reach and pages out of the pool.
+// Measured, head_dim 128, bf16, chunks of 2048 queries over 16k keys, 32 heads on 8: 932 us, 1.10 PFLOP/s.  What bounds it is the chain of a
+// tile: its softmax, then P V and the next Q K^T, while the other tile's softmax and products run beside it.  Tried without gain: P
+// handed over in two halves (1097 against 1037 us), two score buffers with blocks of 64 keys (1661: Q K^T with N = 64 reads Q from shared
+// memory twice as often), two threads a row (981 against 967).
 // 0 * v is not 0 where v is infinite or NaN: in blocks that are not wholly seen the V warp takes such values out of its tile and raises
 // a flag; the rows that do see them add them at the end, from the pages.
 // All waits are bounded (about a second), record a code (b200_paged_attn_status) and make every role leave through the exit that frees
@@ -165,6 +171,16 @@ template <typename T> __device__ __forceinline__ float pt_zero_times(uint4 x, fl
     return any + __uint_as_float(pt_odd<T>(z) ? 0x7fffffffu : 0u);
 }
 
+// x * 0: NaN stays of what is infinite or NaN
+template <typename T> __device__ __forceinline__ void pt_zero(uint4 & x) {
+    uint32_t * w = &x.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) { const __half2 y = __hmul2(*(const __half2 *) &w[i], __half2half2(__ushort_as_half(0))); w[i] = *(const uint32_t *) &y; }
+        else { const __nv_bfloat162 y = __hmul2(*(const __nv_bfloat162 *) &w[i], __bfloat162bfloat162(__ushort_as_bfloat16(0))); w[i] = *(const uint32_t *) &y; }
+    }
+}
+
 template <typename T, int D, int BN, int NS, int NTILE, int MIN_CTAS>
 __global__ void __launch_bounds__(PT_THREADS(NTILE), MIN_CTAS)
 k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps maps) {
@@ -227,14 +243,14 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 uint4 x = make_uint4(0, 0, 0, 0);
-                if (valid) { x = *(const uint4 *) (q + c * 16); x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip; }
+                if (valid) { x = *(const uint4 *) (q + c * 16); x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip; if (a.scale_log2 == 0) pt_zero<T>(x); }
                 *(uint4 *) (dst + (c >> 3) * 128 * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
             }
             pt_proxy_fence();
             __syncwarp();
             if (lane == 0) pt_arrive(q_full);
         }
-        const float scale = fabsf(a.scale_log2);
+        const float scale = a.scale_log2 == 0 ? 1.0f : fabsf(a.scale_log2);        // 0 is in Q: masked scores are -inf, and -inf * 0 is not
         const int last = !valid ? -1 : a.causal ? s.len - s.n_new + tok : s.len - 1;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;              // 32 lanes per warp, in bits 16 and up
         const uint32_t ts = tmem + lanes + t * BN, to = tmem + lanes + NTILE * BN + t * D;
@@ -244,67 +260,72 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             pt_after();
             const int seen = last + 1 - (k0 + j * BN);                   // this row sees the block's first `seen` keys
             const bool edge = k0 + (j + 1) * BN > sure[t];
-            constexpr bool TWICE = MIN_CTAS > 1;                          // few registers: the scores are read once for the maximum, once for the weights
-            uint32_t x[TWICE ? 32 : BN];
-            if (!TWICE) {
+            // Two copies for head_dim 128, so that blocks which every row sees wholly hold no code for masks (chunk of 2048 over 16k keys: 955 -> 932 us);
+            // one copy for head_dim 64, whose four CTAs an SM share the instruction cache (ragged prompts: 36.1 against 37.4 us with two).
+            auto block = [&](auto masked) {
+                constexpr bool MASKED = decltype(masked)::value, BOTH = NTILE == 1;
+                // 32 scores at a time, read once for the maximum and once for the weights: keeping 64, 96 or 128 of them in registers between
+                // the two was no faster (931, 944, 946 us)
+                auto scores = [&](uint32_t * y, int c) {
+                    pt_ld32(y, ts + c);
+                    pt_wait32(y);
+                    if (BOTH ? edge : MASKED) {
 #pragma unroll
-                for (int c = 0; c < BN; c += 32) pt_ld32(x + (TWICE ? 0 : c), ts + c);
-            }
-            float m4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
+                        for (int i = 0; i < 32; ++i) if (c + i >= seen) y[i] = 0xff800000u;
+                    }
+                };
+                float m4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
-            for (int c = 0; c < BN; c += 32) {
-                uint32_t * y = x + (TWICE ? 0 : c);
-                if (TWICE) pt_ld32(y, ts + c);
-                pt_wait32(y);
-                if (edge) {
+                for (int c = 0; c < BN; c += 32) {
+                    uint32_t y[32];
+                    scores(y, c);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) if (c + i >= seen) y[i] = 0xff800000u;
+                    for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], fmaxf(__uint_as_float(y[i + u]), __uint_as_float(y[i + 4 + u])));
                 }
-#pragma unroll
-                for (int i = 0; i < 32; i += 8)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], fmaxf(__uint_as_float(y[i + u]), __uint_as_float(y[i + 4 + u])));
-            }
-            float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            mx = mx == -INFINITY ? mx : mx * scale;
-            const bool grow = mx > m + 8.0f;                              // also when there was no key so far
-            if (__any_sync(0xffffffffu, grow)) {
-                const float m1 = fmaxf(m, mx), f = m1 == -INFINITY ? 1.0f : pa_exp2(m - m1);
-                m = m1;
-                l *= f;
-                if (j > 0) {
+                float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                mx = mx == -INFINITY ? mx : mx * scale;
+                const bool grow = mx > m + 8.0f;                              // also when there was no key so far
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float m1 = fmaxf(m, mx), f = m1 == -INFINITY ? 1.0f : pa_exp2(m - m1);
+                    m = m1;
+                    l *= f;
+                    if (j > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 16) {
-                        uint32_t o[16];
-                        pt_ld16(o, to + c);
-                        pt_wait16(o);
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            pt_ld16(o, to + c);
+                            pt_wait16(o);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        pt_st16(to + c, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            pt_st16(to + c, o);
+                        }
                     }
                 }
-            }
-            const float base = m == -INFINITY ? 0.0f : -m;
-            pt_f2 l2[2] = { 0ull, 0ull };
-            const pt_f2 scale2 = pt_pair(scale, scale), base2 = pt_pair(base, base);
+                const float base = m == -INFINITY ? 0.0f : -m;
+                pt_f2 l2[2] = { 0ull, 0ull };
+                const pt_f2 scale2 = pt_pair(scale, scale), base2 = pt_pair(base, base);
 #pragma unroll
-            for (int c = 0; c < BN; c += 32) {
-                uint32_t w[16], * y = x + (TWICE ? 0 : c);
-                if (TWICE) { pt_ld32(y, ts + c); pt_wait32(y); }
+                for (int c = 0; c < BN; c += 32) {
+                    uint32_t w[16], y[32];
+                    scores(y, c);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float y0, y1;
-                    pt_split(pt_fma2(pt_pair(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), scale2, base2), y0, y1);
-                    if (edge) { if (c + 2 * i >= seen) y0 = -INFINITY; if (c + 2 * i + 1 >= seen) y1 = -INFINITY; }       // -inf * 0 is not -inf
-                    y0 = pa_exp2(y0); y1 = pa_exp2(y1);
-                    l2[i & 1] = pt_add2(l2[i & 1], pt_pair(y0, y1));
-                    w[i] = pt_two<T>(y0, y1);
+                    for (int i = 0; i < 16; ++i) {
+                        float y0, y1;
+                        pt_split(pt_fma2(pt_pair(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), scale2, base2), y0, y1);
+                        y0 = pa_exp2(y0); y1 = pa_exp2(y1);
+                        l2[i & 1] = pt_add2(l2[i & 1], pt_pair(y0, y1));
+                        w[i] = pt_two<T>(y0, y1);
+                    }
+                    pt_st16(ts + c / 2, w);
                 }
-                pt_st16(ts + c / 2, w);
-            }
-            float l0, l1;
-            pt_split(pt_add2(l2[0], l2[1]), l0, l1);
-            l += l0 + l1;
+                float l0, l1;
+                pt_split(pt_add2(l2[0], l2[1]), l0, l1);
+                l += l0 + l1;
+            };
+            if (edge || NTILE == 1) block(std::true_type());
+            else block(std::false_type());
             pt_wait_st();
             pt_before();
             __syncwarp();
@@ -391,7 +412,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
         const char * base = (is_v ? a.v : a.k) + kvh * a.nb_head;
         const uint32_t ring = sb + (is_v ? L::V : L::K), full = is_v ? v_full : k_full, empty = is_v ? v_empty : k_empty;
         const int32_t * table = a.tables + seq * a.table_stride;
-        constexpr int G = BN / 32, LAG = NS - 2;
+        constexpr int G = BN / 32;
         const int box = maps.box;
         // V's non-finite values, in blocks that are not wholly seen, are taken out; a lane looks at the same 16-byte chunks that it copies
         auto clean = [&](int jj) {
@@ -433,30 +454,27 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                 return p < 0 || p > a.n_pages ? a.n_pages : p;
             };
             int page = page_of(0);
-            for (int j = 0; j < n + LAG; ++j) {
-                if (j < n) {
-                    const int now = page;
-                    page = page_of(j + 1);
-                    if (!pt_wait_warp(empty + 8 * (j % NS), (j / NS & 1) ^ 1, abort_flag, 8)) {
-                        for (int i = max(0, j - NS); i < j; ++i) pt_poll((is_v ? v_here : k_full) + 8 * (i % NS), i / NS & 1);       // copies under way
-                        goto done;
-                    }
-                    const uint32_t bar = (is_v ? v_here : k_full) + 8 * (j % NS), dst = ring + (j % NS) * L::TILE + lane * box * 128;
-                    if (lane == 0) pt_expect(bar, L::TILE);
-                    __syncwarp();
-                    if (lane < per) {
-                        const int tok = (k0 + j * BN + lane * box) % a.page_size;
-#pragma unroll
-                        for (int h = 0; h < D / 64; ++h) pt_tma(dst + h * BN * 128, is_v ? &maps.v : &maps.k, h * 64, kvh, tok, now, bar);
-                    }
-                    __syncwarp();
+            for (int j = 0; j < n; ++j) {
+                const int now = page;
+                page = page_of(j + 1);
+                if (!pt_wait_warp(empty + 8 * (j % NS), (j / NS & 1) ^ 1, abort_flag, 8)) {
+                    for (int i = max(0, j - NS); i < j; ++i) pt_poll((is_v ? v_here : k_full) + 8 * (i % NS), i / NS & 1);       // copies under way
+                    goto done;
                 }
-                if (is_v && j >= LAG) {
-                    const int jj = j - LAG;
-                    if (!pt_wait_warp(v_here + 8 * (jj % NS), jj / NS & 1, abort_flag, 9)) goto done;
-                    if (k0 + (jj + 1) * BN > sure[0]) clean(jj);
+                const uint32_t bar = (is_v ? v_here : k_full) + 8 * (j % NS), dst = ring + (j % NS) * L::TILE + lane * box * 128;
+                if (lane == 0) pt_expect(bar, L::TILE);
+                __syncwarp();
+                if (lane < per) {
+                    const int tok = (k0 + j * BN + lane * box) % a.page_size;
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h) pt_tma(dst + h * BN * 128, is_v ? &maps.v : &maps.k, h * 64, kvh, tok, now, bar);
+                }
+                __syncwarp();
+                if (is_v) {
+                    if (!pt_wait_warp(bar, j / NS & 1, abort_flag, 9)) goto done;
+                    if (k0 + (j + 1) * BN > sure[0]) clean(j);
                     __syncwarp();
-                    if (lane == 0) pt_arrive(v_full + 8 * (jj % NS));
+                    if (lane == 0) pt_arrive(v_full + 8 * (j % NS));
                 }
             }
             if (!is_v)                                                    // nothing may be under way when the CTA ends
@@ -469,37 +487,32 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             for (int g = 0; g < G; ++g) { const int key = k0 + j * BN + g * 32 + lane; page[g] = j < n && key < k1 ? table[key / a.page_size] : -1; }
         };
         look(0);
-        for (int j = 0; j < n + LAG; ++j) {
-            if (j < n) {
-                const uint32_t dst = ring + (j % NS) * L::TILE;
-                int64_t at[G];
+        for (int j = 0; j < n; ++j) {
+            const uint32_t dst = ring + (j % NS) * L::TILE;
+            int64_t at[G];
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const int key = k0 + j * BN + g * 32 + lane;
-                    at[g] = page[g] >= 0 && page[g] < a.n_pages ? page[g] * a.nb_page + (key % a.page_size) * a.nb_tok : -1;
-                    asm volatile("" : "+l"(at[g]));       // kept: computed again for every chunk otherwise, division included (30 000 cycles a block)
+            for (int g = 0; g < G; ++g) {
+                const int key = k0 + j * BN + g * 32 + lane;
+                at[g] = page[g] >= 0 && page[g] < a.n_pages ? page[g] * a.nb_page + (key % a.page_size) * a.nb_tok : -1;
+                asm volatile("" : "+l"(at[g]));       // kept: computed again for every chunk otherwise, division included (30 000 cycles a block)
+            }
+            look(j + 1);
+            if (!pt_wait_warp(empty + 8 * (j % NS), (j / NS & 1) ^ 1, abort_flag, 8)) goto done;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int i = c * 32 + lane, r = i / NC, ch = i % NC;        // row of the group, 16-byte chunk of the row
+                    const int64_t off = __shfl_sync(0xffffffffu, at[g], r);
+                    const uint32_t d = dst + (ch >> 3) * BN * 128 + (g * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(d), "l"(base + (off < 0 ? 0 : off + ch * 16)), "r"(off < 0 ? 0 : 16) : "memory");
                 }
-                look(j + 1);
-                if (!pt_wait_warp(empty + 8 * (j % NS), (j / NS & 1) ^ 1, abort_flag, 8)) goto done;
-#pragma unroll
-                for (int g = 0; g < G; ++g)
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        const int i = c * 32 + lane, r = i / NC, ch = i % NC;        // row of the group, 16-byte chunk of the row
-                        const int64_t off = __shfl_sync(0xffffffffu, at[g], r);
-                        const uint32_t d = dst + (ch >> 3) * BN * 128 + (g * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4);
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(d), "l"(base + (off < 0 ? 0 : off + ch * 16)), "r"(off < 0 ? 0 : 16) : "memory");
-                    }
-            }
             asm volatile("cp.async.commit_group;" ::: "memory");
-            if (j >= LAG) {
-                const int jj = j - LAG;
-                asm volatile("cp.async.wait_group %0;" :: "n"(LAG) : "memory");
-                if (is_v && k0 + (jj + 1) * BN > sure[0]) clean(jj);
-                pt_proxy_fence();
-                __syncwarp();
-                if (lane == 0) pt_arrive(full + 8 * (jj % NS));
-            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            if (is_v && k0 + (j + 1) * BN > sure[0]) clean(j);
+            pt_proxy_fence();
+            __syncwarp();
+            if (lane == 0) pt_arrive(full + 8 * (j % NS));
         }
     }
 done:

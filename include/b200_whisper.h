@@ -291,20 +291,21 @@ int b200_beam_reorder(const b200_beam_block * blocks, int n_blocks, const int32_
 
 /* A paged key/value cache.  The value of token t (0..page_size-1), head h, dimension i of page p in layer l lies at
  * base + l * nb_layer + p * nb_page + t * nb_tok + h * nb_head + 2 * i  (bytes; F16 or BF16; all strides and both bases
- * multiples of 16, so token-major and head-major pages are both possible).  head_dim is 64 or 128, page_size >= 1. */
+ * multiples of 16, so token-major and head-major pages are both possible).  head_dim is 64 or 128, page_size 1 .. 2^20, n_head_kv at most 1024,
+ * a page less than 32 GB. */
 typedef struct {
     void * k; void * v; int type, n_layer, n_pages, page_size, n_head_kv, head_dim;
     int64_t nb_layer, nb_page, nb_tok, nb_head;
 } b200_page_pool;
 /* Who uses the pages: row i (a sequence, or a beam of one) holds lens[i] tokens in pages tables[i * table_stride + 0 ..
  * ceil(lens[i] / page_size) - 1]; refs[p] counts the holders of page p over all rows (plus any holder of the caller's own),
- * 0 = free.  At most 8192 rows; table_stride * page_size < 2^31. */
+ * 0 = free.  At most 8192 rows; table_stride * page_size < 2^31, table_stride * n_rows < 2^30. */
 typedef struct { int32_t * tables; int32_t * lens; int32_t * refs; int64_t n_rows, table_stride; } b200_page_state;
 int64_t b200_pages_workspace(int64_t n_rows, int64_t n_pages);
 
 /* Row i becomes the first keep[i] tokens of row parent[i], with room for n_new[i] more - fork (parent != i), truncate
  * (keep < length), free (keep = n_new = 0), grow (n_new > 0), in any mix.  `from` is read, `to` (same n_rows and table_stride) is written;
- * the two must not overlap (a program keeps two states and swaps them).  Whole pages are shared.  A partly filled last page that will be written
+ * it must not overlap `from` nor the other inputs (a program keeps two states and swaps them).  Whole pages are shared.  A partly filled last page that will be written
  * (n_new > 0) stays where it is for one row only: if nobody else holds it, or, among several such rows and no other holder, for
  * the first of them; the others get a new page with a copy of its keep[i] % page_size tokens, in every layer of the pool.  New
  * pages are those free in `from`, lowest number first, row by row (within a row: first the copy, then the following pages);
@@ -339,7 +340,8 @@ int b200_pages_copy(const b200_page_pool * pool, int64_t n_rows, const void * wo
  * k_new / v_new (type of q, [n_tok][n_head_kv][head_dim] with strides nb_new_tok, nb_new_head) are first stored at their positions,
  * rounded to the pool's type; NULL (both) if the pages hold them already.  nb_* in bytes, multiples of 16, and 16-byte
  * aligned pointers.  max_new and max_len bound n_new and lens from above (device values beyond them, or beyond the tables, are cut
- * off); n_tok = q_start[n_seq].  A table entry outside the pool reads as keys and values of zero and stores nothing. */
+ * off); n_tok = q_start[n_seq].  Limits: n_seq 65535, n_head 4096, max_len 2^30 - 1, rows of a sequence (min(max_new, n_tok) * n_head / n_head_kv)
+ * below 2^30.  A table entry outside the pool reads as keys and values of zero and stores nothing. */
 typedef struct {
     const void * q; int q_type; int64_t nb_q_tok, nb_q_head;
     void * dst; int64_t nb_dst_tok, nb_dst_head;

@@ -401,6 +401,7 @@ extern "C" int b200_beam_select(const b200_beam_select_args * a, void * stream) 
     if (!size || a->nb_row % size || a->nb_row < a->n_vocab * size || a->banned_stride < 0) return B200_ERR_ARG;
     if (a->n_seq == 0) return 0;
     if (!a->logits || !a->score || !a->score_out || !a->token_out || !a->parent_out || !a->done_out || (uintptr_t) a->logits % size) return B200_ERR_ARG;
+    if (((uintptr_t) a->score | (uintptr_t) a->banned | (uintptr_t) a->score_out | (uintptr_t) a->token_out | (uintptr_t) a->parent_out) % 4) return B200_ERR_ARG;
     if (!a->workspace || (uintptr_t) a->workspace % 16 || a->workspace_bytes < b200_beam_select_workspace(a->n_seq, a->n_beam, a->n_vocab)) return B200_ERR_ARG;
     int64_t bytes;
     const SelSlices ws = sel_layout(a->workspace, rows, n_slice, a->n_beam, &bytes);
@@ -527,7 +528,7 @@ extern "C" int b200_beam_reorder(const b200_beam_block * blocks, int n_blocks, c
         ctas += tiles * s.n_outer * n_seq;
     }
     if (ctas == 0) return 0;
-    if (!parent) return B200_ERR_ARG;
+    if (!parent || (uintptr_t) parent % 4) return B200_ERR_ARG;
     auto k = n_beam <= 4 ? k_beam_reorder<4> : n_beam <= 8 ? k_beam_reorder<8> : n_beam <= 16 ? k_beam_reorder<16> : k_beam_reorder<32>;
     const cudaError_t e = launch_chained(k, dim3((unsigned) ctas), dim3(REORDER_THREADS), 0, as_stream(stream), a, parent, n_seq, n_beam);
     if (e != cudaSuccess) return (int) e;

@@ -593,16 +593,18 @@ static bool pa_args_ok(const b200_page_pool * p, const b200_paged_attn_args * a,
     if (a->n_seq < 0 || a->n_seq > 65535 || a->n_tok < 0 || a->n_tok > 0x7fffffff || a->max_new < 0 || a->max_len < 0 || a->max_len >= (1ll << 30)) return false;
     if (a->q_type != B200_TYPE_F32 && a->q_type != p->type) return false;
     if (a->n_seq == 0 || a->n_tok == 0 || a->max_new == 0) return true;
-    if (!a->tables || a->table_stride < 1 || !a->lens || !a->q_start) return false;
+    if (!a->tables || a->table_stride < 1 || !a->lens || !a->q_start || ((uintptr_t) a->tables | (uintptr_t) a->lens | (uintptr_t) a->q_start | (uintptr_t) a->lse) % 4) return false;
     if (!a->k_new != !a->v_new || (!attn && !a->k_new)) return false;
     const int64_t size = a->q_type == B200_TYPE_F32 ? 4 : 2, row = size * p->head_dim;
     if (a->k_new && (((uintptr_t) a->k_new | (uintptr_t) a->v_new | (uintptr_t) a->nb_new_tok | (uintptr_t) a->nb_new_head) % 16 ||
                      a->nb_new_tok < 0 || a->nb_new_head < 0)) return false;
     if (!attn) return true;
     if (!a->q || !a->dst || a->n_head < 1 || a->n_head % p->n_head_kv || a->n_head > 4096) return false;
+    if ((a->max_new < a->n_tok ? a->max_new : a->n_tok) * (a->n_head / p->n_head_kv) >= (1ll << 30)) return false;
     if (((uintptr_t) a->q | (uintptr_t) a->dst | (uintptr_t) a->nb_q_tok | (uintptr_t) a->nb_q_head | (uintptr_t) a->nb_dst_tok | (uintptr_t) a->nb_dst_head) % 16) return false;
     if (a->nb_q_tok < 0 || a->nb_q_head < 0 || (a->n_head > 1 && a->nb_dst_head < row) || (a->n_tok > 1 && a->nb_dst_tok < row)) return false;
-    return a->scale == a->scale && a->scale - a->scale == 0.0f;        // finite
+    const float log2 = a->scale * 1.44269504f;
+    return log2 - log2 == 0.0f;                                        // finite
 }
 
 // Which kernel, and how its work is dealt out.

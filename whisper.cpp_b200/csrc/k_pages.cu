@@ -26,7 +26,7 @@ __device__ __forceinline__ void pg_copy(const b200_page_pool & pool, int n, int6
         int src, dst, tokens;
         list(r / pool.n_layer, src, dst, tokens);
         const unsigned used = tokens * vec_tok;
-        if (src < 0 || dst < 0 || src >= pool.n_pages || dst >= pool.n_pages || used > vec_page) continue;
+        if (src < 0 || dst < 0 || src >= pool.n_pages || dst >= pool.n_pages || tokens < 0 || tokens > pool.page_size) continue;
         char * base = (char *) (kv ? pool.v : pool.k) + layer * pool.nb_layer;
         const bool flat = toks || (heads && used == vec_page);      // what is copied is one piece of memory
         uint4 v[PG_COPY_UNROLL];
@@ -391,10 +391,10 @@ k_pages_compact(PgState from, PgState to, int n_rows, int width, int n_pages, in
 // The list of copies is on the device, so its length is not known to the host: a grid of fixed size strides over it (18 000 pages of 64 KB:
 // 211 us with 8 CTAs per SM in the grid, 193 with 64: 6.1 TB/s).
 __global__ void __launch_bounds__(PG_COPY_THREADS)
-k_pages_copy(b200_page_pool pool, const int32_t * head, const int32_t * copies) {
+k_pages_copy(b200_page_pool pool, const int32_t * head, const int32_t * copies, int most) {
     chain_release();
     chain_wait();
-    pg_copy(pool, head[0], blockIdx.x, gridDim.x, [&](int64_t c, int & src, int & dst, int & tokens) { src = copies[3 * c]; dst = copies[3 * c + 1]; tokens = copies[3 * c + 2]; });
+    pg_copy(pool, min(max(head[0], 0), most), blockIdx.x, gridDim.x, [&](int64_t c, int & src, int & dst, int & tokens) { src = copies[3 * c]; dst = copies[3 * c + 1]; tokens = copies[3 * c + 2]; });
 }
 
 bool b200_pool_ok(const b200_page_pool * p, bool data) {
@@ -402,6 +402,7 @@ bool b200_pool_ok(const b200_page_pool * p, bool data) {
     if (!data) return true;
     if (!p->k || !p->v || (p->type != B200_TYPE_F16 && p->type != B200_TYPE_BF16) || (p->head_dim != 64 && p->head_dim != 128)) return false;
     if (p->n_layer < 1 || p->n_head_kv < 1 || p->n_head_kv > 1024) return false;
+    if ((int64_t) p->page_size * p->n_head_kv * (p->head_dim / 8) > 0x7fffffff) return false;          // 16-byte vectors of a page
     const int64_t row = 2 * p->head_dim;
     const int64_t bits = (int64_t) (uintptr_t) p->k | (int64_t) (uintptr_t) p->v | p->nb_page | p->nb_tok | p->nb_head | (p->n_layer > 1 ? p->nb_layer : 0);
     if (bits % 16 || (p->n_head_kv > 1 && p->nb_head < row) || (p->page_size > 1 && p->nb_tok < row) || p->nb_page < row || p->nb_head < 0 || p->nb_tok < 0) return false;
@@ -412,7 +413,7 @@ static int pg_launch_copy(const b200_page_pool * pool, const PgWork & w, int64_t
     const int64_t tiles = ((int64_t) pool->page_size * pool->n_head_kv * pool->head_dim / 8 + PG_COPY_THREADS * PG_COPY_UNROLL - 1) / (PG_COPY_THREADS * PG_COPY_UNROLL);
     const int64_t items = max_copies * pool->n_layer * 2 * tiles;
     const unsigned grid = (unsigned) (items < 148 * 64 ? items : 148 * 64);
-    const cudaError_t e = launch_chained(k_pages_copy, dim3(grid), dim3(PG_COPY_THREADS), 0, st, *pool, (const int32_t *) w.head, (const int32_t *) w.copies);
+    const cudaError_t e = launch_chained(k_pages_copy, dim3(grid), dim3(PG_COPY_THREADS), 0, st, *pool, (const int32_t *) w.head, (const int32_t *) w.copies, (int) max_copies);
     if (e != cudaSuccess) return (int) e;
     B200_LAUNCHED();
     return 0;
@@ -451,6 +452,7 @@ static bool pg_states_ok(const b200_page_state * from, const b200_page_state * t
     if (from->n_rows == 0) return from->refs && to->refs && from->refs != to->refs;
     if (from->table_stride < 1 || to->table_stride != from->table_stride || !from->tables || !to->tables || !from->lens || !to->lens || !from->refs || !to->refs) return false;
     const int64_t width = from->table_stride;
+    if (((uintptr_t) from->tables | (uintptr_t) from->lens | (uintptr_t) from->refs | (uintptr_t) to->tables | (uintptr_t) to->lens | (uintptr_t) to->refs) % 4) return false;
     if (width >= (1ll << 30)) return false;
     if (width * from->n_rows >= (1ll << 30) || width * ps >= (1ll << 31)) return false;
     auto apart = [](const void * a, int64_t na, const void * b, int64_t nb) { return (const char *) a + na <= (const char *) b || (const char *) b + nb <= (const char *) a; };
@@ -468,7 +470,7 @@ extern "C" int b200_pages_update(const b200_page_pool * pool, const b200_page_st
                                  const int32_t * keep, const int32_t * n_new, int32_t * status, void * workspace, int64_t workspace_bytes, void * stream) {
     const bool data = pool && (pool->k || pool->v);
     if (!b200_pool_ok(pool, data) || !pg_states_ok(from, to, pool->n_pages, pool->page_size) || !status) return B200_ERR_ARG;
-    if (from->n_rows && (!keep || !n_new)) return B200_ERR_ARG;
+    if ((from->n_rows && (!keep || !n_new)) || ((uintptr_t) parent | (uintptr_t) keep | (uintptr_t) n_new | (uintptr_t) status) % 4) return B200_ERR_ARG;
     if (!workspace || (uintptr_t) workspace % 16 || workspace_bytes < b200_pages_workspace(from->n_rows, pool->n_pages)) return B200_ERR_ARG;
     PgWork w;
     pg_layout(&w, workspace, from->n_rows, pool->n_pages);
@@ -486,7 +488,7 @@ extern "C" int b200_pages_update(const b200_page_pool * pool, const b200_page_st
 extern "C" int b200_pages_compact(const b200_page_pool * pool, const b200_page_state * from, const b200_page_state * to, int32_t * remap,
                                   int32_t * status, void * workspace, int64_t workspace_bytes, void * stream) {
     const bool data = pool && (pool->k || pool->v);
-    if (!b200_pool_ok(pool, data) || !pg_states_ok(from, to, pool->n_pages, pool->page_size) || !remap || !status) return B200_ERR_ARG;
+    if (!b200_pool_ok(pool, data) || !pg_states_ok(from, to, pool->n_pages, pool->page_size) || !remap || !status || ((uintptr_t) remap | (uintptr_t) status) % 4) return B200_ERR_ARG;
     if (!workspace || (uintptr_t) workspace % 16 || workspace_bytes < b200_pages_workspace(from->n_rows, pool->n_pages)) return B200_ERR_ARG;
     PgWork w;
     pg_layout(&w, workspace, from->n_rows, pool->n_pages);

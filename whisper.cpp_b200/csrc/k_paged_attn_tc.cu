@@ -19,7 +19,7 @@
 //   2 warps          bring K and V by TMA, page by page into the swizzled tile, where pages fit into blocks or blocks into pages (page
 //                    sizes 8, 16, 32, .. and multiples of BN); otherwise per key one page lookup and 16-byte cp.async.  Zeros for keys
 //                    out of reach and pages out of the pool.
-// Measured, head_dim 128, bf16, chunks of 2048 queries over 16k keys, 32 heads on 8: 932 us, 1.10 PFLOP/s.  What bounds it is the chain of a
+// Measured, head_dim 128, bf16, chunks of 2048 queries over 16k keys, 32 heads on 8: 949 us, 1.08 PFLOP/s.  What bounds it is the chain of a
 // tile: its softmax, then P V and the next Q K^T, while the other tile's softmax and products run beside it.  Tried without gain: P
 // handed over in two halves (1097 against 1037 us), two score buffers with blocks of 64 keys (1661: Q K^T with N = 64 reads Q from shared
 // memory twice as often), two threads a row (981 against 967).
@@ -157,7 +157,7 @@ __device__ __forceinline__ void pt_expect(uint32_t bar, uint32_t bytes) {
 typedef unsigned long long pt_f2;                         // two floats for the packed instructions
 __device__ __forceinline__ pt_f2 pt_pair(float a, float b) { pt_f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ void pt_split(pt_f2 v, float & a, float & b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ pt_f2 pt_fma2(pt_f2 a, pt_f2 b, pt_f2 c) { pt_f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ pt_f2 pt_mul2(pt_f2 a, pt_f2 b) { pt_f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ pt_f2 pt_add2(pt_f2 a, pt_f2 b) { pt_f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 // any + 0 * every value of x
 template <typename T> __device__ __forceinline__ float pt_zero_times(uint4 x, float any) {
@@ -260,16 +260,15 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             pt_after();
             const int seen = last + 1 - (k0 + j * BN);                   // this row sees the block's first `seen` keys
             const bool edge = k0 + (j + 1) * BN > sure[t];
-            // Two copies for head_dim 128, so that blocks which every row sees wholly hold no code for masks (chunk of 2048 over 16k keys: 955 -> 932 us);
-            // one copy for head_dim 64, whose four CTAs an SM share the instruction cache (ragged prompts: 36.1 against 37.4 us with two).
+            // Two copies for head_dim 128, so that blocks which every row sees wholly hold no code for masks (chunk of 2048 over 16k keys, with the weights of
+            // the time: 955 -> 932 us); one for head_dim 64, whose four CTAs an SM share the instruction cache (ragged prompts: 36.1 against 37.4 us with two).
             auto block = [&](auto masked) {
-                constexpr bool MASKED = decltype(masked)::value, BOTH = NTILE == 1;
                 // 32 scores at a time, read once for the maximum and once for the weights: keeping 64, 96 or 128 of them in registers between
-                // the two was no faster (931, 944, 946 us)
+                // the two was no faster
                 auto scores = [&](uint32_t * y, int c) {
                     pt_ld32(y, ts + c);
                     pt_wait32(y);
-                    if (BOTH ? edge : MASKED) {
+                    if (decltype(masked)::value && (NTILE > 1 || edge)) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) if (c + i >= seen) y[i] = 0xff800000u;
                     }
@@ -284,11 +283,10 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
 #pragma unroll
                         for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], fmaxf(__uint_as_float(y[i + u]), __uint_as_float(y[i + 4 + u])));
                 }
-                float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                mx = mx == -INFINITY ? mx : mx * scale;
-                const bool grow = mx > m + 8.0f;                              // also when there was no key so far
+                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                const bool grow = (mx - m) * scale > 8.0f;                // also when there was no key so far; -inf - -inf is not
                 if (__any_sync(0xffffffffu, grow)) {
-                    const float m1 = fmaxf(m, mx), f = m1 == -INFINITY ? 1.0f : pa_exp2(m - m1);
+                    const float m1 = fmaxf(m, mx), f = m1 == -INFINITY ? 1.0f : pa_exp2((m - m1) * scale);
                     m = m1;
                     l *= f;
                     if (j > 0) {
@@ -303,9 +301,11 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                         }
                     }
                 }
+                // difference first: exact where it matters, whatever the scores' size.  s * scale - m in one operation is 1.6% faster, but off by
+                // the rounding of m, which is a large number where the scores are (1e36: infinite weights)
                 const float base = m == -INFINITY ? 0.0f : -m;
-                pt_f2 l2[2] = { 0ull, 0ull };
                 const pt_f2 scale2 = pt_pair(scale, scale), base2 = pt_pair(base, base);
+                pt_f2 l2[2] = { 0ull, 0ull };
 #pragma unroll
                 for (int c = 0; c < BN; c += 32) {
                     uint32_t w[16], y[32];
@@ -313,7 +313,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float y0, y1;
-                        pt_split(pt_fma2(pt_pair(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), scale2, base2), y0, y1);
+                        pt_split(pt_mul2(pt_add2(pt_pair(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), base2), scale2), y0, y1);
                         y0 = pa_exp2(y0); y1 = pa_exp2(y1);
                         l2[i & 1] = pt_add2(l2[i & 1], pt_pair(y0, y1));
                         w[i] = pt_two<T>(y0, y1);
@@ -335,6 +335,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             if (!pt_wait_warp(o_full + 8 * t, 0, abort_flag, 2)) goto done;
             pt_after();
         }
+        m *= scale;                                                       // of the scores so far; from here on an exponent of two
         const int64_t out = (s.tok0 + tok) * a.n_head + head;
         const bool odd = n_blk[t] > 0 && *odd_flag;
         const bool whole = item.split < 0;

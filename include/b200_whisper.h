@@ -337,6 +337,7 @@ int b200_pages_copy(const b200_page_pool * pool, int64_t n_rows, const void * wo
  * Scores and sums are 32-bit; for 16-bit q the weights w_j are rounded to the pool's type before the product with V, which
  * adds at most half a step of that type relative to each weight, the size of the output's own rounding.  For F32 q nothing is rounded to fewer bits.  A query
  * without a key gives zeros and lse -inf; a NaN or infinite value in a position that a query does not attend to has no effect on it.
+ * A NaN or infinite value in one that it does attend to leaves the dimensions that it enters infinite or NaN.
  * k_new / v_new (type of q, [n_tok][n_head_kv][head_dim] with strides nb_new_tok, nb_new_head) are first stored at their positions,
  * rounded to the pool's type; NULL (both) if the pages hold them already.  nb_* in bytes, multiples of 16, and 16-byte
  * aligned pointers.  max_new and max_len bound n_new and lens from above (device values beyond them, or beyond the tables, are cut

@@ -292,6 +292,40 @@ def test_select_many_candidates(K, pkg, n_seq, n_beam, V, ties):
             picked.add((b, t))
 
 
+WIDE = [([(300, 700)] * 3 + [(0, 5), (129, 129), (65, 64), (1, 40)], 12, 1, 64, 16), ([(80, 300), (0, 0), (257, 270)], 8, 6, 128, 24), ([(100, 90)] * 8, 20, 1, 64, 7)]
+
+
+@pytest.mark.parametrize("shape", range(len(WIDE)))
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("kw", [dict(), dict(causal=0, layout="head"), dict(n_layer=2, layer=1, pad_q=1, lse=False, extra_new=50, extra_len=99)])
+def test_attention_of_many_f32_rows(K, pkg, shape, t, kw):
+    """Enough rows for CTAs of 128 of them."""
+    seqs, Hkv, g, D, ps = WIDE[shape]
+    rows = max(n for n, _ in seqs) * g
+    assert rows > 64 and -(-rows // 16) * Hkv * len(seqs) >= 6 * 148
+    x = Attn(K, pkg, np.random.default_rng(60 + shape), seqs, Hkv, g, D, t, "f32", ps, **kw)
+    pool = x.want_pool(x.c.view)
+    x.run()
+    x.check(pool)
+
+
+def test_many_f32_rows_do_not_see_what_comes_later(K, pkg):
+    """NaN and infinities in later tokens of the chunk reach only the queries from there on."""
+    def make():
+        return Attn(K, pkg, np.random.default_rng(2), [(200, 230)] * 4, 20, 1, 64, "f16", "f32", 16)
+    x, y = make(), make()
+    x.kn[100, 0], x.vn[100, 1, 3], x.vn[101, 2, 5] = float("nan"), float("inf"), float("nan")
+    x.run()
+    y.run()
+    torch.cuda.synchronize()
+    assert torch.equal(x.out[:100], y.out[:100]) and torch.equal(x.out[200:], y.out[200:]) and torch.equal(x.lse[:100], y.lse[:100])
+    # (a weight is a sum of parts, the later ones of either sign or zero: its product with an infinite value is infinite or NaN)
+    assert x.out[100:200, 0].isnan().all() and not x.out[100:200, 1, 3].isfinite().any() and x.out[101:200, 2, 5].isnan().all()
+    rest = [i for i in range(64) if i != 5]
+    assert torch.equal(x.out[100:200, 2][..., rest], y.out[100:200, 2][..., rest]) and torch.equal(x.out[100, 2], y.out[100, 2])
+    assert torch.equal(x.out[:, 3:], y.out[:, 3:])
+
+
 def test_no_wait_ran_out(K, pkg):
     """After everything above (this process' launches so far)."""
     x = Attn(K, pkg, np.random.default_rng(0), [(300, 400)], 1, 1, 128, "f16", "f16", 16)

@@ -84,6 +84,8 @@ k_paged_store(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew x,
 #define PA_WARPS 4
 #define PA_MIN_ROUNDS 8
 #define PA_TC_MIN_ROWS 64
+#define PA_WIDE_MIN_ROWS 64                      // f32 queries: with more rows a head, and this many tiles of 16 rows, k_paged_attn_wide
+#define PA_WIDE_MIN_ITEMS (6 * 148)
 
 template <typename T> struct PaPack;
 template <> struct PaPack<__half> {
@@ -134,6 +136,188 @@ __device__ __forceinline__ void pa_ldm_t(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3},[%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 
+// 16 rows of a warp and one block of keys after another.  Of the rows a lane has two: lane / 4 and lane / 4 + 8
+template <typename Q, typename KV, int D> struct PaTile {
+    using P = PaPack<KV>;
+    static constexpr int NP = PaParts<Q, KV>::n, NC = D / 8, KS = D / 16, KEYS = PA_BLOCK / (2 * D), NK = KEYS / 8;      // parts, 16-byte chunks and MMA steps of a head; keys of a block, MMA columns of its scores
+    static constexpr float LIFT = PaParts<Q, KV>::lift;
+    uint32_t qf[NP][KS][4], pf[NP][NK / 2][4];
+    float fa, fb, o[NC][4], sc[NK][4], ma, mb, la, lb;
+    int last_a, last_b, first_last;                       // keys up to last_*: seen by the row; up to first_last: by every row
+
+    __device__ __forceinline__ void start(const PaArgs & a, const PaSeq & s, int kvh, int row0, int n_rows) {
+        const int lane = threadIdx.x & 31;
+        const int ra = row0 + (lane >> 2), rb = ra + 8;
+        last_a = ra >= n_rows ? -1 : a.causal ? s.len - s.n_new + ra / a.group : s.len - 1;
+        last_b = rb >= n_rows ? -1 : a.causal ? s.len - s.n_new + rb / a.group : s.len - 1;
+        first_last = a.causal ? s.len - s.n_new + row0 / a.group : s.len - 1;
+        fa = fb = a.scale_log2;
+        ma = mb = -INFINITY; la = lb = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.0f;
+        {
+            const int ia = min(ra, n_rows - 1), ib = min(rb, n_rows - 1);
+            const Q * qa = (const Q *) (a.q + (s.tok0 + ia / a.group) * a.nb_q_tok + (kvh * a.group + ia % a.group) * a.nb_q_head) + (lane & 3) * 2;
+            const Q * qb = (const Q *) (a.q + (s.tok0 + ib / a.group) * a.nb_q_tok + (kvh * a.group + ib % a.group) * a.nb_q_head) + (lane & 3) * 2;
+            if constexpr (NP == 1) {
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    qf[0][i][0] = *(const uint32_t *) (qa + 16 * i);     qf[0][i][1] = *(const uint32_t *) (qb + 16 * i);
+                    qf[0][i][2] = *(const uint32_t *) (qa + 16 * i + 8); qf[0][i][3] = *(const uint32_t *) (qb + 16 * i + 8);
+                }
+            } else {
+                float2 x[KS][4];
+                float xa = 0.0f, xb = 0.0f;
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    x[i][0] = *(const float2 *) (qa + 16 * i);     x[i][1] = *(const float2 *) (qb + 16 * i);
+                    x[i][2] = *(const float2 *) (qa + 16 * i + 8); x[i][3] = *(const float2 *) (qb + 16 * i + 8);
+                    xa = fmaxf(fmaxf(xa, fmaxf(fabsf(x[i][0].x), fabsf(x[i][0].y))), fmaxf(fabsf(x[i][2].x), fabsf(x[i][2].y)));
+                    xb = fmaxf(fmaxf(xb, fmaxf(fabsf(x[i][1].x), fabsf(x[i][1].y))), fmaxf(fabsf(x[i][3].x), fabsf(x[i][3].y)));
+                }
+                float sa = 1.0f, sb = 1.0f;
+                if constexpr (LIFT != 1.0f) {                // powers of two that bring the row's largest value to [1, 2)
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1) { xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, o)); xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, o)); }
+                    auto inverse = [](float m) { const int e = (int) (__float_as_uint(m) >> 23); return e == 0 || e == 255 ? 1.0f : __uint_as_float((uint32_t) max(1, 254 - e) << 23); };
+                    sa = inverse(xa); sb = inverse(xb);
+                    fa = a.scale_log2 / sa; fb = a.scale_log2 / sb;
+                }
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float f = j & 1 ? sb : sa;
+                        uint32_t w[NP];
+                        pa_parts<Q, KV>(x[i][j].x * f, x[i][j].y * f, w);
+#pragma unroll
+                        for (int n = 0; n < NP; ++n) qf[n][i][j] = w[n];
+                    }
+            }
+        }
+    }
+    // of the block at kb
+    __device__ __forceinline__ void scores(uint32_t kb) {
+        const int lane = threadIdx.x & 31;
+        float part[NP][NK][4] = {};
+#pragma unroll
+        for (int h = 0; h < KS / 2; ++h) {
+            uint32_t b[NK][4];
+#pragma unroll
+            for (int j = 0; j < NK; ++j) pa_ldm(b[j], kb + (8 * j + (lane & 7)) * D * 2 + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NP; ++n)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < NK; ++j) P::mma(part[n][j], qf[n][2 * h + u], b[j][2 * u], b[j][2 * u + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float v = part[NP - 1][j][e];
+#pragma unroll
+                for (int n = NP - 2; n >= 0; --n) v = part[n][j][e] + v * (1.0f / LIFT);
+                sc[j][e] = v;
+            }
+    }
+    // masks (edge: some row does not see the whole block), running maximum and sum, weights in parts, o to the new maximum
+    __device__ __forceinline__ void weights(int key0, int k1, bool edge) {
+        const int lane = threadIdx.x & 31;
+        float xa = -INFINITY, xb = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                sc[j][e] *= fa; sc[j][e + 2] *= fb;
+                if (edge) {
+                    const int key = key0 + 8 * j + (lane & 3) * 2 + e;
+                    if (key >= k1 || key > last_a) sc[j][e] = -INFINITY;
+                    if (key >= k1 || key > last_b) sc[j][e + 2] = -INFINITY;
+                }
+                xa = fmaxf(xa, sc[j][e]); xb = fmaxf(xb, sc[j][e + 2]);
+            }
+#pragma unroll
+        for (int of = 1; of < 4; of <<= 1) { xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, of)); xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, of)); }
+        xa = fmaxf(xa, ma); xb = fmaxf(xb, mb);
+        const float ba = xa == -INFINITY ? 0.0f : xa, bb = xb == -INFINITY ? 0.0f : xb;
+        const float ca = pa_exp2(ma - ba), cb = pa_exp2(mb - bb);
+        ma = xa; mb = xb;
+        la *= ca; lb *= cb;
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                sc[j][e] = pa_exp2(sc[j][e] - ba); sc[j][e + 2] = pa_exp2(sc[j][e + 2] - bb);
+                la += sc[j][e]; lb += sc[j][e + 2];
+            }
+            uint32_t w[NP];
+            pa_parts<Q, KV>(sc[j][0], sc[j][1], w);
+#pragma unroll
+            for (int n = 0; n < NP; ++n) pf[n][j >> 1][(j & 1) * 2] = w[n];
+            pa_parts<Q, KV>(sc[j][2], sc[j][3], w);
+#pragma unroll
+            for (int n = 0; n < NP; ++n) pf[n][j >> 1][(j & 1) * 2 + 1] = w[n];
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) { o[c][0] *= ca; o[c][1] *= ca; o[c][2] *= cb; o[c][3] *= cb; }
+    }
+    // o += weights * the block at vb
+    __device__ __forceinline__ void values(const char * smem, uint32_t vb, int key0, int k1, bool edge) {
+        const int lane = threadIdx.x & 31;
+        uint32_t odd = 0;
+#pragma unroll
+        for (int c = 0; c < NC / 2; ++c) {
+            float part[NP][2][4] = {};
+#pragma unroll
+            for (int h = 0; h < NK / 2; ++h) {
+                uint32_t b[4];
+                pa_ldm_t(b, vb + (16 * h + (lane & 15)) * D * 2 + (((2 * c + (lane >> 4)) ^ (lane & 7)) << 4));
+                if (edge) {                               // 0 * v is not 0 where v is infinite or NaN: such values are taken out here
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) { const uint32_t x = P::odd(b[w]); odd |= x; b[w] &= ~x; }
+                }
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    if constexpr (NP == 1) { P::mma(o[2 * c], pf[0][h], b[0], b[1]); P::mma(o[2 * c + 1], pf[0][h], b[2], b[3]); }
+                    else { P::mma(part[n][0], pf[n][h], b[0], b[1]); P::mma(part[n][1], pf[n][h], b[2], b[3]); }
+                }
+            }
+            if constexpr (NP > 1) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float v = part[NP - 1][u][e];
+#pragma unroll
+                        for (int n = NP - 2; n >= 0; --n) v = part[n][u][e] + v * (1.0f / LIFT);
+                        o[2 * c + u][e] += v;
+                    }
+            }
+        }
+        if (edge && __any_sync(0xffffffffu, odd)) {       // ... and given back to the rows that see them
+            for (int j = 0; j < min(KEYS, k1 - key0); ++j)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const KV * v = (const KV *) (smem + (vb - pa_smem(smem)) + j * D * 2 + ((c ^ (j & 7)) << 4)) + (lane & 3) * 2;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float x = (float) v[e];
+                        if (!(fabsf(x) < INFINITY)) {
+                            if (key0 + j <= last_a) o[c][e] += x;
+                            if (key0 + j <= last_b) o[c][e + 2] += x;
+                        }
+                    }
+                }
+        }
+    }
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int of = 1; of < 4; of <<= 1) { la += __shfl_xor_sync(0xffffffffu, la, of); lb += __shfl_xor_sync(0xffffffffu, lb, of); }
+    }
+};
+
 // How the work is dealt out.  Items are (sequence, key/value head, tile of 16 rows), numbered in that order; an item of a sequence of n keys
 // is ceil(n / round) rounds of PA_WARPS blocks, at least one.  Either a CTA takes one item (a.stream = 0), or the rounds of all items are one
 // line that is cut into a.stream equal parts, one per CTA: whatever the lengths, all CTAs end together.  On the line an item begins with
@@ -180,9 +364,7 @@ template <typename Q, typename KV, int D, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, WARPS > PA_WARPS ? 1 : PaParts<Q, KV>::n == 1 ? 3 : 2)
 k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw) {
     using P = PaPack<KV>;
-    constexpr int NP = PaParts<Q, KV>::n, NC = D / 8, KS = D / 16;      // parts, 16-byte chunks and MMA steps of a head
-    constexpr float LIFT = PaParts<Q, KV>::lift;
-    constexpr int BLOCK = PA_BLOCK, KEYS = BLOCK / (2 * D), NK = KEYS / 8, ROUND = KEYS * WARPS;      // keys of a block, MMA columns of its scores
+    constexpr int NP = PaParts<Q, KV>::n, NC = D / 8, BLOCK = PA_BLOCK, KEYS = PaTile<Q, KV, D>::KEYS, ROUND = KEYS * WARPS;
     extern __shared__ __align__(16) char smem[];
     // The successor is let in only when CTAs end: brought in early, the CTAs of the join and of the next call took the places of this kernel's
     // own (111 sequences of 4096 keys: 121 us a call, 85 without).
@@ -268,55 +450,8 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     }
     int page_next = page_of(2);
 
-    // this lane's two rows: lane / 4 and lane / 4 + 8 of the tile
-    const int ra = row0 + (lane >> 2), rb = ra + 8;
-    const int last_a = ra >= n_rows ? -1 : a.causal ? s.len - s.n_new + ra / a.group : s.len - 1;
-    const int last_b = rb >= n_rows ? -1 : a.causal ? s.len - s.n_new + rb / a.group : s.len - 1;
-    const int first_last = a.causal ? s.len - s.n_new + row0 / a.group : s.len - 1;     // keys up to here: seen by every row
-    uint32_t qf[NP][KS][4];
-    float fa = a.scale_log2, fb = a.scale_log2;
-    {
-        const int ia = min(ra, n_rows - 1), ib = min(rb, n_rows - 1);
-        const Q * qa = (const Q *) (a.q + (s.tok0 + ia / a.group) * a.nb_q_tok + (kvh * a.group + ia % a.group) * a.nb_q_head) + (lane & 3) * 2;
-        const Q * qb = (const Q *) (a.q + (s.tok0 + ib / a.group) * a.nb_q_tok + (kvh * a.group + ib % a.group) * a.nb_q_head) + (lane & 3) * 2;
-        if constexpr (NP == 1) {
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                qf[0][i][0] = *(const uint32_t *) (qa + 16 * i);     qf[0][i][1] = *(const uint32_t *) (qb + 16 * i);
-                qf[0][i][2] = *(const uint32_t *) (qa + 16 * i + 8); qf[0][i][3] = *(const uint32_t *) (qb + 16 * i + 8);
-            }
-        } else {
-            float2 x[KS][4];
-            float ma = 0.0f, mb = 0.0f;
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                x[i][0] = *(const float2 *) (qa + 16 * i);     x[i][1] = *(const float2 *) (qb + 16 * i);
-                x[i][2] = *(const float2 *) (qa + 16 * i + 8); x[i][3] = *(const float2 *) (qb + 16 * i + 8);
-                ma = fmaxf(fmaxf(ma, fmaxf(fabsf(x[i][0].x), fabsf(x[i][0].y))), fmaxf(fabsf(x[i][2].x), fabsf(x[i][2].y)));
-                mb = fmaxf(fmaxf(mb, fmaxf(fabsf(x[i][1].x), fabsf(x[i][1].y))), fmaxf(fabsf(x[i][3].x), fabsf(x[i][3].y)));
-            }
-            float sa = 1.0f, sb = 1.0f;
-            if constexpr (LIFT != 1.0f) {                // powers of two that bring the row's largest value to [1, 2)
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) { ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, o)); mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o)); }
-                auto inverse = [](float m) { const int e = (int) (__float_as_uint(m) >> 23); return e == 0 || e == 255 ? 1.0f : __uint_as_float((uint32_t) max(1, 254 - e) << 23); };
-                sa = inverse(ma); sb = inverse(mb);
-                fa = a.scale_log2 / sa; fb = a.scale_log2 / sb;
-            }
-#pragma unroll
-            for (int i = 0; i < KS; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float f = j & 1 ? sb : sa;
-                    uint32_t w[NP];
-                    pa_parts<Q, KV>(x[i][j].x * f, x[i][j].y * f, w);
-#pragma unroll
-                    for (int n = 0; n < NP; ++n) qf[n][i][j] = w[n];
-                }
-        }
-    }
-
-    float o[NC][4] = {}, ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
+    PaTile<Q, KV, D> t;
+    t.start(a, s, kvh, row0, n_rows);
     for (int i = 0; i < n_mine; ++i) {
         const uint32_t kb = ring + (i & 1) * BLOCK, vb = kb + 2 * BLOCK;
         const int key0 = k0 + (i * WARPS + warp) * KEYS;
@@ -324,137 +459,30 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
         page_next = page_of(i + 3);
         pa_wait<3>();
         __syncwarp();
-        // scores of 16 rows and the block's keys
-        float sc[NK][4];
-        {
-            float part[NP][NK][4] = {};
-#pragma unroll
-            for (int h = 0; h < KS / 2; ++h) {
-                uint32_t b[NK][4];
-#pragma unroll
-                for (int j = 0; j < NK; ++j) pa_ldm(b[j], kb + (8 * j + (lane & 7)) * D * 2 + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4));
-#pragma unroll
-                for (int n = 0; n < NP; ++n)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int j = 0; j < NK; ++j) P::mma(part[n][j], qf[n][2 * h + u], b[j][2 * u], b[j][2 * u + 1]);
-            }
-#pragma unroll
-            for (int j = 0; j < NK; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = part[NP - 1][j][e];
-#pragma unroll
-                    for (int n = NP - 2; n >= 0; --n) v = part[n][j][e] + v * (1.0f / LIFT);
-                    sc[j][e] = v;
-                }
-        }
+        t.scores(kb);
         __syncwarp();
         load(i + 2, at_next, false, kb);
-        const bool edge = key0 + KEYS - 1 > first_last || key0 + KEYS > k1;
-        float xa = -INFINITY, xb = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < NK; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                sc[j][e] *= fa; sc[j][e + 2] *= fb;
-                if (edge) {
-                    const int key = key0 + 8 * j + (lane & 3) * 2 + e;
-                    if (key >= k1 || key > last_a) sc[j][e] = -INFINITY;
-                    if (key >= k1 || key > last_b) sc[j][e + 2] = -INFINITY;
-                }
-                xa = fmaxf(xa, sc[j][e]); xb = fmaxf(xb, sc[j][e + 2]);
-            }
-#pragma unroll
-        for (int of = 1; of < 4; of <<= 1) { xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, of)); xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, of)); }
-        xa = fmaxf(xa, ma); xb = fmaxf(xb, mb);
-        const float ba = xa == -INFINITY ? 0.0f : xa, bb = xb == -INFINITY ? 0.0f : xb;
-        const float ca = pa_exp2(ma - ba), cb = pa_exp2(mb - bb);
-        ma = xa; mb = xb;
-        la *= ca; lb *= cb;
-        uint32_t pf[NP][NK / 2][4];
-#pragma unroll
-        for (int j = 0; j < NK; ++j) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                sc[j][e] = pa_exp2(sc[j][e] - ba); sc[j][e + 2] = pa_exp2(sc[j][e + 2] - bb);
-                la += sc[j][e]; lb += sc[j][e + 2];
-            }
-            uint32_t w[NP];
-            pa_parts<Q, KV>(sc[j][0], sc[j][1], w);
-#pragma unroll
-            for (int n = 0; n < NP; ++n) pf[n][j >> 1][(j & 1) * 2] = w[n];
-            pa_parts<Q, KV>(sc[j][2], sc[j][3], w);
-#pragma unroll
-            for (int n = 0; n < NP; ++n) pf[n][j >> 1][(j & 1) * 2 + 1] = w[n];
-        }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) { o[c][0] *= ca; o[c][1] *= ca; o[c][2] *= cb; o[c][3] *= cb; }
+        const bool edge = key0 + KEYS - 1 > t.first_last || key0 + KEYS > k1;
+        t.weights(key0, k1, edge);
         pa_wait<3>();
         __syncwarp();
-        uint32_t odd = 0;
-#pragma unroll
-        for (int c = 0; c < NC / 2; ++c) {
-            float part[NP][2][4] = {};
-#pragma unroll
-            for (int h = 0; h < NK / 2; ++h) {
-                uint32_t b[4];
-                pa_ldm_t(b, vb + (16 * h + (lane & 15)) * D * 2 + (((2 * c + (lane >> 4)) ^ (lane & 7)) << 4));
-                if (edge) {                               // 0 * v is not 0 where v is infinite or NaN: such values are taken out here
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) { const uint32_t x = P::odd(b[w]); odd |= x; b[w] &= ~x; }
-                }
-#pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    if constexpr (NP == 1) { P::mma(o[2 * c], pf[0][h], b[0], b[1]); P::mma(o[2 * c + 1], pf[0][h], b[2], b[3]); }
-                    else { P::mma(part[n][0], pf[n][h], b[0], b[1]); P::mma(part[n][1], pf[n][h], b[2], b[3]); }
-                }
-            }
-            if constexpr (NP > 1) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float v = part[NP - 1][u][e];
-#pragma unroll
-                        for (int n = NP - 2; n >= 0; --n) v = part[n][u][e] + v * (1.0f / LIFT);
-                        o[2 * c + u][e] += v;
-                    }
-            }
-        }
-        if (edge && __any_sync(0xffffffffu, odd)) {       // ... and given back to the rows that see them
-            for (int j = 0; j < min(KEYS, k1 - key0); ++j)
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const KV * v = (const KV *) (smem + (vb - pa_smem(smem)) + j * D * 2 + ((c ^ (j & 7)) << 4)) + (lane & 3) * 2;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float x = (float) v[e];
-                        if (!(fabsf(x) < INFINITY)) {
-                            if (key0 + j <= last_a) o[c][e] += x;
-                            if (key0 + j <= last_b) o[c][e + 2] += x;
-                        }
-                    }
-                }
-        }
+        t.values(smem, vb, key0, k1, edge);
         __syncwarp();
         load(i + 2, at_next, true, vb);
     }
     pa_wait<0>();
-#pragma unroll
-    for (int of = 1; of < 4; of <<= 1) { la += __shfl_xor_sync(0xffffffffu, la, of); lb += __shfl_xor_sync(0xffffffffu, lb, of); }
+    t.finish();
     __syncthreads();
     // join of the four warps: [warp][row] maxima and sums, [warp][row][D + 4] accumulators over the rings
     float * sm = (float *) smem, * sl = sm + WARPS * PA_ROWS, * so = sl + WARPS * PA_ROWS;
     constexpr int LD = D + 4;
     {
         const int wa = warp * PA_ROWS + (lane >> 2), wb = wa + 8;
-        if ((lane & 3) == 0) { sm[wa] = ma; sm[wb] = mb; sl[wa] = la; sl[wb] = lb; }
+        if ((lane & 3) == 0) { sm[wa] = t.ma; sm[wb] = t.mb; sl[wa] = t.la; sl[wb] = t.lb; }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            *(float2 *) (so + wa * LD + c * 8 + (lane & 3) * 2) = make_float2(o[c][0], o[c][1]);
-            *(float2 *) (so + wb * LD + c * 8 + (lane & 3) * 2) = make_float2(o[c][2], o[c][3]);
+            *(float2 *) (so + wa * LD + c * 8 + (lane & 3) * 2) = make_float2(t.o[c][0], t.o[c][1]);
+            *(float2 *) (so + wb * LD + c * 8 + (lane & 3) * 2) = make_float2(t.o[c][2], t.o[c][3]);
         }
     }
     __syncthreads();
@@ -475,11 +503,11 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
                 x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w;
             }
         }
-        const int t = row / a.group, h = kvh * a.group + row % a.group;
-        const int64_t out = (s.tok0 + t) * a.n_head + h;
+        const int tok = row / a.group, h = kvh * a.group + row % a.group;
+        const int64_t out = (s.tok0 + tok) * a.n_head + h;
         if (whole) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            char * dst = a.dst + (s.tok0 + t) * a.nb_dst_tok + h * a.nb_dst_head + d * sizeof(Q);
+            char * dst = a.dst + (s.tok0 + tok) * a.nb_dst_tok + h * a.nb_dst_head + d * sizeof(Q);
             if constexpr (NP == 1) *(uint2 *) dst = make_uint2(P::two(x[0] * inv, x[1] * inv), P::two(x[2] * inv, x[3] * inv));
             else *(float4 *) dst = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
             if (a.lse && d == 0) a.lse[out] = sum == 0.0f ? -INFINITY : mx * 0.69314718f + logf(sum);
@@ -502,6 +530,83 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
         }
     }
     __syncthreads();                                      // the accumulators are read before the ring is filled again
+    }
+}
+
+// F32 queries, many rows: the eight warps of a CTA have 16 rows each and share every block of keys (three stages of two blocks, one barrier
+// a stage), so that K and V come from L2 once per 128 rows.  The rows of a warp are finished in its registers: no join.  Bound by
+// issue: the parts' products, and the additions that keep them in f32.  Against 16 rows a CTA, head_dim 64, f16: 32 ragged prompts of up to 224
+// tokens of 20 heads 103 -> 67 us; 4 chunks of 300 over 1000 keys, 12 heads (912 tiles of 16 rows) 63 -> 52; head_dim 128, chunks of 1024 over
+// 4k keys 1391 -> 1210.  With fewer tiles CTAs of 128 rows leave SMs idle: 16 chunks of 24 tokens x 4 heads x 8 (768 tiles) 95 -> 98, one
+// prompt of 224 tokens of 20 heads 12.7 -> 18.0.
+#define PA_WIDE 8
+template <typename KV, int D>
+__global__ void __launch_bounds__(32 * PA_WIDE, 1)
+k_paged_attn_wide(const __grid_constant__ PaArgs a) {
+    constexpr int NC = D / 8, KEYS = PaTile<float, KV, D>::KEYS, STAGE = 2 * KEYS, N = STAGE * NC / (32 * PA_WIDE), BYTES = 4 * PA_BLOCK, ROWS = PA_ROWS * PA_WIDE;
+    extern __shared__ __align__(16) char smem[];
+    chain_wait();                                         // no early release, as above
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int seq = blockIdx.z, kvh = blockIdx.y, tile = gridDim.x - 1 - blockIdx.x;      // the longest tiles first
+    const PaSeq s = pa_seq(a, seq);
+    const int n_rows = s.n_new * a.group, row0 = tile * ROWS, mine = row0 + warp * PA_ROWS;
+    if (row0 >= n_rows) return;
+    auto reach = [&](int r1) { return a.causal ? min(s.len, max(s.len - s.n_new + (min(r1, n_rows) - 1) / a.group + 1, 0)) : s.len; };
+    const int k1 = reach(row0 + ROWS), my_k1 = mine < n_rows ? reach(mine + PA_ROWS) : 0, n_stage = (k1 + STAGE - 1) / STAGE;
+    const char * kp = a.k + kvh * a.nb_head, * vp = a.v + kvh * a.nb_head;
+    const int32_t * table = a.tables + seq * a.table_stride;
+    const uint32_t ring = pa_smem(smem);
+    int page[N];
+    auto look = [&](int i) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) { const int key = i * STAGE + (c * 32 * PA_WIDE + tid) / NC; page[c] = i < n_stage && key < k1 ? table[key / a.page_size] : -1; }
+    };
+    auto load = [&](int i) {
+        if (i < n_stage) {
+            const uint32_t to = ring + i % 3 * BYTES;
+#pragma unroll
+            for (int c = 0; c < N; ++c) {
+                const int x = c * 32 * PA_WIDE + tid, r = x / NC, ch = x % NC;
+                const bool on = page[c] >= 0 && page[c] < a.n_pages;
+                const int64_t off = on ? page[c] * a.nb_page + ((i * STAGE + r) % a.page_size) * a.nb_tok + ch * 16 : 0;
+                const uint32_t d = to + r * D * 2 + ((ch ^ (r & 7)) << 4);
+                pa_cp16(d, kp + off, on); pa_cp16(d + 2 * PA_BLOCK, vp + off, on);
+            }
+        }
+        pa_commit();
+    };
+    look(0); load(0); look(1); load(1); look(2);
+    PaTile<float, KV, D> t;
+    if (mine < n_rows) t.start(a, s, kvh, mine, n_rows);
+    for (int i = 0; i < n_stage; ++i) {
+        pa_wait<1>();
+        __syncthreads();                                  // the stage is here, and nobody reads the one before it
+        load(i + 2);
+        look(i + 3);
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+            const int key0 = i * STAGE + u * KEYS;
+            if (key0 >= my_k1) break;
+            const uint32_t kb = ring + i % 3 * BYTES + u * PA_BLOCK, vb = kb + 2 * PA_BLOCK;
+            const bool edge = key0 + KEYS - 1 > t.first_last || key0 + KEYS > my_k1;
+            t.scores(kb);
+            t.weights(key0, my_k1, edge);
+            t.values(smem, vb, key0, my_k1, edge);
+        }
+    }
+    pa_wait<0>();
+    if (mine >= n_rows) return;
+    t.finish();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int row = mine + (lane >> 2) + 8 * u;
+        if (row >= n_rows) continue;
+        const float l = u ? t.lb : t.la, inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int tok = row / a.group, h = kvh * a.group + row % a.group;
+        float * dst = (float *) (a.dst + (s.tok0 + tok) * a.nb_dst_tok + h * a.nb_dst_head) + (lane & 3) * 2;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) *(float2 *) (dst + c * 8) = make_float2(t.o[c][2 * u] * inv, t.o[c][2 * u + 1] * inv);
+        if (a.lse && (lane & 3) == 0) a.lse[(s.tok0 + tok) * a.n_head + h] = l == 0.0f ? -INFINITY : (u ? t.mb : t.ma) * 0.69314718f + logf(l);
     }
 }
 
@@ -608,18 +713,20 @@ static bool pa_args_ok(const b200_page_pool * p, const b200_paged_attn_args * a,
 }
 
 // Which kernel, and how its work is dealt out.
-struct PaPlan { bool tc, store; int stream, tiles, n_whole, n_split, chunk; int64_t items; };
+struct PaPlan { bool tc, wide, store; int stream, tiles, n_whole, n_split, chunk; int64_t items; };
 static PaPlan pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a) {
     PaPlan r = {};
     const int64_t group = a->n_head / p->n_head_kv;
     const int64_t new_max = a->max_new < a->n_tok ? a->max_new : a->n_tok, rows = new_max * group;
     r.tc = a->q_type != B200_TYPE_F32 && rows > PA_TC_MIN_ROWS;
-    r.store = a->k_new && (r.tc || new_max > PA_ROWS);     // few new rows are stored by the kernel itself
     const int64_t tile = r.tc ? PA_TC_ROWS(p->head_dim) : PA_ROWS, tiles = (rows + tile - 1) / tile;
     const int64_t round = r.tc ? PA_TC_KEYS(p->head_dim) : PA_BLOCK / (2 * p->head_dim) * PA_WARPS, rounds = (a->max_len + round - 1) / round;
     const int64_t resident = 148 * (r.tc ? PA_TC_CTAS(p->head_dim) : a->q_type == B200_TYPE_F32 ? 2 : 3);
     r.items = tiles * p->n_head_kv * a->n_seq;
     r.tiles = (int) tiles;
+    r.wide = a->q_type == B200_TYPE_F32 && rows > PA_WIDE_MIN_ROWS && r.items >= PA_WIDE_MIN_ITEMS;
+    r.store = a->k_new && (r.tc || r.wide || new_max > PA_ROWS);       // few new rows are stored by the kernel itself
+    if (r.wide) return r;
     if (!r.tc) {
         // Items of few rounds are not worth the join, and many tiles of a chunk fill the device by themselves (their reach differs, which
         // the line does not know).
@@ -725,6 +832,13 @@ extern "C" int b200_paged_attn(const b200_page_pool * pool, const b200_paged_att
     const bool f32 = a->q_type == B200_TYPE_F32, h = pool->type == B200_TYPE_F16;
     const PaNew x = { r.store ? nullptr : (const char *) a->k_new, (const char *) a->v_new, a->nb_new_tok, a->nb_new_head };
     cudaError_t e;
+    if (r.wide) {
+        const dim3 grid((unsigned) ((k.max_new * (int64_t) k.group + PA_ROWS * PA_WIDE - 1) / (PA_ROWS * PA_WIDE)), (unsigned) k.n_head_kv, (unsigned) a->n_seq);
+        auto f = pool->head_dim == 64 ? (h ? k_paged_attn_wide<__half, 64> : k_paged_attn_wide<__nv_bfloat16, 64>) : (h ? k_paged_attn_wide<__half, 128> : k_paged_attn_wide<__nv_bfloat16, 128>);
+        e = launch_chained(f, grid, dim3(32 * PA_WIDE), 3 * 4 * PA_BLOCK, st, k);
+        if (e != cudaSuccess) return (int) e;
+        B200_RETURN_LAST();
+    }
     if (pool->head_dim == 64)
         e = f32 ? (h ? pa_launch<float, __half, 64>(k, x, a->n_seq, r.items, st) : pa_launch<float, __nv_bfloat16, 64>(k, x, a->n_seq, r.items, st))
                 : (h ? pa_launch<__half, __half, 64>(k, x, a->n_seq, r.items, st) : pa_launch<__nv_bfloat16, __nv_bfloat16, 64>(k, x, a->n_seq, r.items, st));

@@ -82,8 +82,6 @@ k_paged_store(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew x,
 #define PA_ROWS  16
 #define PA_BLOCK 4096                            // bytes of a block of K or V: 32 keys of 64 or 16 of 128 dimensions
 #define PA_WARPS 4
-#define PA_MIN_ROUNDS 8
-#define PA_TC_MIN_ROWS 64
 #define PA_WIDE_MIN_ROWS 64                      // f32 queries: with more rows a head, and this many tiles of 16 rows, k_paged_attn_wide
 #define PA_WIDE_MIN_ITEMS (6 * 148)
 
@@ -718,7 +716,15 @@ static PaPlan pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a) 
     PaPlan r = {};
     const int64_t group = a->n_head / p->n_head_kv;
     const int64_t new_max = a->max_new < a->n_tok ? a->max_new : a->n_tok, rows = new_max * group;
-    r.tc = a->q_type != B200_TYPE_F32 && rows > PA_TC_MIN_ROWS;
+    // tcgen05 where its tiles of 128 or 256 rows are not mostly empty and the work fills the device, by the number of tiles of 16 rows and by them
+    // times keys.  us, mma.sync and tcgen05, head_dim 64: 4 prompts of 256 tokens of 20 heads (1280 tiles) 24.5, 19.0; a chunk of 256 over 2256 keys
+    // (320 tiles, 720k) 46, 38; but 1 prompt of 256 (320 tiles, 82k) 12.5, 15.9; a chunk of 256 over 8256 keys of 6 heads (96 tiles) 42, 57.
+    // head_dim 128, 8 heads: 64 prompts of 128 rows (4096 tiles) 63, 45; a chunk of 64 rows over 8k keys (32 tiles, 258k) 38, 28; but 64
+    // prompts of 48 rows (1536 tiles, 18k) 34, 41.  With up to 32 rows equal sequences gain a little, ragged ones lose more (16 of up to 32
+    // tokens, 20 heads, up to 2500 keys: 51, 69).
+    const int64_t small = (rows + PA_ROWS - 1) / PA_ROWS * p->n_head_kv * a->n_seq, work = small * a->max_len;
+    r.tc = a->q_type != B200_TYPE_F32 && rows > 2 * PA_ROWS &&
+           (p->head_dim == 64 ? small >= 640 || (small >= 160 && work >= 500000) : (small >= 512 && rows >= 128) || work >= 250000);
     const int64_t tile = r.tc ? PA_TC_ROWS(p->head_dim) : PA_ROWS, tiles = (rows + tile - 1) / tile;
     const int64_t round = r.tc ? PA_TC_KEYS(p->head_dim) : PA_BLOCK / (2 * p->head_dim) * PA_WARPS, rounds = (a->max_len + round - 1) / round;
     const int64_t resident = 148 * (r.tc ? PA_TC_CTAS(p->head_dim) : a->q_type == B200_TYPE_F32 ? 2 : 3);
@@ -728,18 +734,23 @@ static PaPlan pa_plan(const b200_page_pool * p, const b200_paged_attn_args * a) 
     r.store = a->k_new && (r.tc || r.wide || new_max > PA_ROWS);       // few new rows are stored by the kernel itself
     if (r.wide) return r;
     if (!r.tc) {
-        // Items of few rounds are not worth the join, and many tiles of a chunk fill the device by themselves (their reach differs, which
-        // the line does not know).
-        if (rounds >= PA_MIN_ROUNDS && (tiles == 1 || r.items < 2 * resident)) {
-            const int64_t want = r.items * rounds / (PA_MIN_ROUNDS / 2);
+        // The line where items are long, or, from 12 rounds on, where they would leave the last wave half empty; many tiles of a chunk fill the
+        // device by themselves (their reach differs, which the line does not know).  Single tokens, us without and with the line:
+        // head_dim 64, 20 heads, 16 rounds (2000 keys): 1 sequence 15.9, 16.1; 4: 16.3, 19.9; 16: 36, 41.  head_dim 128, 8 heads, 16 rounds (1000
+        // keys): 1 sequence 16.1, 16.9; 16: 17, 23; 64 (1.15 waves) 66, 57; 21 rounds: 1 sequence 19.9, 17.4; 64 92, 75.
+        const bool tail = r.items > resident && r.items % resident <= resident / 2;
+        if ((rounds >= 18 || (rounds >= 12 && tail)) && (tiles == 1 || r.items < 2 * resident)) {
+            const int64_t want = r.items * rounds / 4;
             r.stream = (int) (want < resident ? want : resident);
         }
         return r;
     }
     const int64_t whole = r.items / resident * resident, rest = r.items - whole;
     int64_t split = rest ? resident / rest : 1;
-    if (split > rounds / (PA_MIN_ROUNDS / 2)) split = rounds / (PA_MIN_ROUNDS / 2);
-    if (whole > 8 * resident || split < 1) split = 1;      // the last of many waves is not worth the join
+    if (split > rounds / 4) split = rounds / 4;
+    // The last of many waves is not worth the join; with four CTAs an SM no last wave is (64 chunks of 300 over 1300 keys, 20 heads: 338 us whole,
+    // 370 split).  head_dim 128: 2 chunks of 2048 over 16k keys, 3.5 waves, 949 split, 1040 whole.
+    if (split < 1 || whole > (p->head_dim == 64 ? 0 : 8 * resident)) split = 1;
     r.n_whole = (int) (split == 1 ? r.items : whole);
     r.chunk = split == 1 ? 0 : (int) ((rounds + split - 1) / split * round);
     r.n_split = split == 1 ? 1 : (int) ((a->max_len + r.chunk - 1) / r.chunk);

@@ -64,7 +64,8 @@ __device__ __forceinline__ void pg_copy(const b200_page_pool & pool, int n, int6
 #define PG_CLUSTER 16
 #define PG_MAX_ROWS 8192
 #define PG_SMALL   (160 * 1024)   // bytes of shared memory that a small state may take
-#define PG_FUSED   4096           // words of tables and counts up to which every CTA works them out for itself
+#define PG_FUSED   3000           // words of tables and counts up to which every CTA works them out for itself (5 beams, pages of 16, 8 layers of 20 heads; us
+                                  // with and without: 1 sequence of 230 tokens 7.5, 9.1; 8 of 400 10.4, 11.4; 16 of 400 16.4, 15.7; 24 of 400 19.3, 17.5)
 #define PG_HEADER  8              // workspace words before the lists: [0] copies, [1] tokens per whole page, [2] see k_pages_compact
 
 struct PgWork { int32_t * head; int32_t * copies; int32_t * a; int32_t * b; };    // copies: (src, dst, tokens) each

@@ -326,6 +326,68 @@ def test_many_f32_rows_do_not_see_what_comes_later(K, pkg):
     assert torch.equal(x.out[:, 3:], y.out[:, 3:])
 
 
+# The forms for many rows of 16-bit queries are taken where tiles are many (head_dim 64: 640 of 16 rows; 128: 512, or 250 000 tiles x keys)
+
+@pytest.mark.parametrize("ps", [1, 3, 8, 16, 24, 48, 64, 128, 256, 512])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kw", [dict(t="f16"), dict(t="bf16", layout="head", causal=0), dict(t="bf16", scale=-0.3), dict(t="f16", scale=0.0, n_layer=2, layer=1, pad_q=1)])
+def test_attention_of_many_16_bit_rows(K, pkg, ps, D, kw):
+    t = kw["t"]
+    x = Attn(K, pkg, np.random.default_rng(ps + D), [(150, 700), (1, 513), (90, 90), (256, 256), (0, 9), (100, 40)], 10, 1, D, t, t, ps, **{k: v for k, v in kw.items() if k != "t"})
+    pool = x.want_pool(x.c.view)
+    x.run()
+    x.check(pool)
+
+
+@pytest.mark.parametrize("seqs,Hkv,g,D,ps", [([(300, 2000), (129, 1300), (0, 0), (1, 900)], 2, 4, 128, 64), ([(70, 60003), (1, 3)], 1, 2, 128, 16), ([(64, 9000), (40, 7000)], 2, 1, 128, 24),
+                                            ([(300, 4000), (129, 3300), (0, 0), (1, 5000)], 3, 1, 64, 16), ([(400, 2100)] * 3, 3, 3, 64, 100)])
+def test_attention_of_many_16_bit_rows_split(K, pkg, seqs, Hkv, g, D, ps):
+    """Few tiles over long contexts: split keys, and their join."""
+    x = Attn(K, pkg, np.random.default_rng(len(seqs)), seqs, Hkv, g, D, "bf16", "bf16", ps)
+    pool = x.want_pool(x.c.view)
+    x.run()
+    x.check(pool)
+
+
+@pytest.mark.parametrize("ps", [64, 48])
+def test_attention_of_many_16_bit_rows_and_pages_far_apart(K, pkg, far, ps):
+    x = Attn(K, pkg, np.random.default_rng(ps), [(150, 260), (40, 300)], 2, 2, 128, "f16", "f16", ps, extra_len=9000)
+    assert x.c.n_pages * x.c.pool.nb_page > 1 << 32
+    pool = x.want_pool(x.c.view)
+    x.run()
+    x.check(pool)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_16_bit_rows_do_not_see_what_comes_later(K, pkg, D):
+    def make():
+        return Attn(K, pkg, np.random.default_rng(2), [(200, 230)] * 4, 20, 1, D, "f16", "f16", 16)
+    x, y = make(), make()
+    x.kn[100, 0], x.vn[100, 1, 3], x.vn[101, 2, 5] = float("nan"), float("inf"), float("nan")
+    x.run()
+    y.run()
+    torch.cuda.synchronize()
+    assert torch.equal(x.out[:100], y.out[:100]) and torch.equal(x.out[200:], y.out[200:]) and torch.equal(x.lse[:100], y.lse[:100])
+    assert x.out[100:200, 0].isnan().all() and not x.out[100:200, 1, 3].isfinite().any() and x.out[101:200, 2, 5].isnan().all()
+    rest = [i for i in range(D) if i != 5]
+    assert torch.equal(x.out[100:200, 2][..., rest], y.out[100:200, 2][..., rest]) and torch.equal(x.out[100, 2], y.out[100, 2])
+    assert torch.equal(x.out[:, 3:], y.out[:, 3:])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_16_bit_rows_with_huge_scores(K, pkg, D):
+    """As test_attention_finite_but_huge_scores."""
+    x = Attn(K, pkg, np.random.default_rng(D), [(130, 170)] * 5, 20, 1, D, "bf16", "bf16", 16, scale=1.0)
+    x.q.mul_(2e17); x.kn.mul_(2e17)
+    pool = x.want_pool(x.c.view)
+    x.run()
+    torch.cuda.synchronize()
+    for i in (0, 4):
+        k, v = (pool[j, 0].double().cpu().numpy()[x.tables[i, np.arange(170) // 16], np.arange(170) % 16] for j in (0, 1))
+        out, _, _, _ = R.attention(x.q[130 * i:130 * (i + 1)].double().cpu().numpy(), k, v, 130, 170, 1.0, 1)
+        assert np.all(np.abs(x.out[130 * i:130 * (i + 1)].double().cpu().numpy() - out) <= 2.0 ** -8 * np.abs(out) + 1e-30)
+
+
 def test_no_wait_ran_out(K, pkg):
     """After everything above (this process' launches so far)."""
     x = Attn(K, pkg, np.random.default_rng(0), [(300, 400)], 1, 1, 128, "f16", "f16", 16)

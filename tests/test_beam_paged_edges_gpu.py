@@ -388,6 +388,35 @@ def test_many_16_bit_rows_with_huge_scores(K, pkg, D):
         assert np.all(np.abs(x.out[130 * i:130 * (i + 1)].double().cpu().numpy() - out) <= 2.0 ** -8 * np.abs(out) + 1e-30)
 
 
+@pytest.mark.parametrize("D,heads", [(64, 20), (128, 10)])
+def test_chunks_right_behind_what_makes_their_inputs(K, pkg, D, heads):
+    """Queries, new rows, tables and lengths written by the launches just before, over and over, without a synchronisation between: attention
+    begins while the store of its new rows still runs, but not before what came earlier."""
+    rng = np.random.default_rng(D)
+    seqs = [(200, 260), (130, 130), (90, 400), (256, 300)]
+    xs = [Attn(K, pkg, rng, seqs, heads, 1, D, "f16", "f16", 16) for _ in range(2)]
+    want = []
+    for x in xs:
+        x.run()
+        torch.cuda.synchronize()
+        want.append((x.out.clone(), x.lse.clone()))
+    a = xs[0]
+    sources = [(x.q.clone(), x.kn.clone(), x.vn.clone(), x.c.buf.clone(), x.dtab.clone(), x.dlen.clone()) for x in xs]
+    got = []
+    for i in range(12):
+        for dst, src in zip((a.c.buf, a.kn, a.vn, a.dtab, a.dlen, a.q), (sources[i % 2][j] for j in (3, 1, 2, 4, 5, 0))):
+            if dst.shape == src.shape:
+                dst.copy_(src)
+        if i % 3 == 0:
+            a.out[:a.n_tok].zero_()
+        a.run()
+        got.append((a.out.clone(), a.lse.clone()))
+    torch.cuda.synchronize()
+    assert all(s[4].shape == a.dtab.shape and s[3].shape == a.c.buf.shape for s in sources)
+    for i, g in enumerate(got):
+        assert torch.equal(g[0], want[i % 2][0]) and torch.equal(g[1], want[i % 2][1]), i
+
+
 def test_no_wait_ran_out(K, pkg):
     """After everything above (this process' launches so far)."""
     x = Attn(K, pkg, np.random.default_rng(0), [(300, 400)], 1, 1, 128, "f16", "f16", 16)

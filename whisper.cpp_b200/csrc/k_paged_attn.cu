@@ -40,8 +40,8 @@ template <> __device__ __forceinline__ void pa_unpack8<__nv_bfloat16>(uint4 q, f
 template <typename KV, bool F32>
 __global__ void __launch_bounds__(256)
 k_paged_store(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew x, int log_vec) {
-    chain_release();
-    chain_wait();
+    chain_wait();                                         // in this order: once all CTAs have released, all that came before this launch is there,
+    chain_release();                                      // and the attention behind it may read its queries and tables at once (32 ragged prompts: 36.1 -> 34.2 us)
     const PaSeq s = pa_seq(a, blockIdx.y);
     const int lane = threadIdx.x & 31, per_tok = 2 * a.n_head_kv << log_vec, mask = (1 << log_vec) - 1;
     for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < s.n_new; t += gridDim.x * 8) {
@@ -838,6 +838,7 @@ extern "C" int b200_paged_attn(const b200_page_pool * pool, const b200_paged_att
     if (r.store) {
         const int rc = b200_paged_store(pool, a, stream);
         if (rc) return rc;
+        k.early = 1;
     }
     const cudaStream_t st = as_stream(stream);
     const bool f32 = a->q_type == B200_TYPE_F32, h = pool->type == B200_TYPE_F16;

@@ -187,7 +187,8 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
     using L = PtSmem<D, BN, NS, NTILE>;
     constexpr int COLS = NTILE * (BN + D) <= 128 ? 128 : NTILE * (BN + D) <= 256 ? 256 : 512, NC = D / 8, ROWS = 128 * NTILE, W_MMA = 4 * NTILE;
     extern __shared__ __align__(16) char smem_raw[];
-    chain_wait();                                         // no early release: this kernel wants whole SMs
+    if (!a.early) chain_wait();                           // behind the store of the same call: only what reads its pages waits (below). No early
+                                                          // release: this kernel wants whole SMs
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // the shuffle tells the compiler that the warp agrees
     const PaItem item = pa_item(a, blockIdx.x);
     const int seq = item.seq, split = max(item.split, 0), kvh = item.kvh, row0 = item.tile * ROWS, chunk = item.split < 0 ? 1 << 30 : a.chunk;
@@ -250,6 +251,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             __syncwarp();
             if (lane == 0) pt_arrive(q_full);
         }
+        if (a.early) chain_wait();
         const float scale = a.scale_log2 == 0 ? 1.0f : fabsf(a.scale_log2);        // 0 is in Q: masked scores are -inf, and -inf * 0 is not
         const int last = !valid ? -1 : a.causal ? s.len - s.n_new + tok : s.len - 1;
         const uint32_t lanes = (uint32_t) (warp & 3) << 21;              // 32 lanes per warp, in bits 16 and up
@@ -409,6 +411,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
         }
     } else {
         // ================= K and V =================
+        if (a.early) chain_wait();
         const bool is_v = warp == W_MMA + 2;
         const char * base = (is_v ? a.v : a.k) + kvh * a.nb_head;
         const uint32_t ring = sb + (is_v ? L::V : L::K), full = is_v ? v_full : k_full, empty = is_v ? v_empty : k_empty;

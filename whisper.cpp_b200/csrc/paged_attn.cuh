@@ -13,6 +13,7 @@ struct PaArgs {
     int64_t n_tok, max_len;
     int n_pages, page_size, n_head, n_head_kv, group, max_new, causal, n_split, chunk, tile_rows, stream, n_seq, tiles, n_whole;
     float scale_log2;               // scale * log2(e): weights are powers of two
+    int early;                      // the launch before this one is the store of the same call: what it waited for is there
 };
 
 // 2^x; below 2^-126 it is 0

@@ -259,7 +259,9 @@ int b200_topk_rows(const float * const * rows, b200_topk_result * const * out, i
  * below do the same work next to the logits.  They are defined by their formulas, not by a reference kernel: sums, softmax
  * statistics and scores are held in 32 bits or more, and every result is independent of the order in which blocks run.
  * None of them allocates, synchronises or keeps anything between calls; all may be captured into a graph.  Scratch memory
- * comes from the caller (16-byte aligned); two calls that may overlap on the device need a scratch area each. */
+ * comes from the caller (16-byte aligned); two calls that may overlap on the device need a scratch area each.  How much a call
+ * needs depends on how its work is dealt out: a smaller call can need more than a larger one, so ask for every size that is used
+ * (b200_paged_attn: never more than 21 MB). */
 
 /* The next beams of every sequence.  Row r = sequence * n_beam + beam has n_vocab logits x (F32, F16 or BF16; nb_row bytes
  * between rows) and an accumulated score.  Candidates are

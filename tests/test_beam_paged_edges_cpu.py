@@ -41,3 +41,16 @@ def test_attention_refuses_unaligned_words_and_too_many_rows(K, pkg):
         assert K.b200_paged_attn(C.byref(pool(pkg)), C.byref(changed(pkg.PagedAttnArgs, ok, **kw)), None) == ERR, kw
     for scale in (3e38, -3e38, float("inf"), float("nan")):        # times log2(e) no float
         assert K.b200_paged_attn(C.byref(pool(pkg)), C.byref(changed(pkg.PagedAttnArgs, ok, scale=scale)), None) == ERR
+
+
+def test_attention_workspace_is_bounded(K, pkg):
+    import random
+    rng = random.Random(1)
+    most = 0
+    for _ in range(20000):
+        d, kv = rng.choice([64, 128]), rng.choice([1, 2, 4, 6, 8, 12, 20, 32])
+        pl = pool(pkg, head_dim=d, n_head_kv=kv, nb_head=2 * d, nb_tok=2 * d * kv, nb_page=8 * d * kv, page_size=4)
+        new, seqs = int(2 ** rng.uniform(0, 13)), int(2 ** rng.uniform(0, 9))
+        a = pkg.PagedAttnArgs(q_type=rng.choice([0, 1]), n_tok=new * seqs, n_seq=seqs, n_head=kv * rng.choice([1, 2, 4, 8]), max_new=new, max_len=int(2 ** rng.uniform(0, 20)))
+        most = max(most, K.b200_paged_attn_workspace(C.byref(pl), C.byref(a)))
+    assert 0 < most <= 21_000_000

@@ -417,6 +417,46 @@ def test_chunks_right_behind_what_makes_their_inputs(K, pkg, D, heads):
         assert torch.equal(g[0], want[i % 2][0]) and torch.equal(g[1], want[i % 2][1]), i
 
 
+@pytest.mark.parametrize("n_new,heads,qt", [(1, 2, "f16"), (3, 2, "f32"), (260, 20, "f16"), (260, 20, "f32")])
+def test_attention_without_any_keys(K, pkg, n_new, heads, qt):
+    """max_len 0, and lengths of 0 under a larger bound: zeros, lse -inf, nothing stored."""
+    for max_len in (0, 500):
+        x = Attn(K, pkg, np.random.default_rng(n_new), [(n_new, 300)] * 4, heads, 1, 64, "f16", qt, 16)
+        before = x.c.view.clone()
+        x.dlen.zero_()
+        x.a.max_len = max_len
+        n = K.b200_paged_attn_workspace(C.byref(x.c.pool), C.byref(x.a))
+        x.ws = torch.zeros(max(n, 16), dtype=torch.uint8, device="cuda")
+        x.a.workspace, x.a.workspace_bytes = p(x.ws), n
+        x.run()
+        torch.cuda.synchronize()
+        assert torch.equal(torch.nan_to_num(x.c.view, 3.0), torch.nan_to_num(before, 3.0))
+        assert (x.out[:x.n_tok] == 0).all() and (x.lse[:x.n_tok] == -np.inf).all() and (x.out[x.n_tok:] == 7).all()
+
+
+def test_pages_of_no_rows(K, pkg):
+    """No rows: update copies the counts, compact moves what other holders have."""
+    c = Cache(pkg, np.random.default_rng(0), 20, 8)
+    refs = np.zeros(20, int)
+    refs[[3, 11, 17]] = 1, 2, 1
+    before = c.view.clone()
+    frm, f = c.state(pkg, np.zeros((0, 1), int), np.zeros(0, int), refs)
+    to, t = c.state(pkg, np.zeros((0, 1), int), np.zeros(0, int), np.full(20, 99))
+    status, remap = (torch.full((n,), 55, dtype=torch.int32, device="cuda") for n in (2, 20))
+    n = K.b200_pages_workspace(0, 20)
+    ws = torch.full((n,), 255, dtype=torch.uint8, device="cuda")
+    assert K.b200_pages_update(C.byref(c.pool), C.byref(f), C.byref(t), None, None, None, p(status), p(ws), n, stream()) == 0
+    torch.cuda.synchronize()
+    assert status.tolist() == [0, 0] and np.array_equal(to["refs"].cpu().numpy(), refs) and torch.equal(c.view, before)
+    assert K.b200_pages_compact(C.byref(c.pool), C.byref(f), C.byref(t), p(remap), p(status), p(ws), n, stream()) == 0
+    torch.cuda.synchronize()
+    got = remap.cpu().numpy()
+    live = [int(i) for i in got[[3, 11, 17]]]
+    assert status.tolist()[0] == 0 and sorted(live) == [0, 1, 2] and (got[refs == 0] == -1).all()
+    for old, new in zip((3, 11, 17), live):
+        assert torch.equal(c.view[:, :, new], before[:, :, old]) and int(to["refs"][new]) == refs[old]
+
+
 def test_no_wait_ran_out(K, pkg):
     """After everything above (this process' launches so far)."""
     x = Attn(K, pkg, np.random.default_rng(0), [(300, 400)], 1, 1, 128, "f16", "f16", 16)

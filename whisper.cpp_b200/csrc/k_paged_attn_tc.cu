@@ -19,7 +19,7 @@
 //   2 warps          bring K and V by TMA, page by page into the swizzled tile, where pages fit into blocks or blocks into pages (page
 //                    sizes 8, 16, 32, .. and multiples of BN); otherwise per key one page lookup and 16-byte cp.async.  Zeros for keys
 //                    out of reach and pages out of the pool.
-// Measured, head_dim 128, bf16, chunks of 2048 queries over 16k keys, 32 heads on 8: 949 us, 1.08 PFLOP/s.  What bounds it is the chain of a
+// Measured, head_dim 128, bf16, chunks of 2048 queries over 16k keys, 32 heads on 8: 946 us, 1.09 PFLOP/s.  What bounds it is the chain of a
 // tile: its softmax, then P V and the next Q K^T, while the other tile's softmax and products run beside it.  Tried without gain: P
 // handed over in two halves (1097 against 1037 us), two score buffers with blocks of 64 keys (1661: Q K^T with N = 64 reads Q from shared
 // memory twice as often), two threads a row (981 against 967).

@@ -13,7 +13,8 @@
 // only those are looked at one by one.  Where equal logits make them more than SEL_CAP, the bound is taken once more over the threads' maxima
 // with the index as the second part of the key; then the n_beam threads that reach it hold all that do.
 // 320 rows of 51866 (f32): 65 us with a sorted list per warp, filled tile by tile; 35 with the n_beam best thread maxima of every warp as the
-// bound and slices of four tiles (two CTAs an SM), 27 with two tiles (four CTAs).
+// bound and slices of four tiles (two CTAs an SM), 27 with two tiles (four CTAs), 23 with the groups' maxima.  No faster: CTAs of 128 threads (22.8),
+// CTAs that stay and ask for their next slice ahead (37: what counts is how many slices are under way).
 #define SEL_THREADS 256
 #define SEL_EPT     16                              // logits per thread and tile
 #define SEL_TILE    (SEL_THREADS * SEL_EPT)
@@ -59,7 +60,8 @@ struct SelSlices {            // workspace of a call: [rows][n_slice] maxima and
     float * m; double * s; float * x; int32_t * v;
 };
 
-// tiles of a slice: single tiles as long as larger slices would not fill the device (5 rows of 51866: 65 CTAs)
+// tiles of a slice: single tiles as long as larger slices would not fill the device twice (rows of 51866 f32 logits, us with one and two tiles: 5 rows
+// 7.9, 8.3; 40 rows 9.7, 10.1; 60 rows 11.5, 11.0; 320 rows 28.3, 24.0)
 static inline int sel_tiles(int64_t rows, int n_beam, int64_t n_vocab) {
     const int64_t slices = (n_vocab + SEL_TILE * SEL_MANY - 1) / (SEL_TILE * SEL_MANY);
     return rows * slices >= 148 * 2 || n_beam * ((n_vocab + SEL_TILE - 1) / SEL_TILE) > 4096 ? SEL_MANY : 1;

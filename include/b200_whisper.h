@@ -337,7 +337,10 @@ int b200_pages_copy(const b200_page_pool * pool, int64_t n_rows, const void * wo
  * = 0).  Query head h reads key/value head h / (n_head / n_head_kv).  q is F16 or BF16 like the pool, or F32; dst has q's type:
  *   dst[tok][h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale * q.k_j - m),   lse[tok][h] = m + log(sum_j w_j)   (lse may be NULL)
  * Scores and sums are 32-bit; for 16-bit q the weights w_j are rounded to the pool's type before the product with V, which
- * adds at most half a step of that type relative to each weight, the size of the output's own rounding.  For F32 q nothing is rounded to fewer bits.  A query
+ * adds at most half a step of that type relative to each weight, the size of the output's own rounding (F16: for weights below 2^-25 of the
+ * largest, at most 2^-36 of the largest instead), and the tensor pipe truncates its 32-bit sums instead of rounding them.  For F32 q the products take q
+ * and the weights with the pool's type in two parts (F16: 22 bits, but no finer than 2^-36 of a row's largest |q| and 2^-50 of the largest weight) or
+ * three (BF16: 24 bits), and their sums are rounded.  A query
  * without a key gives zeros and lse -inf; a NaN or infinite value in a position that a query does not attend to has no effect on it.
  * A NaN or infinite value in one that it does attend to leaves the dimensions that it enters infinite or NaN.
  * k_new / v_new (type of q, [n_tok][n_head_kv][head_dim] with strides nb_new_tok, nb_new_head) are first stored at their positions,

@@ -1,0 +1,50 @@
+"""Attention over the paged cache where weights are small, values infinite, steps have failed or are over; beam selection and page states at their ends.
+Helpers and plain forms as in test_beam_paged_gpu.py."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import paged_ref as R
+from test_beam_paged_gpu import K, Attn, Cache, Select, check_select, check_update, dev, p, run_update, stream  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def one_leader(K, pkg, seqs, Hkv, g, D, t, qt, ps, lead, at):
+    """Every key of a sequence has the same score but the one at `at`, which lies `lead` nats above and has the value 0; all values have one sign."""
+    x = Attn(K, pkg, np.random.default_rng(1), seqs, Hkv, g, D, t, qt, ps, store=False)
+    x.q.zero_()
+    x.q[..., 0] = 8.0
+    x.c.view[0].zero_()
+    x.c.view[1] = x.c.view[1].abs() + 1.0
+    for i in range(len(seqs)):
+        page, tok = int(x.tables[i, at // ps]), at % ps
+        x.c.view[0, 0, page, tok, :, 0] = round(lead / (8.0 * x.scale) * 8) / 8      # exact in the pool's types
+        x.c.view[1, 0, page, tok] = 0.0
+    return x
+
+
+FORMS = [
+    # seqs, Hkv, g, D, ps, position of the leader: eight warps an item, four warps, the line, many rows (tcgen05, or 128 f32 rows a CTA), tcgen05 split
+    ([(1, 400)], 2, 2, 64, 16, 40),
+    ([(1, 400)] * 80, 2, 2, 64, 16, 40),
+    ([(1, 40003)], 1, 2, 64, 16, 39000),
+    ([(1, 9001), (1, 20002)], 2, 4, 128, 16, 8000),
+    ([(200, 900)] * 4, 20, 1, 64, 16, 600),
+    ([(200, 900)] * 4, 20, 1, 128, 16, 600),
+    ([(300, 4000)], 2, 4, 128, 64, 3650),
+    ([(300, 3000)], 10, 1, 64, 64, 2600),
+]
+
+
+@pytest.mark.parametrize("form", range(len(FORMS)))
+@pytest.mark.parametrize("t,qt,lead", [("f16", "f16", 15), ("f16", "f16", 17), ("f16", "f32", 22), ("bf16", "bf16", 17), ("bf16", "f32", 22)])
+def test_small_weights_beside_a_large_one(K, pkg, form, t, qt, lead):
+    """What many keys far below the largest score add up to is there: exp(-17) = 2^-24.5 and, for f32 queries, exp(-22) = 2^-31.7 are below what f16
+    holds with all its bits beside a weight of 1. Tolerances of Attn.check: roundings relative to every weight."""
+    x = one_leader(K, pkg, *FORMS[form][:4], t, qt, FORMS[form][4], lead, FORMS[form][5])
+    pool = x.c.view.clone()
+    x.run()
+    x.check(pool)

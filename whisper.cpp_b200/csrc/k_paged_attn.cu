@@ -139,6 +139,9 @@ template <typename Q, typename KV, int D> struct PaTile {
     using P = PaPack<KV>;
     static constexpr int NP = PaParts<Q, KV>::n, NC = D / 8, KS = D / 16, KEYS = PA_BLOCK / (2 * D), NK = KEYS / 8;      // parts, 16-byte chunks and MMA steps of a head; keys of a block, MMA columns of its scores
     static constexpr float LIFT = PaParts<Q, KV>::lift;
+    // f16 has all its bits from 2^-14 on and nothing below 2^-25: the weights, 1 at the running maximum, enter the product with V times 2^14, so that
+    // many small ones beside a large one count (131072 keys of weight 2^-26 and one of 1 and value 0: the result was 0 instead of 0.002)
+    static constexpr float RAISE = std::is_same<KV, __half>::value ? 16384.0f : 1.0f;
     uint32_t qf[NP][KS][4], pf[NP][NK / 2][4];
     float fa, fb, o[NC][4], sc[NK][4], ma, mb, la, lb;
     int last_a, last_b, first_last;                       // keys up to last_*: seen by the row; up to first_last: by every row
@@ -251,10 +254,10 @@ template <typename Q, typename KV, int D> struct PaTile {
                 la += sc[j][e]; lb += sc[j][e + 2];
             }
             uint32_t w[NP];
-            pa_parts<Q, KV>(sc[j][0], sc[j][1], w);
+            pa_parts<Q, KV>(sc[j][0] * RAISE, sc[j][1] * RAISE, w);
 #pragma unroll
             for (int n = 0; n < NP; ++n) pf[n][j >> 1][(j & 1) * 2] = w[n];
-            pa_parts<Q, KV>(sc[j][2], sc[j][3], w);
+            pa_parts<Q, KV>(sc[j][2] * RAISE, sc[j][3] * RAISE, w);
 #pragma unroll
             for (int n = 0; n < NP; ++n) pf[n][j >> 1][(j & 1) * 2 + 1] = w[n];
         }
@@ -313,6 +316,12 @@ template <typename Q, typename KV, int D> struct PaTile {
     __device__ __forceinline__ void finish() {
 #pragma unroll
         for (int of = 1; of < 4; of <<= 1) { la += __shfl_xor_sync(0xffffffffu, la, of); lb += __shfl_xor_sync(0xffffffffu, lb, of); }
+        if constexpr (RAISE != 1.0f) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[c][e] *= 1.0f / RAISE;
+        }
     }
 };
 

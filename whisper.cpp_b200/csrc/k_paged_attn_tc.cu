@@ -11,7 +11,8 @@
 //   4 NTILE warps    softmax: a thread owns a row.  It reads its scores (tcgen05.ld), masks only blocks that some row does not see wholly,
 //                    and writes the weights back as P.  The reference point of the exponentials is the running maximum, but it follows it
 //                    only when the maximum has grown by more than 2^8: the weights stay below 256, the sums are exact in the same sense,
-//                    and the rescaling of O (a read and a write of tensor memory) is rare.  All exponentials go to the exponential unit:
+//                    and the rescaling of O (a read and a write of tensor memory) is rare.  f16 weights, which have all their bits only from
+//                    2^-14 on, are 2^11 at the reference point and follow from 2^4 on (PtLag).  All exponentials go to the exponential unit:
 //                    one of eight pairs as a polynomial on the FMA pipe made a chunk of 2048 over 16k keys slower (932 -> 966 us), one
 //                    of four more so (1004 us).
 //   1 warp           one thread issues all MMAs.  S_t(j+1) follows P_t V(j) in issue order, so the commit behind S_t(j+1) also says that
@@ -38,6 +39,11 @@ extern "C" int b200_paged_attn_status(void) {
     const cudaError_t e = cudaMemcpyFromSymbol(&v, g_pa_status, sizeof(v));
     return e == cudaSuccess ? v : (int) e;
 }
+
+// powers of two: how far the maximum may run ahead of the reference point, the weight at the reference point; and the factor that takes the latter out
+// (f16, 8 and 2^7 against 4 and 2^11: no difference in time on a chunk of 2048 over 16k keys, 16 times the step for the smallest weights)
+template <typename T> struct PtLag { static constexpr float lag = 8.0f, raise = 0.0f, lower = 1.0f; };
+template <> struct PtLag<__half> { static constexpr float lag = 4.0f, raise = 11.0f, lower = 1.0f / 2048.0f; };
 
 #define PT_THREADS(NTILE) (128 * (NTILE) + 96)
 
@@ -158,6 +164,7 @@ typedef unsigned long long pt_f2;                         // two floats for the 
 __device__ __forceinline__ pt_f2 pt_pair(float a, float b) { pt_f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ void pt_split(pt_f2 v, float & a, float & b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 __device__ __forceinline__ pt_f2 pt_mul2(pt_f2 a, pt_f2 b) { pt_f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ pt_f2 pt_fma2(pt_f2 a, pt_f2 b, pt_f2 c) { pt_f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 __device__ __forceinline__ pt_f2 pt_add2(pt_f2 a, pt_f2 b) { pt_f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 // any + 0 * every value of x
 template <typename T> __device__ __forceinline__ float pt_zero_times(uint4 x, float any) {
@@ -286,7 +293,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                         for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], fmaxf(__uint_as_float(y[i + u]), __uint_as_float(y[i + 4 + u])));
                 }
                 const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                const bool grow = (mx - m) * scale > 8.0f;                // also when there was no key so far; -inf - -inf is not
+                const bool grow = (mx - m) * scale > PtLag<T>::lag;                // also when there was no key so far; -inf - -inf is not
                 if (__any_sync(0xffffffffu, grow)) {
                     const float m1 = fmaxf(m, mx), f = m1 == -INFINITY ? 1.0f : pa_exp2((m - m1) * scale);
                     m = m1;
@@ -306,7 +313,7 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
                 // difference first: exact where it matters, whatever the scores' size.  s * scale - m in one operation is 1.6% faster, but off by
                 // the rounding of m, which is a large number where the scores are (1e36: infinite weights)
                 const float base = m == -INFINITY ? 0.0f : -m;
-                const pt_f2 scale2 = pt_pair(scale, scale), base2 = pt_pair(base, base);
+                const pt_f2 scale2 = pt_pair(scale, scale), base2 = pt_pair(base, base), raise2 = pt_pair(PtLag<T>::raise, PtLag<T>::raise);
                 pt_f2 l2[2] = { 0ull, 0ull };
 #pragma unroll
                 for (int c = 0; c < BN; c += 32) {
@@ -315,7 +322,8 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float y0, y1;
-                        pt_split(pt_mul2(pt_add2(pt_pair(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), base2), scale2), y0, y1);
+                        const pt_f2 d = pt_add2(pt_pair(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), base2);
+                        pt_split(PtLag<T>::raise == 0.0f ? pt_mul2(d, scale2) : pt_fma2(d, scale2, raise2), y0, y1);
                         y0 = pa_exp2(y0); y1 = pa_exp2(y1);
                         l2[i & 1] = pt_add2(l2[i & 1], pt_pair(y0, y1));
                         w[i] = pt_two<T>(y0, y1);
@@ -341,7 +349,8 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
         const int64_t out = (s.tok0 + tok) * a.n_head + head;
         const bool odd = n_blk[t] > 0 && *odd_flag;
         const bool whole = item.split < 0;
-        const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        l *= PtLag<T>::lower;
         char * dst = a.dst + (s.tok0 + tok) * a.nb_dst_tok + head * a.nb_dst_head;
         float * part = a.part + (item.slot * ROWS + t * 128 + r) * (D + 4);
 #pragma unroll 1
@@ -364,7 +373,11 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
             if (!valid) continue;
             if (!whole) {
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) *(uint4 *) (part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                for (int i = 0; i < 16; i += 4) {
+                    float4 x = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                    x.x *= PtLag<T>::lower; x.y *= PtLag<T>::lower; x.z *= PtLag<T>::lower; x.w *= PtLag<T>::lower;
+                    *(float4 *) (part + c + i) = x;
+                }
             } else {
                 uint32_t w[8];
 #pragma unroll

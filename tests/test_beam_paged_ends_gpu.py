@@ -48,3 +48,22 @@ def test_small_weights_beside_a_large_one(K, pkg, form, t, qt, lead):
     pool = x.c.view.clone()
     x.run()
     x.check(pool)
+
+
+@pytest.mark.parametrize("form", range(len(FORMS)))
+@pytest.mark.parametrize("t,qt", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16")])
+def test_infinite_values_far_below_the_largest_score(K, pkg, form, t, qt):
+    """A value that is attended to with a weight of exp(-200) leaves its dimension infinite or NaN, whichever warp, CTA or split has its key."""
+    seqs, Hkv, g, D, ps, at = FORMS[form]
+    x, y = (one_leader(K, pkg, seqs, Hkv, g, D, t, qt, ps, 200, at) for _ in range(2))
+    for i in range(len(seqs)):
+        x.c.view[1, 0, int(x.tables[i, 5 // ps]), 5 % ps, 0, 3] = float("inf")
+        x.c.view[1, 0, int(x.tables[i, 5 // ps]), 5 % ps, Hkv - 1, 4] = float("nan")
+    x.run()
+    y.run()
+    torch.cuda.synchronize()
+    out, want = x.out[:x.n_tok].clone(), y.out[:x.n_tok]
+    assert want.isfinite().all()
+    assert not out[:, :g, 3].isfinite().any() and out[:, -g:, 4].isnan().all()
+    out[:, :g, 3], out[:, -g:, 4] = want[:, :g, 3], want[:, -g:, 4]
+    assert torch.equal(out, want) and torch.equal(x.lse, y.lse)

@@ -505,10 +505,8 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
         for (int w = 0; w < WARPS; ++w) {
             const float f = pa_exp2(sm[w * PA_ROWS + r] - base);
             sum += f * sl[w * PA_ROWS + r];              // NaN of a warp without a finite maximum stays NaN
-            if (f != 0.0f) {
-                const float4 v = *(const float4 *) (so + (w * PA_ROWS + r) * LD + d);
-                x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w;
-            }
+            const float4 v = *(const float4 *) (so + (w * PA_ROWS + r) * LD + d);      // 0 * infinite is NaN, as it has to be
+            x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w;
         }
         const int tok = row / a.group, h = kvh * a.group + row % a.group;
         const int64_t out = (s.tok0 + tok) * a.n_head + h;
@@ -651,7 +649,7 @@ k_paged_join(const __grid_constant__ PaArgs a) {
             const float f = pa_exp2(p[D] - base);
             sum += f * p[D + 1];                          // NaN of a part without a finite maximum stays NaN
 #pragma unroll
-            for (int j = 0; j < DL; ++j) { const float v = p[lane * DL + j]; if (f != 0.0f) acc[j] += f * v; }
+            for (int j = 0; j < DL; ++j) acc[j] += f * p[lane * DL + j];
         }
         const int64_t out = (s.tok0 + t) * a.n_head + h;
 #pragma unroll
@@ -688,7 +686,7 @@ k_paged_join_tc(const __grid_constant__ PaArgs a) {
             const float f = pa_exp2(p[i * step + D] - base);
             sum += f * p[i * step + D + 1];               // NaN of a split without a finite maximum stays NaN
 #pragma unroll
-            for (int j = 0; j < DL; ++j) { const float v = p[i * step + lane * DL + j]; if (f != 0.0f) acc[j] += f * v; }
+            for (int j = 0; j < DL; ++j) acc[j] += f * p[i * step + lane * DL + j];
         }
         const int t = (row0 + r) / a.group, h = item.kvh * a.group + (row0 + r) % a.group;
         const int64_t out = (s.tok0 + t) * a.n_head + h;

@@ -268,8 +268,10 @@ int b200_topk_rows(const float * const * rows, b200_topk_result * const * out, i
  *   of a live beam b   every token v that is not banned:  score[b] + x[v] - max(x) - log(sum(exp(x - max(x))))
  *   of a done beam b   the one token eos, with score[b]
  * and the n_beam best become the new beams, best first, ties towards the lower b * n_vocab + v.  Banned tokens (bit v of word
- * v / 32; banned_stride words between the rows' masks, 0 = one mask for all) and NaN count as -inf logits; a candidate of
- * score -inf or NaN is none, and of a row whose score is that, or that is done, the logits do not matter.  The new beam is done when its parent
+ * v / 32; banned_stride words between the rows' masks, 0 = one mask for all) and NaN count as -inf logits; where a row has logits of +inf,
+ * they share it (-log of their number each) and its other tokens are none.  A candidate of
+ * score -inf or NaN is none, and of a row whose score is that, or that is done, the logits do not matter; with a score of +inf a row's candidates are equal.
+ * The new beam is done when its parent
  * was or its token is eos.  Where candidates run out: score -inf, token and parent -1, done 1.
  * score_out / done_out may be score / done.  n_beam <= B200_BEAM_MAX, n_beam * n_vocab < 2^31, n_beam * ceil(n_vocab / 8192) <= 32768, any
  * alignment of the rows that suits their type.  done, banned may be NULL. */

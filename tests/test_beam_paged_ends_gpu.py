@@ -67,3 +67,26 @@ def test_infinite_values_far_below_the_largest_score(K, pkg, form, t, qt):
     assert not out[:, :g, 3].isfinite().any() and out[:, -g:, 4].isnan().all()
     out[:, :g, 3], out[:, -g:, 4] = want[:, :g, 3], want[:, -g:, 4]
     assert torch.equal(out, want) and torch.equal(x.lse, y.lse)
+
+
+@pytest.mark.parametrize("V", [100, 9001, 51866])
+@pytest.mark.parametrize("n_beam", [1, 5, 32])
+def test_select_with_infinite_scores(K, pkg, V, n_beam):
+    """A score of +inf makes a row's candidates equal: the lowest tokens that are allowed and have a logit above -inf."""
+    rng = np.random.default_rng(V + n_beam)
+    x = rng.standard_normal((3 * n_beam, V)).astype(np.float32)
+    score = -rng.random(3 * n_beam).astype(np.float32)
+    score[0] = np.inf                                      # one row beside ordinary ones
+    score[n_beam:2 * n_beam] = np.inf                      # all of them, with logits that are none, and infinite ones
+    x[n_beam, :min(50, V // 2)] = -np.inf
+    x[n_beam, 3] = np.nan
+    x[2 * n_beam - 1, V - 1] = np.inf
+    score[2 * n_beam] = np.inf
+    done = np.zeros(3 * n_beam, np.uint8)
+    done[2 * n_beam] = 1
+    banned = rng.random((1, V)) < 0.3
+    for m in (None, banned):
+        s = Select(K, pkg, torch.from_numpy(x).cuda(), score, done, m, 7, n_beam, 1, 1)
+        s.run()
+        with np.errstate(all="ignore"):
+            check_select(s.got(), R.beam_select(x, score, done, m, 7, n_beam))

@@ -139,6 +139,12 @@ k_beam_scan(const char * logits, int64_t nb_row, int n_vocab, const float * scor
 #pragma unroll
             for (int i = 0; i < VEC; ++i) if (w[j] & (1u << i)) x[j][i] = -INFINITY;
     }
+    if (sc == INFINITY) {                        // the score of all of them: equal candidates, of which the lowest tokens count, not the largest logits
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) if (fabsf(x[j][i]) < INFINITY) x[j][i] = 0.0f;
+    }
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NV; ++j)

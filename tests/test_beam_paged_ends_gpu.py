@@ -90,3 +90,32 @@ def test_select_with_infinite_scores(K, pkg, V, n_beam):
         s.run()
         with np.errstate(all="ignore"):
             check_select(s.got(), R.beam_select(x, score, done, m, 7, n_beam))
+
+
+def test_steps_without_new_tokens(K, pkg):
+    """Captured steps of many rows whose sequences are all finished: nothing is stored or written, and what follows may change the tables at once."""
+    seqs = [(200, 260), (130, 130), (90, 400), (256, 300)]
+    x = Attn(K, pkg, np.random.default_rng(2), seqs, 20, 1, 64, "f16", "f16", 16)
+    first = x.c.view.clone()
+    pool = x.want_pool(first)
+    start, over = x.dstart.clone(), torch.zeros_like(x.dstart)
+    next_lens, lens = torch.zeros_like(x.dlen), x.dlen.clone()
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            x.dstart.copy_(over)
+            x.run()
+            x.dlen.copy_(next_lens)
+        for _ in range(20):
+            x.dlen.copy_(lens)
+            g.replay()
+            x.run()
+        st.synchronize()
+        assert torch.equal(torch.nan_to_num(x.c.view, 3.0), torch.nan_to_num(first, 3.0)) and (x.out == 7).all() and (x.lse == 7).all()
+        x.dlen.copy_(lens)
+        x.dstart.copy_(start)
+        x.run()
+    torch.cuda.synchronize()
+    x.check(pool)

@@ -450,15 +450,15 @@ static cudaError_t pg_launch(int64_t n_rows, int64_t width, int64_t n_pages, con
 // what update and compact ask of their states
 static bool pg_states_ok(const b200_page_state * from, const b200_page_state * to, int64_t n_pages, int64_t ps) {
     if (!from || !to || from->n_rows < 0 || from->n_rows > PG_MAX_ROWS || to->n_rows != from->n_rows) return false;
-    if (from->n_rows == 0) return from->refs && to->refs && from->refs != to->refs;
-    if (from->table_stride < 1 || to->table_stride != from->table_stride || !from->tables || !to->tables || !from->lens || !to->lens || !from->refs || !to->refs) return false;
+    auto apart = [](const void * a, int64_t na, const void * b, int64_t nb) { return (const char *) a + na <= (const char *) b || (const char *) b + nb <= (const char *) a; };
+    if (!from->refs || !to->refs || ((uintptr_t) from->refs | (uintptr_t) to->refs) % 4 || !apart(from->refs, 4 * n_pages, to->refs, 4 * n_pages)) return false;
+    if (from->n_rows == 0) return true;
+    if (from->table_stride < 1 || to->table_stride != from->table_stride || !from->tables || !to->tables || !from->lens || !to->lens) return false;
     const int64_t width = from->table_stride;
-    if (((uintptr_t) from->tables | (uintptr_t) from->lens | (uintptr_t) from->refs | (uintptr_t) to->tables | (uintptr_t) to->lens | (uintptr_t) to->refs) % 4) return false;
+    if (((uintptr_t) from->tables | (uintptr_t) from->lens | (uintptr_t) to->tables | (uintptr_t) to->lens) % 4) return false;
     if (width >= (1ll << 30)) return false;
     if (width * from->n_rows >= (1ll << 30) || width * ps >= (1ll << 31)) return false;
-    auto apart = [](const void * a, int64_t na, const void * b, int64_t nb) { return (const char *) a + na <= (const char *) b || (const char *) b + nb <= (const char *) a; };
-    return apart(from->tables, 4 * from->table_stride * from->n_rows, to->tables, 4 * to->table_stride * to->n_rows) &&
-           apart(from->lens, 4 * from->n_rows, to->lens, 4 * to->n_rows) && apart(from->refs, 4 * n_pages, to->refs, 4 * n_pages);
+    return apart(from->tables, 4 * from->table_stride * from->n_rows, to->tables, 4 * to->table_stride * to->n_rows) && apart(from->lens, 4 * from->n_rows, to->lens, 4 * to->n_rows);
 }
 
 extern "C" int64_t b200_pages_workspace(int64_t n_rows, int64_t n_pages) {

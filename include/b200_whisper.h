@@ -303,7 +303,7 @@ typedef struct {
 } b200_page_pool;
 /* Who uses the pages: row i (a sequence, or a beam of one) holds lens[i] tokens in pages tables[i * table_stride + 0 ..
  * ceil(lens[i] / page_size) - 1]; refs[p] counts the holders of page p over all rows (plus any holder of the caller's own),
- * 0 = free.  At most 8192 rows; table_stride * page_size < 2^31, table_stride * n_rows < 2^30. */
+ * 0 = free.  At most 8192 rows and 2^30 pages; table_stride * page_size < 2^31, table_stride * n_rows < 2^30. */
 typedef struct { int32_t * tables; int32_t * lens; int32_t * refs; int64_t n_rows, table_stride; } b200_page_state;
 int64_t b200_pages_workspace(int64_t n_rows, int64_t n_pages);
 

@@ -11,3 +11,15 @@ def test_pages_of_no_rows_refuse_bad_counts(K, pkg):
         f, t = (pkg.PageState(refs=r, n_rows=0) for r in (a, b))
         assert K.b200_pages_update(C.byref(pool(pkg)), C.byref(f), C.byref(t), None, None, None, P, P + 8192, n, None) == ERR, (a, b)
         assert K.b200_pages_compact(C.byref(pool(pkg)), C.byref(f), C.byref(t), P + 512, P, P + 8192, n, None) == ERR, (a, b)
+
+
+def test_pages_refuse_more_pages_than_they_can_number(K, pkg):
+    """Beyond 2^30 pages, 32-bit positions in the lists of pages would overflow."""
+    most = 1 << 30
+    assert K.b200_pages_workspace(1, most) > 0 and K.b200_pages_workspace(1, most + 1) == 0
+    for n_pages in (most + 1, (1 << 31) - 1):
+        f, t = (pkg.PageState(tables=P + i, lens=P + i + 256, refs=P + (i << 30), n_rows=1, table_stride=5) for i in (0, 1024))      # refused: nothing is read
+        tables_only = pool(pkg, k=None, v=None, n_pages=n_pages)
+        assert K.b200_pages_update(C.byref(tables_only), C.byref(f), C.byref(t), None, P, P, P, P + 8192, 1 << 60, None) == ERR
+        assert K.b200_pages_compact(C.byref(tables_only), C.byref(f), C.byref(t), P, P, P + 8192, 1 << 60, None) == ERR
+        assert K.b200_pages_copy(C.byref(pool(pkg, n_pages=n_pages)), 1, P + 8192, 1 << 60, None) == ERR

@@ -63,6 +63,7 @@ __device__ __forceinline__ void pg_copy(const b200_page_pool & pool, int n, int6
 #define PG_THREADS 1024
 #define PG_CLUSTER 16
 #define PG_MAX_ROWS 8192
+#define PG_MAX_PAGES (1 << 30)    // so that 3 words a copy (of at most half of them) and a thread's run of pages stay within 31 bits
 #define PG_SMALL   (160 * 1024)   // bytes of shared memory that a small state may take
 #define PG_FUSED   3000           // words of tables and counts up to which every CTA works them out for itself (5 beams, pages of 16, 8 layers of 20 heads; us
                                   // with and without: 1 sequence of 230 tokens 7.5, 9.1; 8 of 400 10.4, 11.4; 16 of 400 16.4, 15.7; 24 of 400 19.3, 17.5)
@@ -449,7 +450,7 @@ static cudaError_t pg_launch(int64_t n_rows, int64_t width, int64_t n_pages, con
 
 // what update and compact ask of their states
 static bool pg_states_ok(const b200_page_state * from, const b200_page_state * to, int64_t n_pages, int64_t ps) {
-    if (!from || !to || from->n_rows < 0 || from->n_rows > PG_MAX_ROWS || to->n_rows != from->n_rows) return false;
+    if (!from || !to || from->n_rows < 0 || from->n_rows > PG_MAX_ROWS || to->n_rows != from->n_rows || n_pages > PG_MAX_PAGES) return false;
     auto apart = [](const void * a, int64_t na, const void * b, int64_t nb) { return (const char *) a + na <= (const char *) b || (const char *) b + nb <= (const char *) a; };
     if (!from->refs || !to->refs || ((uintptr_t) from->refs | (uintptr_t) to->refs) % 4 || !apart(from->refs, 4 * n_pages, to->refs, 4 * n_pages)) return false;
     if (from->n_rows == 0) return true;
@@ -462,7 +463,7 @@ static bool pg_states_ok(const b200_page_state * from, const b200_page_state * t
 }
 
 extern "C" int64_t b200_pages_workspace(int64_t n_rows, int64_t n_pages) {
-    if (n_rows < 0 || n_rows > PG_MAX_ROWS || n_pages < 1 || n_pages > 0x7fffffff) return 0;
+    if (n_rows < 0 || n_rows > PG_MAX_ROWS || n_pages < 1 || n_pages > PG_MAX_PAGES) return 0;
     PgWork w;
     return pg_layout(&w, nullptr, n_rows, n_pages);
 }
@@ -505,7 +506,7 @@ extern "C" int b200_pages_compact(const b200_page_pool * pool, const b200_page_s
 }
 
 extern "C" int b200_pages_copy(const b200_page_pool * pool, int64_t n_rows, const void * workspace, int64_t workspace_bytes, void * stream) {
-    if (!b200_pool_ok(pool, true) || n_rows < 0 || n_rows > PG_MAX_ROWS) return B200_ERR_ARG;
+    if (!b200_pool_ok(pool, true) || n_rows < 0 || n_rows > PG_MAX_ROWS || pool->n_pages > PG_MAX_PAGES) return B200_ERR_ARG;
     if (!workspace || (uintptr_t) workspace % 16 || workspace_bytes < b200_pages_workspace(n_rows, pool->n_pages)) return B200_ERR_ARG;
     PgWork w;
     pg_layout(&w, (void *) workspace, n_rows, pool->n_pages);

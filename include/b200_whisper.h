@@ -348,8 +348,8 @@ int b200_pages_copy(const b200_page_pool * pool, int64_t n_rows, const void * wo
  * k_new / v_new (type of q, [n_tok][n_head_kv][head_dim] with strides nb_new_tok, nb_new_head) are first stored at their positions,
  * rounded to the pool's type; NULL (both) if the pages hold them already.  nb_* in bytes, multiples of 16, and 16-byte
  * aligned pointers.  max_new and max_len bound n_new and lens from above (device values beyond them, or beyond the tables, are cut
- * off); n_tok = q_start[n_seq].  Limits: n_seq 65535, n_head 4096, max_len 2^30 - 1, rows of a sequence (min(max_new, n_tok) * n_head / n_head_kv)
- * below 2^30.  A table entry outside the pool reads as keys and values of zero and stores nothing. */
+ * off); n_tok = q_start[n_seq].  Limits: n_seq 65535, n_head 4096, max_len 2^30 - 1, table_stride below 2^31, new tokens (min(max_new, n_tok)) and
+ * rows (that * n_head / n_head_kv) of a sequence below 2^30.  A table entry outside the pool reads as keys and values of zero and stores nothing. */
 typedef struct {
     const void * q; int q_type; int64_t nb_q_tok, nb_q_head;
     void * dst; int64_t nb_dst_tok, nb_dst_head;

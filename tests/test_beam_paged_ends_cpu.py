@@ -23,3 +23,16 @@ def test_pages_refuse_more_pages_than_they_can_number(K, pkg):
         assert K.b200_pages_update(C.byref(tables_only), C.byref(f), C.byref(t), None, P, P, P, P + 8192, 1 << 60, None) == ERR
         assert K.b200_pages_compact(C.byref(tables_only), C.byref(f), C.byref(t), P, P, P + 8192, 1 << 60, None) == ERR
         assert K.b200_pages_copy(C.byref(pool(pkg, n_pages=n_pages)), 1, P + 8192, 1 << 60, None) == ERR
+
+
+def test_attention_and_store_refuse_what_overflows(K, pkg):
+    """2^30 new tokens of one sequence and more (the store alone has no heads to count rows by), and rows of tables that no state can have."""
+    pl = pool(pkg)
+    ok = dict(q=P, q_type=1, nb_q_tok=512, nb_q_head=128, dst=P, nb_dst_tok=512, nb_dst_head=128, k_new=P, v_new=P, nb_new_tok=0, nb_new_head=128, layer=0, tables=P, table_stride=5, lens=P,
+              q_start=P, n_tok=4, n_seq=1, n_head=4, max_new=2, max_len=20, causal=1, scale=0.1, workspace=P, workspace_bytes=1 << 60)
+    for n in (1 << 30, (1 << 31) - 1):
+        a = changed(pkg.PagedAttnArgs, ok, n_tok=n, max_new=n)
+        assert K.b200_paged_store(C.byref(pl), C.byref(a), None) == ERR
+    for stride in (1 << 31, 1 << 62):
+        a = changed(pkg.PagedAttnArgs, ok, table_stride=stride)
+        assert K.b200_paged_store(C.byref(pl), C.byref(a), None) == ERR and K.b200_paged_attn(C.byref(pl), C.byref(a), None) == ERR

@@ -703,6 +703,7 @@ static bool pa_args_ok(const b200_page_pool * p, const b200_paged_attn_args * a,
     if (a->n_seq < 0 || a->n_seq > 65535 || a->n_tok < 0 || a->n_tok > 0x7fffffff || a->max_new < 0 || a->max_len < 0 || a->max_len >= (1ll << 30)) return false;
     if (a->q_type != B200_TYPE_F32 && a->q_type != p->type) return false;
     if (a->n_seq == 0 || a->n_tok == 0 || a->max_new == 0) return true;
+    if ((a->max_new < a->n_tok ? a->max_new : a->n_tok) >= (1ll << 30) || a->table_stride >= (1ll << 31)) return false;      // positions are 32 bits
     if (!a->tables || a->table_stride < 1 || !a->lens || !a->q_start || ((uintptr_t) a->tables | (uintptr_t) a->lens | (uintptr_t) a->q_start | (uintptr_t) a->lse) % 4) return false;
     if (!a->k_new != !a->v_new || (!attn && !a->k_new)) return false;
     const int64_t size = a->q_type == B200_TYPE_F32 ? 4 : 2, row = size * p->head_dim;

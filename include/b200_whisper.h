@@ -316,8 +316,8 @@ int64_t b200_pages_workspace(int64_t n_rows, int64_t n_pages);
  * pages that become free here can be taken by the next call.  Table entries behind a row's last page are set to -1.
  * parent NULL: every row is its own parent.  pool NULL: tables only; b200_pages_copy then makes the copies, for as many
  * pools as the caller has (n_pages and page_size are needed, so they come with pool: pass k = v = NULL for tables only).
- * status[0] (device): 0; the number of pages that are missing; or -1 (a parent, keep, n_new or table entry out of range: a
- * row cannot keep more than its parent holds, nor grow beyond table_stride pages).  If it is not 0, `to` is a copy of `from` and
+ * status[0] (device): 0; the number of pages that are missing; or -1 (a parent, keep, n_new or table entry out of range, or
+ * a used entry on a free page: a row cannot keep more than its parent holds, nor grow beyond table_stride pages).  If it is not 0, `to` is a copy of `from` and
  * nothing else happened.  status[1]: pages copied. */
 int b200_pages_update(const b200_page_pool * pool, const b200_page_state * from, const b200_page_state * to, const int32_t * parent,
                       const int32_t * keep, const int32_t * n_new, int32_t * status, void * workspace, int64_t workspace_bytes, void * stream);

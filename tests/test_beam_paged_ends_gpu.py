@@ -119,3 +119,23 @@ def test_steps_without_new_tokens(K, pkg):
         x.run()
     torch.cuda.synchronize()
     x.check(pool)
+
+
+@pytest.mark.parametrize("rows,n_pages", [(3, 12), (300, 40000)])
+def test_update_refuses_entries_on_free_pages(K, pkg, rows, n_pages):
+    """A used entry on a page that nobody holds would be handed out as new."""
+    rng = np.random.default_rng(rows)
+    c = Cache(pkg, rng, n_pages, 4, Hkv=1)
+    tables = np.full((rows, 4), -1)
+    tables[:, :2] = rng.permutation(n_pages)[:2 * rows].reshape(rows, 2)
+    lens, before = np.full(rows, 7), c.view.clone()
+    refs = np.bincount(tables[:, :2].ravel(), minlength=n_pages)
+    for row, keep in ((0, 7), (rows - 1, 0), (rows // 2, 7)):
+        free = refs.copy()
+        free[tables[row, 1]] = 0
+        k = lens.copy()
+        k[row] = keep
+        got, status, _ = run_update(K, pkg, c, tables, lens, free, None, k, np.ones(rows, int))
+        check_update(c, before, got, status, (tables, lens, free, [], -1))
+    got, status, _ = run_update(K, pkg, c, tables, lens, refs, None, lens, np.ones(rows, int))
+    check_update(c, before, got, status, R.pages_update(tables, lens, refs, np.arange(rows), lens, np.ones(rows, int), 4))

@@ -194,7 +194,11 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
     }
     pg_sync<SMALL>(cl);
     // 2. old holders out, new ones in (what both have in the same column cancels); first writer and number of writers of a page.  Every entry
-    // that is used has to be a page; where one is not, `to` is made a copy of `from` in the end
+    // that is used has to be a page that is held (a free one would be given away as new); where one is not, `to` is made a copy of `from` in the end.
+    // The counts are looked at one batch later, when they are there (64 x 5 rows of 259 pages: 20.7 us without, 22.0 at once, 21.7 so)
+    int r[PG_BATCH];
+#pragma unroll
+    for (int x = 0; x < PG_BATCH; ++x) r[x] = 1;
     for (int c0 = gtid; c0 < cells; c0 += PG_BATCH * all) {
         int o[PG_BATCH], n[PG_BATCH];
 #pragma unroll
@@ -204,6 +208,11 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
             o[x] = in && j < s_old[i] ? tables[c] : -1;
             n[x] = in && j < s_kept[i] ? tables[s_par[i] * width + j] : -1;
             if (in && j < s_old[i] && (o[x] < 0 || o[x] >= n_pages)) { sh.err = 1; o[x] = -1; }
+        }
+#pragma unroll
+        for (int x = 0; x < PG_BATCH; ++x) {
+            if (r[x] == 0) sh.err = 1;
+            r[x] = o[x] >= 0 ? refs[o[x]] : 1;
         }
 #pragma unroll
         for (int x = 0; x < PG_BATCH; ++x) if (o[x] != n[x]) {
@@ -217,6 +226,8 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
         s_page[i] = s;
         if (i % n_cta == me && s >= 0 && s < n_pages) { atomicMin(&w.a[s], i); atomicAdd(&w.b[s], 1); }
     }
+#pragma unroll
+    for (int x = 0; x < PG_BATCH; ++x) if (r[x] == 0) sh.err = 1;
     int n_free, err;
     pg_across<SMALL>(cl, sh, &my_free, &n_free, &err);
     free_before += my_free;

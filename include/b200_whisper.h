@@ -348,8 +348,12 @@ int b200_pages_copy(const b200_page_pool * pool, int64_t n_rows, const void * wo
  * k_new / v_new (type of q, [n_tok][n_head_kv][head_dim] with strides nb_new_tok, nb_new_head) are first stored at their positions,
  * rounded to the pool's type; NULL (both) if the pages hold them already.  nb_* in bytes, multiples of 16, and 16-byte
  * aligned pointers.  max_new and max_len bound n_new and lens from above (device values beyond them, or beyond the tables, are cut
- * off); n_tok = q_start[n_seq].  Limits: n_seq 65535, n_head 4096, max_len 2^30 - 1, table_stride below 2^31, new tokens (min(max_new, n_tok)) and
- * rows (that * n_head / n_head_kv) of a sequence below 2^30.  A table entry outside the pool reads as keys and values of zero and stores nothing. */
+ * off, and the new tokens then replace the last ones below the cut); n_tok = q_start[n_seq].  Limits: n_seq 65535, n_head 4096, max_len 2^30 - 1, table_stride below 2^31, new tokens (min(max_new, n_tok)) and
+ * rows (that * n_head / n_head_kv) of a sequence below 2^30.  A table entry outside the pool reads as keys and values of zero and stores nothing.
+ * status (device, may be NULL): that of the b200_pages_update that made the state.  Where status[0] is not 0 there is no room for the new tokens - the state
+ * is the old one, and its last tokens would be taken for them - so that nothing is stored and no row of dst and lse written.  Without it the status
+ * has to be looked at before any attention or store with k_new.  For the same reason q_start has to give a sequence as many tokens as the update's n_new did
+ * (none where that was 0). */
 typedef struct {
     const void * q; int q_type; int64_t nb_q_tok, nb_q_head;
     void * dst; int64_t nb_dst_tok, nb_dst_head;
@@ -359,13 +363,14 @@ typedef struct {
     int64_t n_tok; int n_seq, n_head; int64_t max_new, max_len; int causal; float scale;
     float * lse;
     void * workspace; int64_t workspace_bytes;
+    const int32_t * status;
 } b200_paged_attn_args;
 int64_t b200_paged_attn_workspace(const b200_page_pool * pool, const b200_paged_attn_args * a);
 int b200_paged_attn(const b200_page_pool * pool, const b200_paged_attn_args * a, void * stream);
 /* 0, or the code of a device-side wait that ran out in an earlier launch (which then left its rows unfinished); synchronises. */
 int b200_paged_attn_status(void);
 /* The store alone (prompts whose attention runs elsewhere, caches filled from another source); uses of *a: k_new .. q_start,
- * n_tok, n_seq, max_new, max_len, and q_type as the type of k_new / v_new. */
+ * n_tok, n_seq, max_new, max_len, status, and q_type as the type of k_new / v_new. */
 int b200_paged_store(const b200_page_pool * pool, const b200_paged_attn_args * a, void * stream);
 
 /* IM2COL 1-D, F16 output (ops.cpp:5784-5855): x f32 [IW, IC] (row stride bytes) ->

@@ -36,3 +36,10 @@ def test_attention_and_store_refuse_what_overflows(K, pkg):
     for stride in (1 << 31, 1 << 62):
         a = changed(pkg.PagedAttnArgs, ok, table_stride=stride)
         assert K.b200_paged_store(C.byref(pl), C.byref(a), None) == ERR and K.b200_paged_attn(C.byref(pl), C.byref(a), None) == ERR
+
+
+def test_attention_and_store_refuse_an_unaligned_status(K, pkg):
+    ok = dict(q=P, q_type=1, nb_q_tok=512, nb_q_head=128, dst=P, nb_dst_tok=512, nb_dst_head=128, k_new=P, v_new=P, nb_new_tok=256, nb_new_head=128, layer=0, tables=P, table_stride=5, lens=P,
+              q_start=P, n_tok=4, n_seq=2, n_head=4, max_new=2, max_len=20, causal=1, scale=0.1, workspace=P, workspace_bytes=1 << 15, status=P + 2)
+    for f in (K.b200_paged_attn, K.b200_paged_store):
+        assert f(C.byref(pool(pkg)), C.byref(changed(pkg.PagedAttnArgs, ok)), None) == ERR

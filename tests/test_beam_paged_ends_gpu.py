@@ -139,3 +139,64 @@ def test_update_refuses_entries_on_free_pages(K, pkg, rows, n_pages):
         check_update(c, before, got, status, (tables, lens, free, [], -1))
     got, status, _ = run_update(K, pkg, c, tables, lens, refs, None, lens, np.ones(rows, int))
     check_update(c, before, got, status, R.pages_update(tables, lens, refs, np.arange(rows), lens, np.ones(rows, int), 4))
+
+
+@pytest.mark.parametrize("n_new,rows,heads,qt,t", [(1, 5, 4, "f16", "f16"), (1, 5, 4, "f32", "bf16"), (1, 300, 4, "bf16", "bf16"), (60, 4, 2, "f32", "f16"), (200, 5, 20, "f16", "f16"),
+                                                   (200, 5, 20, "f32", "f16")])
+def test_a_step_that_ran_out_of_pages_changes_no_page(K, pkg, n_new, rows, heads, qt, t):
+    """The update leaves a copy of the state; attention and store with its status do nothing, so that the rows' last tokens stay what they were.
+    With pages enough the same calls store and attend."""
+    rng = np.random.default_rng(n_new)
+    ps, D, n = 16, 64, 300
+    used, more = R.ceil(n, ps), R.ceil(n + n_new, ps) - R.ceil(n, ps)
+    width = used + more + 1
+    for short in (True, False):
+        n_pages = rows * (used + more) + (rows if more == 0 else -int(short))
+        c = Cache(pkg, rng, n_pages, ps, heads, D, t)
+        tables = np.full((rows, width), -1)
+        tables[:, :used] = rng.permutation(n_pages)[:rows * used].reshape(rows, used)
+        refs = np.bincount(tables[tables >= 0], minlength=n_pages)
+        if short and more == 0:
+            refs[refs == 0] = 1
+            refs[tables[0, used - 1]] += 1                 # a holder besides: row 0 has to copy its last page, and none is free
+        lens = np.full(rows, n)
+        keep, new = lens.copy(), np.full(rows, n_new)
+        frm, f = c.state(pkg, tables, lens, refs)
+        to, s = c.state(pkg, np.zeros_like(tables), np.zeros_like(lens), np.zeros_like(refs))
+        status = torch.full((2,), 55, dtype=torch.int32, device="cuda")
+        m = K.b200_pages_workspace(rows, n_pages)
+        ws = torch.empty(m, dtype=torch.uint8, device="cuda")
+        dt = dict(f16=torch.float16, bf16=torch.bfloat16, f32=torch.float32)[qt]
+        q, kn, vn = (torch.from_numpy(rng.standard_normal((rows * n_new, heads, D))).to(dt).cuda() for _ in range(3))
+        out, lse = torch.full_like(q, 7.0), torch.full((rows * n_new, heads), 7.0, device="cuda")
+        start, es = dev(np.arange(rows + 1) * n_new, np.int32), q.element_size()
+        kd, nd = dev(keep, np.int32), dev(new, np.int32)
+        a = pkg.PagedAttnArgs(q=p(q), q_type=dict(f32=0, f16=1, bf16=30)[qt], nb_q_tok=heads * D * es, nb_q_head=D * es, dst=p(out), nb_dst_tok=heads * D * es, nb_dst_head=D * es,
+                              k_new=p(kn), v_new=p(vn), nb_new_tok=heads * D * es, nb_new_head=D * es, layer=0, tables=p(to["tables"]), table_stride=width, lens=p(to["lens"]),
+                              q_start=p(start), n_tok=rows * n_new, n_seq=rows, n_head=heads, max_new=n_new, max_len=n + n_new, causal=1, scale=0.125, lse=p(lse), status=p(status))
+        w = K.b200_paged_attn_workspace(C.byref(c.pool), C.byref(a))
+        aws = torch.empty(max(w, 16), dtype=torch.uint8, device="cuda")
+        a.workspace, a.workspace_bytes = p(aws), w
+        before = c.view.clone()
+        st = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):           # nothing between them looks at the status on the host
+                assert K.b200_pages_update(C.byref(c.pool), C.byref(f), C.byref(s), None, p(kd), p(nd), p(status), p(ws), m, stream()) == 0
+                assert K.b200_paged_store(C.byref(c.pool), C.byref(a), stream()) == 0
+                assert K.b200_paged_attn(C.byref(c.pool), C.byref(a), stream()) == 0
+            g.replay()
+            st.synchronize()
+        if short:
+            assert status.tolist() == [1, 0] and torch.equal(c.view, before)
+            assert (out == 7).all() and (lse == 7).all()
+            continue
+        assert status.tolist()[0] == 0
+        table = to["tables"].cpu().numpy()
+        for i in range(rows):
+            for j, x in enumerate((kn, vn)):
+                pos = n + np.arange(n_new)
+                assert torch.equal(c.view[j, 0][torch.from_numpy(table[i, pos // ps]).long().cuda(), torch.from_numpy(pos % ps).cuda()],
+                                   x[i * n_new:(i + 1) * n_new].to(c.view.dtype))
+        assert not (out == 7).all() and lse.isfinite().all() and not (lse == 7).any()

@@ -42,7 +42,9 @@ __global__ void __launch_bounds__(256)
 k_paged_store(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew x, int log_vec) {
     chain_wait();                                         // in this order: once all CTAs have released, all that came before this launch is there,
     chain_release();                                      // and the attention behind it may read its queries and tables at once (32 ragged prompts: 36.1 -> 34.2 us)
+    const int failed = pa_failed(a);
     const PaSeq s = pa_seq(a, blockIdx.y);
+    if (failed) return;
     const int lane = threadIdx.x & 31, per_tok = 2 * a.n_head_kv << log_vec, mask = (1 << log_vec) - 1;
     for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < s.n_new; t += gridDim.x * 8) {
         const int pos = s.len - s.n_new + t;
@@ -379,11 +381,12 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // the shuffle tells the compiler that the warp agrees
     int seq, kvh, tile, at = 0;                           // the item, and where in it (on the line) this CTA begins
     int64_t todo = 1ll << 60;                             // what is left of this CTA's part
+    const int failed = pa_failed(a);
     if (a.stream) {
         int64_t rest;
         const PaLine l = pa_line(a, ROUND, blockIdx.x, -1, &seq, &rest);
         todo = ((int64_t) blockIdx.x + 1) * l.total / a.stream - (int64_t) blockIdx.x * l.total / a.stream;
-        if (seq >= a.n_seq || todo == 0) return;
+        if (seq >= a.n_seq || todo == 0 || failed) return;
         const PaSeq s = pa_seq(a, seq);
         const int rounds = max(1, (s.len + ROUND - 1) / ROUND), tiles = (s.n_new * a.group + PA_ROWS - 1) / PA_ROWS;
         const int64_t item = rest / (rounds + PA_START);
@@ -394,7 +397,7 @@ k_paged_attn(const __grid_constant__ PaArgs a, const __grid_constant__ PaNew nw)
     for (;;) {
     const PaSeq s = pa_seq(a, seq);
     const int n_rows = s.n_new * a.group, row0 = tile * PA_ROWS;
-    if (!a.stream && row0 >= n_rows) return;
+    if (!a.stream && (row0 >= n_rows || failed)) return;
     const int rounds = max(1, (s.len + ROUND - 1) / ROUND), steps = (int) min((int64_t) (rounds + PA_START - at), todo);
     const int first_round = max(0, at - PA_START), n_round = max(0, at + steps - PA_START) - first_round;
     const int k0 = first_round * ROUND, k1 = min(pa_reach(a, s, row0), k0 + n_round * ROUND);
@@ -553,9 +556,10 @@ k_paged_attn_wide(const __grid_constant__ PaArgs a) {
     chain_wait();                                         // no early release, as above
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int seq = blockIdx.z, kvh = blockIdx.y, tile = gridDim.x - 1 - blockIdx.x;      // the longest tiles first
+    const int failed = pa_failed(a);
     const PaSeq s = pa_seq(a, seq);
     const int n_rows = s.n_new * a.group, row0 = tile * ROWS, mine = row0 + warp * PA_ROWS;
-    if (row0 >= n_rows) return;
+    if (row0 >= n_rows || failed) return;
     auto reach = [&](int r1) { return a.causal ? min(s.len, max(s.len - s.n_new + (min(r1, n_rows) - 1) / a.group + 1, 0)) : s.len; };
     const int k1 = reach(row0 + ROWS), my_k1 = mine < n_rows ? reach(mine + PA_ROWS) : 0, n_stage = (k1 + STAGE - 1) / STAGE;
     const char * kp = a.k + kvh * a.nb_head, * vp = a.v + kvh * a.nb_head;
@@ -623,9 +627,9 @@ k_paged_join(const __grid_constant__ PaArgs a) {
     constexpr int DL = D / 32, ROUND = PA_BLOCK / (2 * D) * PA_WARPS;
     chain_release();
     chain_wait();
-    const int lane = threadIdx.x & 31, seq = blockIdx.y;
+    const int lane = threadIdx.x & 31, seq = blockIdx.y, failed = pa_failed(a);
     const PaSeq s = pa_seq(a, seq);
-    if (s.n_new == 0) return;
+    if (s.n_new == 0 || failed) return;
     const PaLine l = pa_line(a, ROUND, 0, seq, nullptr, nullptr);
     const int rounds = max(1, (s.len + ROUND - 1) / ROUND), tiles = (s.n_new * a.group + PA_ROWS - 1) / PA_ROWS;
     for (int64_t w = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 5); w < (int64_t) s.n_new * a.n_head; w += (int64_t) gridDim.x * 4) {
@@ -666,11 +670,11 @@ k_paged_join_tc(const __grid_constant__ PaArgs a) {
     chain_release();
     chain_wait();
     constexpr int DL = D / 32;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, failed = pa_failed(a);
     const PaItem item = pa_item(a, a.n_whole + blockIdx.x * a.n_split);
     const PaSeq s = pa_seq(a, item.seq);
     const int row0 = item.tile * a.tile_rows, rows = min(a.tile_rows, s.n_new * a.group - row0);
-    if (rows <= 0) return;
+    if (rows <= 0 || failed) return;
     const int n = min(a.n_split, max(1, (pa_reach(a, s, row0) + a.chunk - 1) / a.chunk));
     const int64_t step = (int64_t) a.tile_rows * (D + 4);
     for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 4) {
@@ -704,7 +708,7 @@ static bool pa_args_ok(const b200_page_pool * p, const b200_paged_attn_args * a,
     if (a->q_type != B200_TYPE_F32 && a->q_type != p->type) return false;
     if (a->n_seq == 0 || a->n_tok == 0 || a->max_new == 0) return true;
     if ((a->max_new < a->n_tok ? a->max_new : a->n_tok) >= (1ll << 30) || a->table_stride >= (1ll << 31)) return false;      // positions are 32 bits
-    if (!a->tables || a->table_stride < 1 || !a->lens || !a->q_start || ((uintptr_t) a->tables | (uintptr_t) a->lens | (uintptr_t) a->q_start | (uintptr_t) a->lse) % 4) return false;
+    if (!a->tables || a->table_stride < 1 || !a->lens || !a->q_start || ((uintptr_t) a->tables | (uintptr_t) a->lens | (uintptr_t) a->q_start | (uintptr_t) a->lse | (uintptr_t) a->status) % 4) return false;
     if (!a->k_new != !a->v_new || (!attn && !a->k_new)) return false;
     const int64_t size = a->q_type == B200_TYPE_F32 ? 4 : 2, row = size * p->head_dim;
     if (a->k_new && (((uintptr_t) a->k_new | (uintptr_t) a->v_new | (uintptr_t) a->nb_new_tok | (uintptr_t) a->nb_new_head) % 16 ||
@@ -778,7 +782,7 @@ static PaArgs pa_pack(const b200_page_pool * p, const b200_paged_attn_args * a) 
     k.dst = (char *) a->dst; k.nb_dst_tok = a->nb_dst_tok; k.nb_dst_head = a->nb_dst_head;
     k.k = (const char *) p->k + a->layer * p->nb_layer; k.v = (const char *) p->v + a->layer * p->nb_layer;
     k.nb_page = p->nb_page; k.nb_tok = p->nb_tok; k.nb_head = p->nb_head;
-    k.tables = a->tables; k.table_stride = a->table_stride; k.lens = a->lens; k.q_start = a->q_start;
+    k.tables = a->tables; k.table_stride = a->table_stride; k.lens = a->lens; k.q_start = a->q_start; k.status = a->status;
     k.lse = a->lse; k.part = (float *) a->workspace; k.n_tok = a->n_tok; k.max_len = a->max_len;
     k.n_pages = p->n_pages; k.page_size = p->page_size; k.n_head = a->n_head; k.n_head_kv = p->n_head_kv;
     k.group = a->n_head / p->n_head_kv; k.causal = a->causal != 0;

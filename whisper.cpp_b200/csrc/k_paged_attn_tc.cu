@@ -197,12 +197,13 @@ k_paged_attn_tc(const __grid_constant__ PaArgs a, const __grid_constant__ PtMaps
     if (!a.early) chain_wait();                           // behind the store of the same call: only what reads its pages waits (below). No early
                                                           // release: this kernel wants whole SMs
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // the shuffle tells the compiler that the warp agrees
+    const int failed = pa_failed(a);
     const PaItem item = pa_item(a, blockIdx.x);
     const int seq = item.seq, split = max(item.split, 0), kvh = item.kvh, row0 = item.tile * ROWS, chunk = item.split < 0 ? 1 << 30 : a.chunk;
     const PaSeq s = pa_seq(a, seq);
     const int n_rows = s.n_new * a.group;
     const int k0 = split * chunk, k1 = row0 < n_rows ? min(pa_reach(a, s, row0), k0 + chunk) : 0;
-    if (row0 >= n_rows || (k0 >= k1 && split != 0)) {    // no rows, or an empty split, which the join does not read
+    if (row0 >= n_rows || failed || (k0 >= k1 && split != 0)) {      // no rows, or an empty split, which the join does not read
         // What follows waits for this launch only, which therefore must not end before the store, not even where no sequence has a new token.  One
         // CTA sees to that: with all of those that have no rows, ragged prompts took 35.3 us instead of 34.4.
         if (a.early && blockIdx.x == 0) chain_wait();

@@ -57,7 +57,7 @@ class PagedAttnArgs(C.Structure):
                 ("k_new", C.c_void_p), ("v_new", C.c_void_p), ("nb_new_tok", C.c_int64), ("nb_new_head", C.c_int64), ("layer", C.c_int),
                 ("tables", C.c_void_p), ("table_stride", C.c_int64), ("lens", C.c_void_p), ("q_start", C.c_void_p),
                 ("n_tok", C.c_int64), ("n_seq", C.c_int), ("n_head", C.c_int), ("max_new", C.c_int64), ("max_len", C.c_int64),
-                ("causal", C.c_int), ("scale", C.c_float), ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+                ("causal", C.c_int), ("scale", C.c_float), ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("status", C.c_void_p)]
 
 
 def kernels_lib() -> C.CDLL:

@@ -272,7 +272,9 @@ int b200_topk_rows(const float * const * rows, b200_topk_result * const * out, i
  * they share it (-log of their number each) and its other tokens are none.  A candidate of
  * score -inf or NaN is none, and of a row whose score is that, or that is done, the logits do not matter; with a score of +inf a row's candidates are equal.
  * The new beam is done when its parent
- * was or its token is eos.  Where candidates run out: score -inf, token and parent -1, done 1.
+ * was or its token is eos.  Where candidates run out: score -inf, token and parent -1, done 1
+ * (b200_beam_reorder leaves such a beam as it is; for b200_pages_update, which counts rows over all sequences, it is row_parent = the row itself with
+ * keep = n_new = 0, and never sequence * n_beam - 1, the row before the sequence).
  * score_out / done_out may be score / done.  n_beam <= B200_BEAM_MAX, n_beam * n_vocab < 2^31, n_beam * ceil(n_vocab / 8192) <= 32768, any
  * alignment of the rows that suits their type.  done, banned may be NULL. */
 #define B200_BEAM_MAX 32

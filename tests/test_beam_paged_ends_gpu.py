@@ -200,3 +200,44 @@ def test_a_step_that_ran_out_of_pages_changes_no_page(K, pkg, n_new, rows, heads
                 assert torch.equal(c.view[j, 0][torch.from_numpy(table[i, pos // ps]).long().cuda(), torch.from_numpy(pos % ps).cuda()],
                                    x[i * n_new:(i + 1) * n_new].to(c.view.dtype))
         assert not (out == 7).all() and lse.isfinite().all() and not (lse == 7).any()
+
+
+def test_beams_that_run_out_of_candidates(K, pkg):
+    """A step over several sequences in which the second has fewer candidates than beams: the beams without one (parent -1) give their pages back, take
+    nothing from another sequence, and come back when a later selection gives them a parent."""
+    rng = np.random.default_rng(4)
+    n_seq, nb, V, ps, width, n_pages = 3, 4, 50, 4, 6, 80
+    rows = n_seq * nb
+    c = Cache(pkg, rng, n_pages, ps, Hkv=1)
+    tables = np.full((rows, width), -1)
+    tables[:, :3] = rng.permutation(n_pages)[:rows * 3].reshape(rows, 3)
+    lens = np.repeat([9, 10, 11], nb)
+    refs = np.bincount(tables[tables >= 0], minlength=n_pages)
+    score = -rng.random(rows).astype(np.float32)
+    x = rng.standard_normal((2, rows, V)).astype(np.float32)
+    x[0, nb:2 * nb] = -np.inf
+    x[0, nb + 2, 5] = 1.0                                  # one candidate in the second sequence
+    score[0:nb] = -np.inf                                  # and none at all in the first
+    done = np.zeros(rows, np.uint8)
+    for step in range(2):
+        s = Select(K, pkg, torch.from_numpy(x[step]).cuda(), score, done, None, 3, nb)
+        s.run()
+        got = s.got()
+        check_select(got, R.beam_select(x[step], score, done, None, 3, nb))
+        parent, score, done = got["parent"], got["score"], got["done"]
+        own, none = np.arange(rows), parent < 0
+        row_parent = np.where(none, own, own // nb * nb + parent)
+        keep = np.where(none, 0, lens[row_parent])
+        new = np.where(none | (done != 0), 0, 1)
+        before = c.view.clone()
+        want = R.pages_update(tables, lens, refs, row_parent, keep, new, ps)
+        up, status, _ = run_update(K, pkg, c, tables, lens, refs, row_parent, keep, new)
+        assert status[0] == 0
+        check_update(c, before, up, status, want)
+        old = {i // nb: set(tables[i // nb * nb:(i // nb + 1) * nb].ravel()) for i in range(rows)}
+        for i in range(rows):
+            other = set().union(*(old[q] for q in old if q != i // nb)) - {-1}
+            assert not other & set(up["tables"][i])
+        assert (up["lens"][none] == 0).all() and (up["tables"][none] == -1).all()
+        tables, lens, refs = (up[k].astype(int) for k in ("tables", "lens", "refs"))
+    assert none[:nb].all() and (refs == np.bincount(tables[tables >= 0], minlength=n_pages)).all()

@@ -369,7 +369,9 @@ typedef struct {
 } b200_paged_attn_args;
 int64_t b200_paged_attn_workspace(const b200_page_pool * pool, const b200_paged_attn_args * a);
 int b200_paged_attn(const b200_page_pool * pool, const b200_paged_attn_args * a, void * stream);
-/* 0, or the code of a device-side wait that ran out in an earlier launch (which then left its rows unfinished); synchronises. */
+/* 0, or the code of the first device-side wait that ran out on the current device since the code was last asked for (its launch left rows unfinished, although
+ * the call had returned 0).  Waits for all work on the device; not while a stream is being captured.  With launches by several threads the code does not
+ * tell whose it was. */
 int b200_paged_attn_status(void);
 /* The store alone (prompts whose attention runs elsewhere, caches filled from another source); uses of *a: k_new .. q_start,
  * n_tok, n_seq, max_new, max_len, status, and q_type as the type of k_new / v_new. */

@@ -241,3 +241,14 @@ def test_beams_that_run_out_of_candidates(K, pkg):
         assert (up["lens"][none] == 0).all() and (up["tables"][none] == -1).all()
         tables, lens, refs = (up[k].astype(int) for k in ("tables", "lens", "refs"))
     assert none[:nb].all() and (refs == np.bincount(tables[tables >= 0], minlength=n_pages)).all()
+
+
+def test_the_wait_status_waits_for_every_stream(K, pkg):
+    """Streams that do not wait for the default stream are waited for as well."""
+    st = torch.cuda.Stream()
+    x = Attn(K, pkg, np.random.default_rng(0), [(300, 400)], 1, 1, 128, "f16", "f16", 16)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        torch.cuda._sleep(200_000_000)                     # about a tenth of a second
+        x.run()
+    assert K.b200_paged_attn_status() == 0 and st.query()

@@ -35,8 +35,11 @@
 __device__ int g_pa_status;
 
 extern "C" int b200_paged_attn_status(void) {
+    static const int none = 0;
     int v = 0;
-    const cudaError_t e = cudaMemcpyFromSymbol(&v, g_pa_status, sizeof(v));
+    cudaError_t e = cudaDeviceSynchronize();              // all streams: those that do not wait for the default stream as well
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_pa_status, sizeof(v));
+    if (e == cudaSuccess && v != 0) e = cudaMemcpyToSymbol(g_pa_status, &none, sizeof(none));
     return e == cudaSuccess ? v : (int) e;
 }
 

@@ -82,6 +82,7 @@ def kernels_lib() -> C.CDLL:
         lib.b200_paged_attn_workspace.argtypes = [pool, attn]
         lib.b200_paged_attn.argtypes = [pool, attn, vp]
         lib.b200_paged_store.argtypes = [pool, attn, vp]
+        lib.b200_paged_attn_status.argtypes = []
         for f in ("b200_beam_select_workspace", "b200_pages_workspace", "b200_paged_attn_workspace"):
             getattr(lib, f).restype = i64
         _kernels = lib

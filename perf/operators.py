@@ -256,7 +256,7 @@ def _handle(s):
     """The argument blocks, workspaces and output buffers that a decoding program sets up once and uses at every step."""
     P, c, op = _package(), s["case"], s["case"]["op"]
     lib, types = P.kernels_lib(), {"f32": 0, "f16": 1, "bf16": 30}
-    h = {"lib": lib, "stream": torch.cuda.current_stream().cuda_stream}
+    h = {"lib": lib, "device": torch.cuda.current_device()}
     space = lambda n: torch.empty(max(int(n), 16), dtype=torch.uint8, device="cuda")  # noqa: E731
     if op == "select":
         rows = c["n_seq"] * c["n_beam"]
@@ -304,7 +304,7 @@ def _checked(rc):
 
 def _run_own(s):
     h, c = s["handle"], s["case"]
-    op, lib, ref, stream = c["op"], h["lib"], ctypes.byref, h["stream"]
+    op, lib, ref, stream = c["op"], h["lib"], ctypes.byref, torch._C._cuda_getCurrentRawStream(h["device"])      # as torch.cuda.current_stream().cuda_stream, 3 us less
     if op == "select":
         _checked(lib.b200_beam_select(ref(h["args"]), stream))
         return h["out"]

@@ -811,28 +811,30 @@ extern "C" int b200_paged_store(const b200_page_pool * pool, const b200_paged_at
 template <typename Q, typename KV, int D>
 static cudaError_t pa_launch(PaArgs & k, const PaNew & x, int n_seq, int64_t n_items, cudaStream_t st) {
     cudaError_t e;
-    const int64_t rows = (int64_t) k.max_new * k.n_head;
-    const dim3 join((unsigned) (rows < 16384 ? (rows + 3) / 4 : 4096), (unsigned) n_seq);
-    if (k.tile_rows != PA_ROWS) {
-        e = pa_tc_launch(k, D, std::is_same<KV, __half>::value ? B200_TYPE_F16 : B200_TYPE_BF16, n_items, st);
-        if (e != cudaSuccess || k.n_split == 1) return e;
-        e = launch_chained(k_paged_join_tc<Q, D>, dim3((unsigned) (n_items - k.n_whole), (unsigned) k.tile_rows / 16), dim3(128), 0, st, k);
-    } else {
-        const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
-        const dim3 grid = k.stream ? dim3((unsigned) k.stream) : dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) n_seq);
-        // few items, one CTA per SM at most: eight warps share an item's blocks (5 beams of 20 heads, 431 keys, f32: 11.2 -> 8.8 us)
-        if (!k.stream && n_items <= 148) {
-            e = allow_once<k_paged_attn<Q, KV, D, 8>>(4 * 8 * PA_BLOCK);
-            if (e == cudaSuccess) e = launch_chained(k_paged_attn<Q, KV, D, 8>, grid, dim3(256), 4 * 8 * PA_BLOCK, st, k, x);
-        } else {
-            e = allow_once<k_paged_attn<Q, KV, D, PA_WARPS>>(4 * PA_WARPS * PA_BLOCK);
-            if (e == cudaSuccess) e = launch_chained(k_paged_attn<Q, KV, D, PA_WARPS>, grid, dim3(32 * PA_WARPS), 4 * PA_WARPS * PA_BLOCK, st, k, x);
+    if constexpr (std::is_same<Q, KV>::value) {            // (f32 queries never go there)
+        if (k.tile_rows != PA_ROWS) {
+            e = pa_tc_launch(k, D, std::is_same<KV, __half>::value ? B200_TYPE_F16 : B200_TYPE_BF16, n_items, st);
+            if (e != cudaSuccess || k.n_split == 1) return e;
+            e = launch_chained(k_paged_join_tc<Q, D>, dim3((unsigned) (n_items - k.n_whole), (unsigned) k.tile_rows / 16), dim3(128), 0, st, k);
+            if (e == cudaSuccess) B200_LAUNCHED();
+            return e;
         }
-        if (e != cudaSuccess) return e;
-        B200_LAUNCHED();
-        if (!k.stream) return cudaGetLastError();
-        e = launch_chained(k_paged_join<Q, D>, join, dim3(128), 0, st, k);
     }
+    const int64_t tiles = ((int64_t) k.max_new * k.group + PA_ROWS - 1) / PA_ROWS;
+    const dim3 grid = k.stream ? dim3((unsigned) k.stream) : dim3((unsigned) tiles, (unsigned) k.n_head_kv, (unsigned) n_seq);
+    // few items, one CTA per SM at most: eight warps share an item's blocks (5 beams of 20 heads, 431 keys, f32: 11.2 -> 8.8 us)
+    if (!k.stream && n_items <= 148) {
+        e = allow_once<k_paged_attn<Q, KV, D, 8>>(4 * 8 * PA_BLOCK);
+        if (e == cudaSuccess) e = launch_chained(k_paged_attn<Q, KV, D, 8>, grid, dim3(256), 4 * 8 * PA_BLOCK, st, k, x);
+    } else {
+        e = allow_once<k_paged_attn<Q, KV, D, PA_WARPS>>(4 * PA_WARPS * PA_BLOCK);
+        if (e == cudaSuccess) e = launch_chained(k_paged_attn<Q, KV, D, PA_WARPS>, grid, dim3(32 * PA_WARPS), 4 * PA_WARPS * PA_BLOCK, st, k, x);
+    }
+    if (e != cudaSuccess) return e;
+    B200_LAUNCHED();
+    if (!k.stream) return cudaGetLastError();
+    const int64_t rows = (int64_t) k.max_new * k.n_head;
+    e = launch_chained(k_paged_join<Q, D>, dim3((unsigned) (rows < 16384 ? (rows + 3) / 4 : 4096), (unsigned) n_seq), dim3(128), 0, st, k);
     if (e == cudaSuccess) B200_LAUNCHED();
     return e;
 }

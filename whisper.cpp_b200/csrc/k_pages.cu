@@ -67,7 +67,7 @@ __device__ __forceinline__ void pg_copy(const b200_page_pool & pool, int n, int6
 #define PG_SMALL   (160 * 1024)   // bytes of shared memory that a small state may take
 #define PG_FUSED   3000           // words of tables and counts up to which every CTA works them out for itself (5 beams, pages of 16, 8 layers of 20 heads; us
                                   // with and without: 1 sequence of 230 tokens 7.5, 9.1; 8 of 400 10.4, 11.4; 16 of 400 16.4, 15.7; 24 of 400 19.3, 17.5)
-#define PG_HEADER  8              // workspace words before the lists: [0] copies, [1] tokens per whole page, [2] see k_pages_compact
+#define PG_HEADER  8              // workspace words before the lists: [0] copies, [2] see k_pages_compact
 
 struct PgWork { int32_t * head; int32_t * copies; int32_t * a; int32_t * b; };    // copies: (src, dst, tokens) each
 
@@ -261,7 +261,7 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
         for (int p = gtid; p < n_pages; p += all) to.refs[p] = refs[p];
         for (int i = gtid; i < n_rows; i += all) to.lens[i] = from.lens[i];
         for (int c = gtid; c < cells; c += all) to.tables[c] = tables[c];
-        if (gtid == 0) { status[0] = missing; status[1] = 0; w.head[0] = 0; w.head[1] = ps; }
+        if (gtid == 0) { status[0] = missing; status[1] = 0; w.head[0] = 0; }
         return;
     }
     for (int p = p0, f = free_before; p < p1 && f < wanted; p += PG_BATCH) {
@@ -298,7 +298,7 @@ k_pages_update(PgState from, PgState to, int n_rows, int width, int n_pages, int
             l[1] = pg_get<SMALL>(&w.a[l[1]]);
             if (SMALL && out) { w.copies[3 * c] = l[0]; w.copies[3 * c + 1] = l[1]; w.copies[3 * c + 2] = l[2]; }
         }
-        if (tid == 0 && out) { status[0] = 0; status[1] = n_copy; w.head[0] = n_copy; w.head[1] = ps; }
+        if (tid == 0 && out) { status[0] = 0; status[1] = n_copy; w.head[0] = n_copy; }
     }
     if (SMALL && fused) {
         __syncthreads();
@@ -380,7 +380,7 @@ k_pages_compact(PgState from, PgState to, int n_rows, int width, int n_pages, in
         r += n != 0;
     }
     for (int c = gtid; out && c < moves; c += all) { w.copies[3 * c] = pg_get<SMALL>(&w.a[low + c]); w.copies[3 * c + 1] = pg_get<SMALL>(&w.b[c]); w.copies[3 * c + 2] = ps; }
-    if (gtid == 0 && out) { status[0] = err ? -1 : 0; status[1] = moves; w.head[0] = moves; w.head[1] = ps; }
+    if (gtid == 0 && out) { status[0] = err ? -1 : 0; status[1] = moves; w.head[0] = moves; }
     pg_sync<SMALL>(cl);
     for (int i = gtid; out && i < n_rows; i += all) to.lens[i] = lens[i];
     for (int c0 = gtid; out && c0 < cells; c0 += PG_BATCH * all) {

@@ -25,6 +25,17 @@ def pytest_configure(config):
     sys.path.insert(0, ROOT)
 
 
+# read the symbols of the plugin, which build() leaves out without a whisper.cpp checkout
+NEED_PLUGIN = ("test_kernel_library_exports_every_declared_symbol", "test_plugin_exports_entry_points_and_refuses_without_gpu")
+
+
+def pytest_collection_modifyitems(items):
+    if not os.path.exists(os.path.join(PKG, "libggml-b200.so")):
+        for item in items:
+            if item.name in NEED_PLUGIN:
+                item.add_marker(pytest.mark.skip(reason="libggml-b200.so was not built (it needs a whisper.cpp checkout)"))
+
+
 @pytest.fixture(scope="session")
 def pkg():
     return load_pkg()

@@ -261,7 +261,7 @@ int b200_topk_rows(const float * const * rows, b200_topk_result * const * out, i
  * None of them allocates, synchronises or keeps anything between calls; all may be captured into a graph.  Scratch memory
  * comes from the caller (16-byte aligned); two calls that may overlap on the device need a scratch area each.  How much a call
  * needs depends on how its work is dealt out: a smaller call can need more than a larger one, so ask for every size that is used
- * (b200_paged_attn: never more than 21 MB). */
+ * (b200_paged_attn: an area of 21 MB serves every call). */
 
 /* The next beams of every sequence.  Row r = sequence * n_beam + beam has n_vocab logits x (F32, F16 or BF16; nb_row bytes
  * between rows) and an accumulated score.  Candidates are
@@ -276,7 +276,8 @@ int b200_topk_rows(const float * const * rows, b200_topk_result * const * out, i
  * (b200_beam_reorder leaves such a beam as it is; for b200_pages_update, which counts rows over all sequences, it is row_parent = the row itself with
  * keep = n_new = 0, and never sequence * n_beam - 1, the row before the sequence).
  * score_out / done_out may be score / done.  n_beam <= B200_BEAM_MAX, n_beam * n_vocab < 2^31, n_beam * ceil(n_vocab / 8192) <= 32768, any
- * alignment of the rows that suits their type.  done, banned may be NULL. */
+ * alignment of the rows that suits their type.  done, banned may be NULL.  Rules that weigh tokens against each other (whisper's timestamps against text)
+ * are no mask: they change the logits before this call. */
 #define B200_BEAM_MAX 32
 typedef struct {
     const void * logits; int type; int64_t nb_row; int64_t n_vocab; int n_seq, n_beam;

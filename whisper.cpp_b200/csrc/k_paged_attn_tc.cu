@@ -44,7 +44,8 @@ extern "C" int b200_paged_attn_status(void) {
 }
 
 // powers of two: how far the maximum may run ahead of the reference point, the weight at the reference point; and the factor that takes the latter out
-// (f16, 8 and 2^7 against 4 and 2^11: no difference in time on a chunk of 2048 over 16k keys, 16 times the step for the smallest weights)
+// (f16, 8 and 2^7 against 4 and 2^11: no difference in time on a chunk of 2048 over 16k keys, 16 times the step for the smallest weights; 8 and no raise is 1%
+// faster, 1107 against 1118 us, and loses them)
 template <typename T> struct PtLag { static constexpr float lag = 8.0f, raise = 0.0f, lower = 1.0f; };
 template <> struct PtLag<__half> { static constexpr float lag = 4.0f, raise = 11.0f, lower = 1.0f / 2048.0f; };
 

@@ -312,7 +312,7 @@ int64_t b200_pages_workspace(int64_t n_rows, int64_t n_pages);
 
 /* Row i becomes the first keep[i] tokens of row parent[i], with room for n_new[i] more - fork (parent != i), truncate
  * (keep < length), free (keep = n_new = 0), grow (n_new > 0), in any mix.  `from` is read, `to` (same n_rows and table_stride) is written;
- * it must not overlap `from` nor the other inputs (a program keeps two states and swaps them).  Whole pages are shared.  A partly filled last page that will be written
+ * neither its arrays nor status nor the workspace may overlap one another or an input (a program keeps two states and swaps them).  Whole pages are shared.  A partly filled last page that will be written
  * (n_new > 0) stays where it is for one row only: if nobody else holds it, or, among several such rows and no other holder, for
  * the first of them; the others get a new page with a copy of its keep[i] % page_size tokens, in every layer of the pool.  New
  * pages are those free in `from`, lowest number first, row by row (within a row: first the copy, then the following pages);
@@ -326,8 +326,8 @@ int b200_pages_update(const b200_page_pool * pool, const b200_page_state * from,
                       const int32_t * keep, const int32_t * n_new, int32_t * status, void * workspace, int64_t workspace_bytes, void * stream);
 
 /* With L pages in use, the i-th used page numbered L or more moves to the i-th free page below L.  `to` receives tables, lens
- * and refs in the new numbers, remap[p] the new number of page p (-1: free) for holders that the tables do not show.  `from` and
- * `to` must not overlap; the pages themselves move within the pool.  status as above ([0]: 0, or -1 for a table entry out of
+ * and refs in the new numbers, remap[p] the new number of page p (-1: free) for holders that the tables do not show.  What is written
+ * must not overlap itself or `from`; the pages themselves move within the pool.  status as above ([0]: 0, or -1 for a table entry out of
  * range or on a free page; [1]: pages moved). */
 int b200_pages_compact(const b200_page_pool * pool, const b200_page_state * from, const b200_page_state * to, int32_t * remap,
                        int32_t * status, void * workspace, int64_t workspace_bytes, void * stream);

@@ -43,3 +43,26 @@ def test_attention_and_store_refuse_an_unaligned_status(K, pkg):
               q_start=P, n_tok=4, n_seq=2, n_head=4, max_new=2, max_len=20, causal=1, scale=0.1, workspace=P, workspace_bytes=1 << 15, status=P + 2)
     for f in (K.b200_paged_attn, K.b200_paged_store):
         assert f(C.byref(pool(pkg)), C.byref(changed(pkg.PagedAttnArgs, ok)), None) == ERR
+
+
+def test_pages_refuse_results_that_overlap_what_is_read(K, pkg):
+    """Every CTA reads the inputs for itself while the results are written."""
+    n = K.b200_pages_workspace(3, 10)
+    at = dict(tables=P, lens=P + 1024, refs=P + 2048)
+    to = dict(tables=P + 4096, lens=P + 5120, refs=P + 6144)
+    rest = dict(parent=P + 512, keep=P + 600, n_new=P + 700, status=P + 800, remap=P + 3072, ws=P + 8192)
+
+    def call(f=at, t=to, **kw):
+        a = dict(rest, **kw)
+        f, t = (pkg.PageState(n_rows=3, table_stride=5, **s) for s in (f, t))
+        pl = pool(pkg)
+        return (K.b200_pages_update(C.byref(pl), C.byref(f), C.byref(t), a["parent"], a["keep"], a["n_new"], a["status"], a["ws"], n, None),
+                K.b200_pages_compact(C.byref(pl), C.byref(f), C.byref(t), a["remap"], a["status"], a["ws"], n, None))
+    for name, size in (("tables", 60), ("lens", 12), ("refs", 40)):
+        for other, at_other in list(at.items()) + [(k, v) for k, v in to.items() if k != name]:
+            assert call(t=dict(to, **{name: at_other})) == (ERR, ERR), (name, other)
+        assert call(status=to[name] + size - 4) == (ERR, ERR) and call(status=at[name]) == (ERR, ERR), name
+        assert call(ws=to[name] // 16 * 16) == (ERR, ERR) and call(remap=to[name] + size - 4)[1] == ERR and call(remap=at[name])[1] == ERR, name
+        for k in ("parent", "keep", "n_new"):
+            assert call(**{k: to[name] + size - 4})[0] == ERR, (name, k)
+    assert call(status=rest["keep"] + 4)[0] == ERR and call(status=rest["ws"]) == (ERR, ERR) and call(status=rest["remap"] + 8)[1] == ERR

@@ -459,18 +459,29 @@ static cudaError_t pg_launch(int64_t n_rows, int64_t width, int64_t n_pages, con
     return cudaLaunchKernelEx(&cfg, fits ? SMALL_KERNEL : LARGE_KERNEL, std::forward<Args>(args)..., *pool, *fused);
 }
 
+// No output may overlap another one or an input: every CTA of a launch reads the inputs for itself, some of them when others already write.
+struct PgSpan { const void * p; int64_t bytes; };
+template <int OUT, int IN> static bool pg_apart(const PgSpan (&out)[OUT], const PgSpan (&in)[IN]) {
+    auto meet = [](const PgSpan & a, const PgSpan & b) {
+        return a.p && b.p && a.bytes > 0 && b.bytes > 0 && (uintptr_t) a.p < (uintptr_t) b.p + b.bytes && (uintptr_t) b.p < (uintptr_t) a.p + a.bytes;
+    };
+    for (int i = 0; i < OUT; ++i) {
+        for (int j = 0; j < i; ++j) if (meet(out[i], out[j])) return false;
+        for (int j = 0; j < IN; ++j) if (meet(out[i], in[j])) return false;
+    }
+    return true;
+}
+
 // what update and compact ask of their states
 static bool pg_states_ok(const b200_page_state * from, const b200_page_state * to, int64_t n_pages, int64_t ps) {
     if (!from || !to || from->n_rows < 0 || from->n_rows > PG_MAX_ROWS || to->n_rows != from->n_rows || n_pages > PG_MAX_PAGES) return false;
-    auto apart = [](const void * a, int64_t na, const void * b, int64_t nb) { return (const char *) a + na <= (const char *) b || (const char *) b + nb <= (const char *) a; };
-    if (!from->refs || !to->refs || ((uintptr_t) from->refs | (uintptr_t) to->refs) % 4 || !apart(from->refs, 4 * n_pages, to->refs, 4 * n_pages)) return false;
+    if (!from->refs || !to->refs || ((uintptr_t) from->refs | (uintptr_t) to->refs) % 4) return false;
     if (from->n_rows == 0) return true;
     if (from->table_stride < 1 || to->table_stride != from->table_stride || !from->tables || !to->tables || !from->lens || !to->lens) return false;
     const int64_t width = from->table_stride;
     if (((uintptr_t) from->tables | (uintptr_t) from->lens | (uintptr_t) to->tables | (uintptr_t) to->lens) % 4) return false;
     if (width >= (1ll << 30)) return false;
-    if (width * from->n_rows >= (1ll << 30) || width * ps >= (1ll << 31)) return false;
-    return apart(from->tables, 4 * from->table_stride * from->n_rows, to->tables, 4 * to->table_stride * to->n_rows) && apart(from->lens, 4 * from->n_rows, to->lens, 4 * to->n_rows);
+    return width * from->n_rows < (1ll << 30) && width * ps < (1ll << 31);
 }
 
 extern "C" int64_t b200_pages_workspace(int64_t n_rows, int64_t n_pages) {
@@ -489,6 +500,9 @@ extern "C" int b200_pages_update(const b200_page_pool * pool, const b200_page_st
     pg_layout(&w, workspace, from->n_rows, pool->n_pages);
     const PgState f = { from->tables, from->lens, from->refs }, t = { to->tables, to->lens, to->refs };
     const int width = from->n_rows ? (int) from->table_stride : 0;
+    const int64_t rows = 4 * from->n_rows, cells = rows * width, pages = 4ll * pool->n_pages;
+    if (!pg_apart({ { t.tables, cells }, { t.lens, rows }, { t.refs, pages }, { status, 8 }, { workspace, b200_pages_workspace(from->n_rows, pool->n_pages) } },
+                  { { f.tables, cells }, { f.lens, rows }, { f.refs, pages }, { parent, rows }, { keep, rows }, { n_new, rows } })) return B200_ERR_ARG;
     const cudaStream_t st = as_stream(stream);
     bool fused;
     cudaError_t e = pg_launch<k_pages_update<true>, k_pages_update<false>>(from->n_rows, width, pool->n_pages, pool, data, from->n_rows, &fused, st, f, t, (int) from->n_rows, width, pool->n_pages, pool->page_size, parent, keep, n_new, status, w);
@@ -507,6 +521,9 @@ extern "C" int b200_pages_compact(const b200_page_pool * pool, const b200_page_s
     pg_layout(&w, workspace, from->n_rows, pool->n_pages);
     const PgState f = { from->tables, from->lens, from->refs }, t = { to->tables, to->lens, to->refs };
     const int width = from->n_rows ? (int) from->table_stride : 0;
+    const int64_t rows = 4 * from->n_rows, cells = rows * width, pages = 4ll * pool->n_pages;
+    if (!pg_apart({ { t.tables, cells }, { t.lens, rows }, { t.refs, pages }, { remap, pages }, { status, 8 }, { workspace, b200_pages_workspace(from->n_rows, pool->n_pages) } },
+                  { { f.tables, cells }, { f.lens, rows }, { f.refs, pages } })) return B200_ERR_ARG;
     const cudaStream_t st = as_stream(stream);
     bool fused;
     cudaError_t e = pg_launch<k_pages_compact<true>, k_pages_compact<false>>(from->n_rows, width, pool->n_pages, pool, data, pool->n_pages / 2 + 1, &fused, st, f, t, (int) from->n_rows, width, pool->n_pages, pool->page_size, remap, status, w);

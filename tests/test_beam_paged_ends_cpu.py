@@ -50,7 +50,7 @@ def test_pages_refuse_results_that_overlap_what_is_read(K, pkg):
     n = K.b200_pages_workspace(3, 10)
     at = dict(tables=P, lens=P + 1024, refs=P + 2048)
     to = dict(tables=P + 4096, lens=P + 5120, refs=P + 6144)
-    rest = dict(parent=P + 512, keep=P + 600, n_new=P + 700, status=P + 800, remap=P + 3072, ws=P + 8192)
+    rest = dict(parent=P + 512, keep=P + 600, n_new=P + 700, status=P + 800, remap=P + 3328, ws=P + 8192)
 
     def call(f=at, t=to, **kw):
         a = dict(rest, **kw)
